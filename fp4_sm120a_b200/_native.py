@@ -7,10 +7,20 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_size_t, c_uint32, c_void_p, POINTER
+from ctypes import (c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p,
+                    POINTER)
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnvfp4_b200.so"
+
+
+class AdamWTensor(ctypes.Structure):
+    """nvfp4_adamw_tensor."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p),
+                ("exp_avg_sq", c_void_p), ("exp_avg_scale", c_void_p),
+                ("exp_avg_sq_scale", c_void_p), ("copy", c_void_p), ("n", c_uint64),
+                ("offset", c_uint64), ("weight_decay", c_double)]
+
 
 # Every symbol declared in include/nvfp4_b200.h with its argument types.
 SIGNATURES: dict[str, tuple[list, object]] = {
@@ -65,6 +75,25 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                                                    c_void_p, c_void_p, c_void_p, c_void_p,
                                                    c_uint32, c_void_p, c_int, c_int, c_int,
                                                    c_int, c_int, c_void_p], c_int),
+    "nvfp4_gemm": ([c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                    c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_int,
+                    c_void_p, c_int64, c_void_p, c_uint32, c_void_p], c_int),
+    "nvfp4_gemm_dact_workspace_bytes": ([c_int64, c_int64, c_int64], c_size_t),
+    "nvfp4_gemm_dact": ([c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                         c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int,
+                         c_void_p, c_void_p, c_void_p, c_size_t, c_uint32, c_void_p], c_int),
+    "nvfp4_layernorm_fwd": ([c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+                             c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                             c_void_p], c_int),
+    "nvfp4_layernorm_bwd_workspace_bytes": ([c_int64, c_int64], c_size_t),
+    "nvfp4_layernorm_bwd": ([c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                             c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p,
+                             c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
+    "nvfp4_adamw_step": ([POINTER(AdamWTensor), c_int, c_int, c_int, c_int, c_double, c_double,
+                          c_double, c_double, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_void_p], c_int),
+    "nvfp4_adamw_unpack_state": ([c_void_p, c_void_p, c_size_t, c_int, c_void_p, c_int,
+                                  c_void_p], c_int),
 }
 
 _lib = None

@@ -8,6 +8,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,7 +19,8 @@ LIB = PKG / "libnvfp4_b200.so"
 OBJDIR = PKG / "_build"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-SOURCES = ["rht_gemm_sm100.cu", "sr_kernels.cu", "fp8_kernels.cu", "fp8_kernels_loose.cu"]
+SOURCES = ["rht_gemm_sm100.cu", "sr_kernels.cu", "fp8_kernels.cu", "fp8_kernels_loose.cu",
+           "gemm_nvfp4_sm100.cu", "layernorm.cu", "adamw.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
@@ -29,31 +31,39 @@ FLAGS = [
 
 
 def _deps() -> list[Path]:
-    return [CSRC / s for s in SOURCES] + sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + \
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + \
         sorted(INCLUDE.glob("*.h")) + sorted(INCLUDE.glob("*.cuh"))
 
 
+def _stale(target: Path, deps: list[Path]) -> bool:
+    return not target.exists() or any(d.stat().st_mtime > target.stat().st_mtime for d in deps)
+
+
 def needs_build() -> bool:
-    if not LIB.exists():
-        return True
-    t = LIB.stat().st_mtime
-    return any(d.stat().st_mtime > t for d in _deps())
+    return _stale(LIB, _deps())
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
     OBJDIR.mkdir(exist_ok=True)
-    objs = []
-    for src in SOURCES:
+
+    headers = [d for d in _deps() if d.suffix != ".cu"]
+
+    def compile_one(src: str) -> str:
         obj = OBJDIR / (Path(src).stem + ".o")
+        if not force and not _stale(obj, [CSRC / src, *headers]):
+            return str(obj)
         cmd = [NVCC, *FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode != 0:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed on {src}")
-        objs.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", *objs, "-o", str(tmp)]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,0 +1,937 @@
+// Product of two NVFP4 matrices with a fused epilogue, for B200 (sm_100a).
+//
+//   z[i, j] = S_a S_b sum_k (a[i, k] sfa[i, k / 16]) (b[j, k] sfb[j, k / 16]) + bias[j]
+//   nvfp4_gemm        D = act(z) + residual, aux = z
+//   nvfp4_gemm_dact   D = z act'(aux), dbias[j] = sum_i D[i, j]
+//
+// with S = 1 / global_encode_scale(amax) of each operand, the scale that the
+// casts of this library divide out.  Both operands are what the casts write:
+// packed E2M1 rows along k and row-major E4M3 scales of 16-element blocks.
+//
+// The products run on the tensor cores' block-scaled form (kind::mxf4nvf4,
+// one E4M3 scale per 16 elements, fp32 accumulators in TMEM): code products
+// and scales are exact there, only the accumulation rounds.
+//
+// Orientation: the n side (weights) lies along the 128 TMEM lanes and the m
+// side (tokens) along the accumulator's columns.  A short m then costs a
+// narrow column tile rather than an empty lane tile, bias is one register a
+// thread, a warp's stores cover 32 consecutive elements of a row of D, and a
+// column sum of D (the bias gradient) never leaves a thread.
+//
+// Work: output tiles of 128 (n) x TN (m), persistent grid, warp-specialised:
+//   warps 0-7   epilogue: two groups of four warps, each half of the columns
+//   warp  8     TMA producer: 128-byte k-slices (256 codes) of both operands
+//               into a ring of 128-byte-swizzled stages
+//   warp  9     MMA issuer: copies a stage's scales to TMEM (tcgen05.cp),
+//               issues four K = 64 MMAs; owns the TMEM columns
+//   warps 10-12 scale loaders: the casts' row-major scales into the 32 x 16
+//               byte atoms that tcgen05.cp spreads over the lanes.  A lane
+//               takes 16 bytes (one k-slice) of rows l, l + 32, l + 64, l + 96,
+//               so the transpose is a choice of registers.
+// Few tiles (short m): the k range is split over a cluster of up to 8 CTAs,
+// whose partial tiles meet in distributed shared memory and are added in rank
+// order (no atomics: results repeat bit for bit).
+// Every wait is bounded; a kernel that gives up records an error word, waits
+// for its own copies and MMAs, frees TMEM and returns.
+#include <cstdint>
+#include <mutex>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "element_io.cuh"
+#include "launch_common.h"
+#include "nvfp4_b200.h"
+#include "nvfp4_device.cuh"
+
+namespace nvfp4 {
+namespace gemm {
+
+__device__ uint32_t g_gemm_error_word;
+
+constexpr int kTileF = 128;                  // n side: TMEM lanes
+constexpr int kSliceK = 256;                 // codes per k-slice (128 bytes)
+constexpr int kSteps = kSliceK / 64;         // MMAs per k-slice
+constexpr int kEpiWarps = 8;
+constexpr int kEpiThreads = 32 * kEpiWarps;
+constexpr int kWarpTma = 8, kWarpMma = 9, kWarpScales = 10;
+constexpr int kThreads = 32 * 13;
+constexpr uint32_t kAtomBytes = 512;         // scales of 128 rows x one MMA step
+constexpr uint32_t kSmemMax = 227 * 1024;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr int kMaxSplit = 8;
+
+// Tile widths and what follows from them.
+template <int TN>
+struct Tile {
+  static constexpr int kAtomsT = (TN + 127) / 128;           // scale atoms per step, m side
+  static constexpr uint32_t kBytesF = kTileF * 128;
+  static constexpr uint32_t kBytesT = TN * 128;
+  static constexpr uint32_t kBytesSf = kSteps * (1 + kAtomsT) * kAtomBytes;
+  static constexpr uint32_t kStageBytes = kBytesF + kBytesT + kBytesSf;
+  // TN >= 128: one CTA per SM with all of its shared memory.  Narrow tiles
+  // (short m) leave room for two, so that a split that does not divide the
+  // SMs evenly still runs in one wave.
+  static constexpr int kCtasPerSm = TN >= 128 ? 1 : 2;
+  static constexpr uint32_t kBudget = kSmemMax / kCtasPerSm - 2048;
+  static constexpr int kStagesRaw = (int)(kBudget / kStageBytes);
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
+  static constexpr int kAccStages = TN <= 128 ? 2 : 1;
+  static constexpr uint32_t kSfCols = kSteps * 4 * (1 + kAtomsT);   // TMEM columns of a slice's scales
+  static constexpr uint32_t kColsUsed = kAccStages * TN + 2 * kSfCols;
+  static constexpr uint32_t kTmemCols = kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;   // + alignment
+  static constexpr int kSfWarps = 1 + kAtomsT;
+  static_assert(kStages >= 3, "the scale columns of slice g - 2 are checked through its stage");
+  static_assert(kColsUsed <= 512, "TMEM");
+  static_assert(kTmemCols * kCtasPerSm <= 512, "TMEM of all CTAs of an SM");
+  // Instruction descriptor, kind::mxf4nvf4: E2M1 operands, both K-major,
+  // UE4M3 scales, N = TN, M = 128.
+  static constexpr uint32_t kIdesc =
+      (1u << 7) | (1u << 10) | ((uint32_t)(TN / 8) << 17) | ((uint32_t)(kTileF / 16) << 24);
+};
+
+enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
+
+struct Params {
+  int m, n, k;
+  int slices;                 // ceil(k / 256)
+  int tiles_f, tiles_t;
+  const uint8_t* sf_f;        // scales of the n side (B), pitch k / 16
+  const uint8_t* sf_t;        // scales of the m side (A)
+  int sf_pitch;
+  int sf_width_f, sf_width_t;   // bytes per scale load: 16, 4 or 1
+  const float* amax_f;
+  const float* amax_t;
+  void* d;
+  int64_t ldd;
+  const void* bias;
+  int bias_dtype;
+  const void* res;            // forward: residual; backward: the activation's argument
+  int64_t ldr;
+  void* aux;
+  int64_t ldaux;
+  int act;
+  float* dbias_partial;       // [partial rows][n]
+  uint32_t* amax;
+};
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                     uint32_t err) {
+  return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, err, &g_gemm_error_word);
+}
+
+// tcgen05.mma, block-scaled: D (+)= (A sfa) (B sfb)^T, one E4M3 scale for each
+// 16 elements of a row.
+__device__ __forceinline__ void mma_nvfp4(uint32_t d, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
+      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 bytes to 32 lanes x 4 columns, repeated for the four warps' lanes.
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z,
+                                       uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z),
+               "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ void sts_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// 16 scale bytes (one k-slice) of a row; bytes behind the row's end are zero.
+__device__ __forceinline__ uint4 load_scales(const uint8_t* sf, int pitch, int width, int row,
+                                             int rows, int slice) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  if (row < rows) {
+    const uint8_t* p = sf + (int64_t)row * pitch + slice * 16;
+    const int left = pitch - slice * 16;
+    if (width == 16) {
+      const uint4 q = *reinterpret_cast<const uint4*>(p);
+      return q;
+    }
+    if (width == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * i < left) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < left) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// COLS consecutive fp32 columns of this thread's TMEM lane.
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[COLS]) {
+  if constexpr (COLS == 32) {
+    tmem_ld_32cols(taddr, v);
+  } else if constexpr (COLS == 16) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  } else {
+    static_assert(COLS == 8, "8, 16 or 32 columns");
+    uint32_t r[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+
+// 1 / (1 + exp(-x)) from the hardware's exponential and reciprocal.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+constexpr float kGeluC = 1.5957691216057308f;    // 2 sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
+// 0.5 z (1 + tanh(c z (1 + a z^2))) = z sigmoid(2 c z (1 + a z^2))
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == kRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if constexpr (ACT == kGelu) return z * sigmoid(kGeluC * z * (1.0f + kGeluA * z * z));
+  if constexpr (ACT == kSilu) return z * sigmoid(z);
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+  if constexpr (ACT == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+  // Beyond |z| = 64 both slopes are 0 or 1 to the last bit; the clamp keeps
+  // powers of a huge argument from overflowing (and lets NaN through).
+  const float c = fmax_nan(fmin_nan(z, 64.0f), -64.0f);
+  if constexpr (ACT == kGelu) {
+    const float q = sigmoid(kGeluC * c * (1.0f + kGeluA * c * c));
+    return q + c * q * (1.0f - q) * kGeluC * (1.0f + 3.0f * kGeluA * c * c);
+  }
+  if constexpr (ACT == kSilu) {
+    const float q = sigmoid(c);
+    return q + c * q * (1.0f - q);
+  }
+  return 1.0f;
+}
+
+// A thread's share of a tile: one feature (lane) and COLS columns from
+// column c0 on, the accumulator's values in v.
+struct Out {
+  float alpha, bias;
+  float dbias;
+  uint32_t top;
+};
+
+template <typename T, bool DACT, int ACT, int COLS>
+__device__ __forceinline__ void finish_act(const Params& p, Out& o, float (&v)[COLS],
+                                           const float (&r)[COLS], int f, int t0, int step,
+                                           int count) {
+  T* d = reinterpret_cast<T*>(p.d) + f;
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    if (j < count) {
+      const int64_t t = t0 + (int64_t)j * step;
+      float x;
+      if constexpr (DACT) {
+        x = v[j] * o.alpha * slope<ACT>(r[j]);
+        o.dbias += x;
+      } else {
+        const float z = v[j] * o.alpha + o.bias;
+        if (p.aux) reinterpret_cast<T*>(p.aux)[t * p.ldaux + f] = from_f32<T>(z);
+        x = activate<ACT>(z) + r[j];
+      }
+      const T s = from_f32<T>(x);
+      d[t * p.ldd] = s;
+      o.top = max(o.top, __float_as_uint(to_f32(s)) & 0x7FFFFFFFu);
+    }
+  }
+}
+
+// Epilogue of COLS columns (tokens t0, t0 + step, ...; the first `count` are real).
+template <typename T, bool DACT, int COLS>
+__device__ __forceinline__ void finish(const Params& p, Out& o, float (&v)[COLS], int f, int t0,
+                                       int step, int count) {
+  float r[COLS];
+  const T* res = reinterpret_cast<const T*>(p.res) + f;
+#pragma unroll
+  for (int j = 0; j < COLS; ++j)
+    r[j] = (DACT || p.res) && j < count ? to_f32(res[(t0 + (int64_t)j * step) * p.ldr]) : 0.0f;
+  switch (p.act) {
+    case kRelu: finish_act<T, DACT, kRelu, COLS>(p, o, v, r, f, t0, step, count); break;
+    case kGelu: finish_act<T, DACT, kGelu, COLS>(p, o, v, r, f, t0, step, count); break;
+    case kSilu: finish_act<T, DACT, kSilu, COLS>(p, o, v, r, f, t0, step, count); break;
+    default: finish_act<T, DACT, kNone, COLS>(p, o, v, r, f, t0, step, count); break;
+  }
+}
+
+__device__ __forceinline__ float load_bias(const Params& p, int f) {
+  if (!p.bias) return 0.0f;
+  if (p.bias_dtype == NVFP4_DTYPE_F32) return reinterpret_cast<const float*>(p.bias)[f];
+  if (p.bias_dtype == NVFP4_DTYPE_BF16)
+    return to_f32(reinterpret_cast<const __nv_bfloat16*>(p.bias)[f]);
+  return to_f32(reinterpret_cast<const __half*>(p.bias)[f]);
+}
+
+// Tiles in an order that keeps a wave's tiles near a square: groups of
+// kGroup column tiles, walked feature tile by feature tile.
+constexpr int kGroup = 8;
+__device__ __forceinline__ void tile_at(const Params& p, int i, int& tf, int& tt) {
+  const int per = kGroup * p.tiles_f;
+  const int g = i / per, in = i - g * per;
+  const int wide = min(kGroup, p.tiles_t - g * kGroup);
+  tf = in / wide;
+  tt = g * kGroup + in - tf * wide;
+}
+
+template <int TN, typename T, bool DACT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
+    k_gemm(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUtensorMap tm_t,
+           const Params p) {
+  using C = Tile<TN>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * C::kStages + 2 * C::kAccStages + 1];
+  __shared__ uint32_t tmem_holder;
+  __shared__ uint32_t abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar0 = smem_addr(bars);
+  auto full = [&](uint32_t s) { return bar0 + 8 * s; };
+  auto empty = [&](uint32_t s) { return bar0 + 8 * (C::kStages + s); };
+  auto acc_full = [&](uint32_t a) { return bar0 + 8 * (2 * C::kStages + a); };
+  auto acc_empty = [&](uint32_t a) { return bar0 + 8 * (2 * C::kStages + C::kAccStages + a); };
+  const uint32_t drain = bar0 + 8 * (2 * C::kStages + 2 * C::kAccStages);
+  volatile uint32_t* abort_flag = &abort_word;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 1 + C::kSfWarps);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < C::kAccStages; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), kEpiThreads);
+    }
+    mbar_init(drain, 1);
+    abort_word = 0u;
+    fence_barrier_init();
+  }
+  if (warp == kWarpTma && lane == 0) {
+    prefetch_tmap(&tm_f);
+    prefetch_tmap(&tm_t);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(smem_addr(&tmem_holder), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem_sf = tmem + C::kAccStages * TN;
+
+  // This CTA's tiles and k-slices.
+  const uint32_t split = SPLIT ? cluster_size() : 1u, rank = SPLIT ? cluster_rank() : 0u;
+  const int first = SPLIT ? (int)(blockIdx.x / split) : (int)blockIdx.x;
+  const int tiles = p.tiles_f * p.tiles_t;
+  const int stride = SPLIT ? tiles : (int)gridDim.x;
+  const int s_begin = SPLIT ? (int)((int64_t)p.slices * rank / split) : 0;
+  const int s_end = SPLIT ? (int)((int64_t)p.slices * (rank + 1) / split) : p.slices;
+
+  if (warp == kWarpTma) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride) {
+        int tf, tt;
+        tile_at(p, i, tf, tt);
+        for (int s = s_begin; s < s_end; ++s) {
+          if (!wait(empty(stage), phase ^ 1u, abort_flag, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = ring + stage * C::kStageBytes;
+          mbar_arrive_expect_tx(full(stage), C::kBytesF + C::kBytesT);
+          tma_load_2d(dst, &tm_f, full(stage), s * 128, tf * kTileF);
+          tma_load_2d(dst + C::kBytesF, &tm_t, full(stage), s * 128, tt * TN);
+          ++issued;
+          if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {
+        // Given up: the loads in flight land before the CTA ends.  (A stage
+        // whose scale loader gave up too never completes: its wait runs to the
+        // limit, far longer than a load takes.)
+        const uint32_t n = issued < (uint32_t)C::kStages ? issued : (uint32_t)C::kStages;
+        volatile uint32_t never = 0u;
+        for (uint32_t j = 0; j < n; ++j) {
+          if (stage == 0) { stage = C::kStages - 1; phase ^= 1u; } else { --stage; }
+          wait(full(stage), phase, &never, kErrTimeoutDrain);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kWarpMma) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, g = 0;
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride) {
+        if (!wait(acc_empty(acc), acc_phase ^ 1u, abort_flag, kErrTimeoutMma)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * TN;
+        for (int s = s_begin; s < s_end; ++s, ++g) {
+          if (!wait(full(stage), phase, abort_flag, kErrTimeoutMma)) { ok = false; break; }
+          // The scale columns of slice g alternate between two sets: the MMAs
+          // of slice g - 2 are done with this one when they have freed their
+          // stage.  (That stage's next phase needs a commit still to come, so
+          // the parity cannot have moved on.)
+          if (g >= 2) {
+            const uint32_t h = g - 2;
+            if (!wait(empty(h % C::kStages), (h / C::kStages) & 1u, abort_flag, kErrTimeoutMma)) {
+              ok = false;
+              break;
+            }
+          }
+          tc_fence_after();
+          const uint32_t base = ring + stage * C::kStageBytes;
+          const uint32_t sf = base + C::kBytesF + C::kBytesT;
+          const uint32_t sf_f = tmem_sf + (g & 1u) * C::kSfCols, sf_t = sf_f + kSteps * 4;
+          const int steps = min(kSteps, (p.k - s * kSliceK + 63) / 64);
+          for (int q = 0; q < steps; ++q) {
+            cp_scales(sf_f + 4 * q, umma_smem_desc(sf + q * kAtomBytes, 128, 128, 0));
+#pragma unroll
+            for (int b = 0; b < C::kAtomsT; ++b)
+              cp_scales(sf_t + 4 * (q * C::kAtomsT + b),
+                        umma_smem_desc(sf + (kSteps * (1 + b) + q) * kAtomBytes, 128, 128, 0));
+          }
+          for (int q = 0; q < steps; ++q)
+            mma_nvfp4(d, umma_smem_desc(base + 32 * q, 16, 1024, 2),
+                      umma_smem_desc(base + C::kBytesF + 32 * q, 16, 1024, 2), C::kIdesc,
+                      sf_f + 4 * q, sf_t + 4 * q * C::kAtomsT, s > s_begin || q > 0);
+          tc_commit(empty(stage));
+          if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        tc_commit(acc_full(acc));
+        if (++acc == (uint32_t)C::kAccStages) { acc = 0; acc_phase ^= 1u; }
+      }
+      // All issued work completes before TMEM is released.
+      tc_commit(drain);
+      volatile uint32_t never = 0u;
+      wait(drain, 0, &never, kErrTimeoutDrain);
+    }
+    __syncwarp();
+  } else if (warp >= kWarpScales) {
+    const int part = warp - kWarpScales;      // 0: n side; 1, 2: m side
+    if (part < C::kSfWarps) {
+      const bool f_side = part == 0;
+      const uint8_t* sf = f_side ? p.sf_f : p.sf_t;
+      const int width = f_side ? p.sf_width_f : p.sf_width_t;
+      const int rows = f_side ? p.n : p.m;
+      const int tile_rows = f_side ? kTileF : min(TN - (part - 1) * 128, 128);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      // Two k-slices of scales in flight ahead of the one being stored.
+      uint4 buf[3][4];
+      int li = first, ls = s_begin;           // next (tile, slice) to load
+      auto load = [&](uint4 (&b)[4]) {
+        if (li >= tiles) return;
+        int tf, tt;
+        tile_at(p, li, tf, tt);
+        const int row0 = f_side ? tf * kTileF : tt * TN + (part - 1) * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = q * 32 + lane;
+          b[q] = load_scales(sf, p.sf_pitch, width, r < tile_rows ? row0 + r : rows, rows, ls);
+        }
+        if (++ls == s_end) { ls = s_begin; li += stride; }
+      };
+      auto store = [&](const uint4 (&b)[4]) {
+        if (!__all_sync(0xFFFFFFFFu, wait(empty(stage), phase ^ 1u, abort_flag,
+                                          kErrTimeoutProducer))) {
+          ok = false;
+          return;
+        }
+        const uint32_t dst = ring + stage * C::kStageBytes + C::kBytesF + C::kBytesT +
+                             part * kSteps * kAtomBytes + lane * 16;
+        sts128(dst, b[0].x, b[1].x, b[2].x, b[3].x);
+        sts128(dst + kAtomBytes, b[0].y, b[1].y, b[2].y, b[3].y);
+        sts128(dst + 2 * kAtomBytes, b[0].z, b[1].z, b[2].z, b[3].z);
+        sts128(dst + 3 * kAtomBytes, b[0].w, b[1].w, b[2].w, b[3].w);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(stage));
+        if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
+      };
+      const int per_tile = s_end - s_begin;
+      const int64_t total =
+          first < tiles ? (int64_t)((tiles - first + stride - 1) / stride) * per_tile : 0;
+      load(buf[0]);
+      load(buf[1]);
+      for (int64_t j = 0; j < total && ok; j += 3) {
+        load(buf[2]);
+        store(buf[0]);
+        if (j + 1 < total && ok) { load(buf[0]); store(buf[1]); }
+        if (j + 2 < total && ok) { load(buf[1]); store(buf[2]); }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------- epilogue -------------------------------
+    const int group = warp >> 2, quad = warp & 3;
+    constexpr int kHalf = TN / 2;
+    constexpr int kMost = C::kCtasPerSm == 1 ? 32 : 16;   // what the registers hold
+    constexpr int kChunk = kHalf < kMost ? kHalf : kMost;
+    Out o;
+    o.top = 0u;
+    {
+      // The two amax are on their way while the first tile is computed.
+      const float ea = global_encode_scale(*p.amax_f), eb = global_encode_scale(*p.amax_t);
+      o.alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
+    }
+    uint32_t acc = 0, acc_phase = 0;
+    for (int i = first; i < tiles; i += stride) {
+      int tf, tt;
+      tile_at(p, i, tf, tt);
+      const int f = tf * kTileF + quad * 32 + lane;
+      if (!__all_sync(0xFFFFFFFFu, wait(acc_full(acc), acc_phase, abort_flag,
+                                        kErrTimeoutEpilogue)))
+        break;
+      tc_fence_after();
+      const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * TN + group * kHalf;
+      if constexpr (SPLIT) {
+        // The partial tile to shared memory, column by column (the ring is
+        // free: every load has been consumed).
+        for (int c = 0; c < kHalf; c += kChunk) {
+          float v[kChunk];
+          tmem_ld_cols<kChunk>(src + c, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j)
+            sts_f32(ring + (uint32_t)((group * kHalf + c + j) * kTileF + quad * 32 + lane) * 4,
+                    v[j]);
+        }
+      } else {
+        o.dbias = 0.0f;
+        if (f < p.n) o.bias = load_bias(p, f);
+        for (int c = 0; c < kHalf; c += kChunk) {
+          const int t0 = tt * TN + group * kHalf + c;
+          float v[kChunk];
+          tmem_ld_cols<kChunk>(src + c, v);
+          tc_wait_ld();
+          if (c + kChunk >= kHalf) {
+            // The last of this warp's columns are in registers.
+            tc_fence_before();
+            mbar_arrive(acc_empty(acc));
+          }
+          if (f < p.n) finish<T, DACT, kChunk>(p, o, v, f, t0, 1, p.m - t0);
+        }
+        if (DACT && p.dbias_partial && f < p.n)
+          p.dbias_partial[(int64_t)(tt * 2 + group) * p.n + f] = o.dbias;
+        if (++acc == (uint32_t)C::kAccStages) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+    if constexpr (!SPLIT) {
+      if (p.amax) {
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, o.top);
+        if (lane == 0 && top) atomicMax(p.amax, top);
+      }
+    }
+    tc_fence_before();
+  }
+  if constexpr (SPLIT) {
+    // Rank r adds the partial tiles' columns r, r + split, ... over the ranks
+    // in order.  A CTA that gave up still comes here (its values are void and
+    // the error word says so).
+    cluster_sync();
+    if (warp < kEpiWarps) {
+      int tf, tt;
+      tile_at(p, first, tf, tt);
+      const int group = warp >> 2, quad = warp & 3;
+      const int l = quad * 32 + lane, f = tf * kTileF + l;
+      Out o;
+      o.top = 0u;
+      o.dbias = 0.0f;
+      const float ea = global_encode_scale(*p.amax_f), eb = global_encode_scale(*p.amax_t);
+      o.alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
+      if (f < p.n) {
+        o.bias = load_bias(p, f);
+        const int c0 = (int)rank + group * (int)split;     // this group's first column
+        const int step = 2 * (int)split;
+        const int have = min(TN, p.m - tt * TN);
+        for (int c = c0; c < have; c += 4 * step) {
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (uint32_t r = 0; r < split; ++r) {
+            const uint32_t src = map_rank(ring + (uint32_t)(c * kTileF + l) * 4, r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c + j * step < have) v[j] += ld_cluster_f32(src + (uint32_t)(j * step * kTileF) * 4);
+          }
+          finish<T, DACT, 4>(p, o, v, f, tt * TN + c, step, (have - c + step - 1) / step);
+        }
+        if (DACT && p.dbias_partial)
+          p.dbias_partial[(int64_t)((tt * (int)split + (int)rank) * 2 + group) * p.n + f] = o.dbias;
+      }
+      if (p.amax) {
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, o.top);
+        if (lane == 0 && top) atomicMax(p.amax, top);
+      }
+    }
+    cluster_sync();   // the others have read this CTA's partial tile
+  }
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// dbias: the partial rows summed in a fixed order, 32 columns a block.
+__global__ void __launch_bounds__(256) k_dbias(const float* __restrict__ partial, int rows, int n,
+                                               float* __restrict__ out) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float v = 0.0f;
+  if (c < n)
+    for (int r = warp; r < rows; r += 8) v += partial[(int64_t)r * n + c];
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp == 0 && c < n) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v += s[w][lane];
+    out[c] = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// Packed codes [rows, k / 2] as bytes, box 128 bytes x `box_rows`, 128-byte swizzle.
+int encode_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t k, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return cuda_status(cudaErrorNotSupported);
+  const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims,
+                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NVFP4_OK : cuda_status(cudaErrorInvalidValue);
+}
+
+// Tile width and split, from the sizes alone (148 SMs), so that a workspace
+// can be sized without a device.
+struct Plan {
+  int tn, split;
+  int64_t tiles_f, tiles_t;
+  int64_t partial_rows() const { return tiles_t * split * 2; }
+};
+constexpr int kSms = 148;
+
+Plan make_plan(int64_t m, int64_t n, int64_t k) {
+  Plan p;
+  p.tiles_f = (n + kTileF - 1) / kTileF;
+  const int64_t slices = (k + kSliceK - 1) / kSliceK;
+  if (m <= 16) p.tn = 16;
+  else if (m <= 32) p.tn = 32;
+  else if (m <= 64) p.tn = 64;
+  else if (m <= 128 || p.tiles_f * ((m + 255) / 256) < kSms) p.tn = 128;
+  else p.tn = 256;
+  p.tiles_t = (m + p.tn - 1) / p.tn;
+  // Split k while the tiles leave CTA slots empty and every part keeps at
+  // least two slices.
+  const int64_t slots = (p.tn < 128 ? 2 : 1) * kSms;
+  int64_t s = p.tn == 256 ? 1 : slots / (p.tiles_f * p.tiles_t);
+  if (s > slices / 2) s = slices / 2;
+  p.split = (int)(s < 1 ? 1 : s > kMaxSplit ? kMaxSplit : s);
+  return p;
+}
+
+template <int TN, typename T, bool DACT>
+int launch_tile(const Plan& plan, const Params& p, const CUtensorMap& f, const CUtensorMap& t,
+                int sms, cudaStream_t st) {
+  using C = Tile<TN>;
+  const int64_t tiles = plan.tiles_f * plan.tiles_t;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)plan.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  auto go = [&](auto kernel) {
+    if (cudaError_t e = cudaFuncSetAttribute(
+            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes))
+      return cuda_status(e);
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, f, t, p)) return cuda_status(e);
+    return cuda_status(cudaGetLastError());
+  };
+  if constexpr (TN <= 128) {
+    if (plan.split > 1) {
+      cfg.gridDim = dim3((unsigned)(tiles * plan.split));
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      return go(k_gemm<TN, T, DACT, true>);
+    }
+  }
+  const int64_t slots = (int64_t)sms * C::kCtasPerSm;
+  cfg.gridDim = dim3((unsigned)(tiles < slots ? tiles : slots));
+  return go(k_gemm<TN, T, DACT, false>);
+}
+
+template <typename T, bool DACT>
+int launch_type(const Plan& plan, const Params& p, const CUtensorMap& f, const CUtensorMap& t,
+                int sms, cudaStream_t st) {
+  switch (plan.tn) {
+    case 16: return launch_tile<16, T, DACT>(plan, p, f, t, sms, st);
+    case 32: return launch_tile<32, T, DACT>(plan, p, f, t, sms, st);
+    case 64: return launch_tile<64, T, DACT>(plan, p, f, t, sms, st);
+    case 128: return launch_tile<128, T, DACT>(plan, p, f, t, sms, st);
+    default: return launch_tile<256, T, DACT>(plan, p, f, t, sms, st);
+  }
+}
+
+int scale_width(const void* sf, int64_t pitch) {
+  if ((uintptr_t)sf % 16 == 0 && pitch % 16 == 0) return 16;
+  if ((uintptr_t)sf % 4 == 0 && pitch % 4 == 0) return 4;
+  return 1;
+}
+
+struct Call {
+  int64_t m, n, k;
+  const void *a, *sfa, *b, *sfb;
+  const float *amax_a, *amax_b;
+  void* d;
+  int64_t ldd;
+  int dtype;
+  const void* bias;
+  int bias_dtype;
+  const void* res;
+  int64_t ldr;
+  int act;
+  void* aux;
+  int64_t ldaux;
+  bool dact;
+  float* dbias;
+  float* amax_out;
+  void* ws;
+  size_t ws_bytes;
+  uint32_t sm_count;
+  cudaStream_t st;
+};
+
+bool known_dtype(int d) { return d >= NVFP4_DTYPE_F32 && d <= NVFP4_DTYPE_F16; }
+
+int run(const Call& c) {
+  constexpr int64_t kMaxDim = 1 << 30;
+  if (c.m < 0 || c.n < 0 || c.k < 0 || c.m > kMaxDim || c.n > kMaxDim || c.k > kMaxDim ||
+      c.k % 32 != 0 || c.ldd < c.n || (c.res && c.ldr < c.n) || (c.aux && c.ldaux < c.n))
+    return NVFP4_ERR_INVALID_SHAPE;
+  if (!known_dtype(c.dtype) || (c.bias && !known_dtype(c.bias_dtype)) || c.act < kNone ||
+      c.act > kSilu)
+    return NVFP4_ERR_INVALID_ARGUMENT;
+  const uintptr_t es = c.dtype == NVFP4_DTYPE_F32 ? 4 : 2;
+  const uintptr_t bs = c.bias_dtype == NVFP4_DTYPE_F32 ? 4 : 2;
+  if ((uintptr_t)c.a % 16 || (uintptr_t)c.b % 16 || (uintptr_t)c.d % es ||
+      (uintptr_t)c.res % es || (uintptr_t)c.aux % es || (c.bias && (uintptr_t)c.bias % bs) ||
+      (uintptr_t)c.amax_a % 4 || (uintptr_t)c.amax_b % 4 || (uintptr_t)c.amax_out % 4 ||
+      (uintptr_t)c.dbias % 4 || (uintptr_t)c.ws % 4)
+    return NVFP4_ERR_MISALIGNED;
+  const bool empty = c.m == 0 || c.n == 0;
+  // k = 0 would be an empty sum; no cast writes such an operand.
+  if (!empty && c.k == 0) return NVFP4_ERR_INVALID_SHAPE;
+  if (!empty) {
+    if (!c.a || !c.sfa || !c.b || !c.sfb || !c.amax_a || !c.amax_b || !c.d || (c.dact && !c.res))
+      return NVFP4_ERR_INVALID_ARGUMENT;
+    const Plan plan = make_plan(c.m, c.n, c.k);
+    if (plan.tiles_f * plan.tiles_t > (1ll << 28)) return NVFP4_ERR_INVALID_SHAPE;
+    if (c.dbias &&
+        (!c.ws || c.ws_bytes < (size_t)plan.partial_rows() * (size_t)c.n * sizeof(float)))
+      return NVFP4_ERR_INVALID_ARGUMENT;
+  }
+  if (empty && !c.amax_out && !(c.dbias && c.n)) return NVFP4_OK;
+  int sms = 0;
+  if (int e = device_sm_count(&sms)) return e;
+  if (c.sm_count && (int)c.sm_count < sms) sms = (int)c.sm_count;
+  if (c.amax_out)
+    if (cudaError_t e = cudaMemsetAsync(c.amax_out, 0, sizeof(float), c.st)) return cuda_status(e);
+  if (empty) {
+    if (c.dbias && c.n)
+      if (cudaError_t e = cudaMemsetAsync(c.dbias, 0, sizeof(float) * (size_t)c.n, c.st))
+        return cuda_status(e);
+    return NVFP4_OK;
+  }
+  const Plan plan = make_plan(c.m, c.n, c.k);
+  CUtensorMap map_f, map_t;
+  if (int e = encode_map(&map_f, c.b, c.n, c.k, kTileF)) return e;
+  if (int e = encode_map(&map_t, c.a, c.m, c.k, plan.tn)) return e;
+  Params p = {};
+  p.m = (int)c.m;
+  p.n = (int)c.n;
+  p.k = (int)c.k;
+  p.slices = (int)((c.k + kSliceK - 1) / kSliceK);
+  p.tiles_f = (int)plan.tiles_f;
+  p.tiles_t = (int)plan.tiles_t;
+  p.sf_f = reinterpret_cast<const uint8_t*>(c.sfb);
+  p.sf_t = reinterpret_cast<const uint8_t*>(c.sfa);
+  p.sf_pitch = (int)(c.k / 16);
+  p.sf_width_f = scale_width(c.sfb, c.k / 16);
+  p.sf_width_t = scale_width(c.sfa, c.k / 16);
+  p.amax_f = c.amax_b;
+  p.amax_t = c.amax_a;
+  p.d = c.d;
+  p.ldd = c.ldd;
+  p.bias = c.bias;
+  p.bias_dtype = c.bias_dtype;
+  p.res = c.res;
+  p.ldr = c.ldr;
+  p.aux = c.aux;
+  p.ldaux = c.ldaux;
+  p.act = c.act;
+  p.dbias_partial = c.dbias ? reinterpret_cast<float*>(c.ws) : nullptr;
+  p.amax = reinterpret_cast<uint32_t*>(c.amax_out);
+  auto typed = [&](auto t) {
+    using T = decltype(t);
+    return c.dact ? launch_type<T, true>(plan, p, map_f, map_t, sms, c.st)
+                  : launch_type<T, false>(plan, p, map_f, map_t, sms, c.st);
+  };
+  const int e = c.dtype == NVFP4_DTYPE_F32    ? typed(float())
+                : c.dtype == NVFP4_DTYPE_BF16 ? typed(__nv_bfloat16())
+                                              : typed(__half());
+  if (e || !c.dbias) return e;
+  k_dbias<<<(unsigned)((c.n + 31) / 32), 256, 0, c.st>>>(p.dbias_partial,
+                                                         (int)plan.partial_rows(), p.n, c.dbias);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace gemm
+
+int gemm_device_error(uint32_t* code, int clear) {
+  if (cudaError_t e = cudaMemcpyFromSymbol(code, gemm::g_gemm_error_word, sizeof(uint32_t)))
+    return cuda_status(e);
+  if (clear && *code) {
+    const uint32_t zero = 0;
+    if (cudaError_t e = cudaMemcpyToSymbol(gemm::g_gemm_error_word, &zero, sizeof(uint32_t)))
+      return cuda_status(e);
+  }
+  return NVFP4_OK;
+}
+
+}  // namespace nvfp4
+
+extern "C" {
+
+NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
+                         const float* amax_a, const void* B, const void* SFB, const float* amax_b,
+                         void* D, int64_t ldd, int out_dtype, const void* bias, int bias_dtype,
+                         const void* residual, int64_t ldr, int activation, void* aux,
+                         int64_t ldaux, float* amax_out, uint32_t sm_count,
+                         nvfp4_stream_t stream) {
+  nvfp4::gemm::Call c = {};
+  c.m = m; c.n = n; c.k = k;
+  c.a = A; c.sfa = SFA; c.amax_a = amax_a;
+  c.b = B; c.sfb = SFB; c.amax_b = amax_b;
+  c.d = D; c.ldd = ldd; c.dtype = out_dtype;
+  c.bias = bias; c.bias_dtype = bias_dtype;
+  c.res = residual; c.ldr = ldr;
+  c.act = activation;
+  c.aux = aux; c.ldaux = ldaux;
+  c.amax_out = amax_out;
+  c.sm_count = sm_count;
+  c.st = (cudaStream_t)stream;
+  return nvfp4::gemm::run(c);
+}
+
+NVFP4_API size_t nvfp4_gemm_dact_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  return (size_t)nvfp4::gemm::make_plan(m, n, k).partial_rows() * (size_t)n * sizeof(float);
+}
+
+NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
+                              const float* amax_a, const void* B, const void* SFB,
+                              const float* amax_b, const void* aux, int64_t ldaux, int activation,
+                              void* D, int64_t ldd, int out_dtype, float* dbias, float* amax_out,
+                              void* workspace, size_t workspace_bytes, uint32_t sm_count,
+                              nvfp4_stream_t stream) {
+  nvfp4::gemm::Call c = {};
+  c.m = m; c.n = n; c.k = k;
+  c.a = A; c.sfa = SFA; c.amax_a = amax_a;
+  c.b = B; c.sfb = SFB; c.amax_b = amax_b;
+  c.d = D; c.ldd = ldd; c.dtype = out_dtype;
+  c.res = aux; c.ldr = ldaux;
+  c.act = activation;
+  c.dact = true;
+  c.dbias = dbias;
+  c.amax_out = amax_out;
+  c.ws = workspace; c.ws_bytes = workspace_bytes;
+  c.sm_count = sm_count;
+  c.st = (cudaStream_t)stream;
+  return nvfp4::gemm::run(c);
+}
+
+}  // extern "C"

@@ -17,4 +17,9 @@ int cuda_status(cudaError_t e);
 // that are not compute capability 10.0.
 int device_sm_count(int* sms);
 
+// Read (and with clear reset) the error words of the kernels in the other
+// source files, for nvfp4_device_error.  The device is already synchronized.
+int gemm_device_error(uint32_t* code, int clear);
+int layernorm_device_error(uint32_t* code, int clear);
+
 }  // namespace nvfp4

@@ -1952,6 +1952,11 @@ NVFP4_API int nvfp4_device_error(uint32_t* code, int clear) {
     if (cudaError_t e = cudaMemcpyToSymbol(nvfp4::g_device_error_word, &zero, sizeof(uint32_t)))
       return nvfp4::cuda_status(e);
   }
+  for (auto other : {nvfp4::gemm_device_error, nvfp4::layernorm_device_error}) {
+    uint32_t word = 0;
+    if (int e = other(&word, clear)) return e;
+    if (*code == 0) *code = word;
+  }
   return NVFP4_OK;
 }
 

@@ -11,7 +11,7 @@ from typing import Optional, Union
 
 import torch
 
-from ._native import call
+from ._native import call, load
 
 Ptr = Union[int, torch.Tensor, None]
 
@@ -216,6 +216,81 @@ def mul_cvt_fp8_4x(inp: Ptr, in_dtype, scale: Ptr, scale_width: int, scale_strid
     else:
         call("nvfp4_mul_cvt_fp8_4x", _ptr(inp), _dtype_code(in_dtype), _ptr(scale), scale_width,
              scale_stride, _ptr(out), FP8_FORMATS[fmt], ngroups, _stream(stream))
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+MOMENTS = {"exp_avg": 0, "exp_avg_sq": 1}
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+def gemm_nvfp4(m: int, n: int, k: int, A: Ptr, SFA: Ptr, amax_a: Ptr, B: Ptr, SFB: Ptr,
+               amax_b: Ptr, D: Ptr, ldd: int, out_dtype, bias: Ptr, bias_dtype, residual: Ptr,
+               ldr: int, activation: str, aux: Ptr, ldaux: int, amax_out: Ptr, sm_count: int = 0,
+               stream=None) -> None:
+    """nvfp4_gemm: D = act(A B^T + bias) + residual of two NVFP4 operands."""
+    call("nvfp4_gemm", m, n, k, _ptr(A), _ptr(SFA), _ptr(amax_a), _ptr(B), _ptr(SFB),
+         _ptr(amax_b), _ptr(D), ldd, _dtype_code(out_dtype), _ptr(bias), _dtype_code(bias_dtype),
+         _ptr(residual), ldr, _activation(activation), _ptr(aux), ldaux, _ptr(amax_out), sm_count,
+         _stream(stream))
+
+
+def gemm_nvfp4_dact_workspace_bytes(m: int, n: int, k: int) -> int:
+    return load().nvfp4_gemm_dact_workspace_bytes(m, n, k)
+
+
+def gemm_nvfp4_dact(m: int, n: int, k: int, A: Ptr, SFA: Ptr, amax_a: Ptr, B: Ptr, SFB: Ptr,
+                    amax_b: Ptr, aux: Ptr, ldaux: int, activation: str, D: Ptr, ldd: int,
+                    out_dtype, dbias: Ptr, amax_out: Ptr, workspace: Ptr, workspace_bytes: int,
+                    sm_count: int = 0, stream=None) -> None:
+    """nvfp4_gemm_dact: D = (A B^T) act'(aux) and its column sums."""
+    call("nvfp4_gemm_dact", m, n, k, _ptr(A), _ptr(SFA), _ptr(amax_a), _ptr(B), _ptr(SFB),
+         _ptr(amax_b), _ptr(aux), ldaux, _activation(activation), _ptr(D), ldd,
+         _dtype_code(out_dtype), _ptr(dbias), _ptr(amax_out), _ptr(workspace), workspace_bytes,
+         sm_count, _stream(stream))
+
+
+def layernorm_fwd(rows: int, cols: int, x: Ptr, ldx: int, gamma: Ptr, beta: Ptr, dtype,
+                  weight_dtype, eps: float, y: Ptr, ldy: int, mean: Ptr, rstd: Ptr,
+                  amax_out: Ptr, stream=None) -> None:
+    call("nvfp4_layernorm_fwd", rows, cols, _ptr(x), ldx, _ptr(gamma), _ptr(beta),
+         _dtype_code(dtype), _dtype_code(weight_dtype), eps, _ptr(y), ldy, _ptr(mean), _ptr(rstd),
+         _ptr(amax_out), _stream(stream))
+
+
+def layernorm_bwd_workspace_bytes(rows: int, cols: int) -> int:
+    return load().nvfp4_layernorm_bwd_workspace_bytes(rows, cols)
+
+
+def layernorm_bwd(rows: int, cols: int, dy: Ptr, lddy: int, x: Ptr, ldx: int, mean: Ptr,
+                  rstd: Ptr, gamma: Ptr, residual: Ptr, ldr: int, dtype, weight_dtype, dx: Ptr,
+                  lddx: int, dgamma: Ptr, dbeta: Ptr, workspace: Ptr, workspace_bytes: int,
+                  stream=None) -> None:
+    call("nvfp4_layernorm_bwd", rows, cols, _ptr(dy), lddy, _ptr(x), ldx, _ptr(mean), _ptr(rstd),
+         _ptr(gamma), _ptr(residual), ldr, _dtype_code(dtype), _dtype_code(weight_dtype),
+         _ptr(dx), lddx, _ptr(dgamma), _ptr(dbeta), _ptr(workspace), workspace_bytes,
+         _stream(stream))
+
+
+def adamw_step(tensors, count: int, param_dtype, grad_dtype, state_format: int, lr: float,
+               beta1: float, beta2: float, eps: float, step: int, grad_scale: Ptr, scalars: Ptr,
+               amax_out: Ptr, rng_state: Ptr, stream=None) -> None:
+    """nvfp4_adamw_step over a ctypes array of _native.AdamWTensor (host memory)."""
+    call("nvfp4_adamw_step", tensors, count, _dtype_code(param_dtype), _dtype_code(grad_dtype),
+         state_format, lr, beta1, beta2, eps, step, _ptr(grad_scale), _ptr(scalars),
+         _ptr(amax_out), _ptr(rng_state), _stream(stream))
+
+
+def adamw_unpack_state(codes: Ptr, scales: Ptr, n: int, moment: str, out: Ptr, out_dtype,
+                       stream=None) -> None:
+    if moment not in MOMENTS:
+        raise ValueError(f"unknown moment {moment!r}: one of {', '.join(MOMENTS)}")
+    call("nvfp4_adamw_unpack_state", _ptr(codes), _ptr(scales), n, MOMENTS[moment], _ptr(out),
+         _dtype_code(out_dtype), _stream(stream))
 
 
 def device_error(clear: bool = True) -> int:

@@ -267,6 +267,138 @@ NVFP4_API int nvfp4_mul_cvt_fp8_4x_loose(const void* in, int in_dtype, const flo
                                          size_t ngroups, nvfp4_stream_t stream);
 
 /* ---------------------------------------------------------------------- */
+/* A training step around the cast: products of NVFP4 operands, layer norm, */
+/* AdamW.  No reference counterparts: the reference ends at the cast.       */
+/* ---------------------------------------------------------------------- */
+
+/* Activations of the products' epilogues: z, max(z, 0), the tanh form of GELU
+ * 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), z / (1 + exp(-z)). */
+enum { NVFP4_ACT_NONE = 0, NVFP4_ACT_RELU = 1, NVFP4_ACT_GELU = 2, NVFP4_ACT_SILU = 3 };
+
+/* D = act(z) + residual with z = A B^T + bias, where A (m x k) and B (n x k)
+ * are NVFP4 as this library's casts write them: packed E2M1 codes row-major
+ * along k (C of the casts), row-major E4M3 scales of 16-element blocks (SFC)
+ * and the amax that the cast was given.  So the rows are a row-wise cast's
+ * rows (y = x W^T: A = cast of x, B = cast of W) or an RHT cast's rows (a
+ * weight gradient: A = transposed cast of dy, B = transposed cast of x, k =
+ * tokens; the two Hadamard transforms cancel).
+ *   out_dtype   NVFP4_DTYPE_*: type of D, residual and aux
+ *   ldd, ldr, ldaux   row strides in elements, >= n
+ *   bias        n values of bias_dtype, or NULL
+ *   residual    m x n, or NULL; may be D itself (accumulation in place)
+ *   aux         receives z (what the backward pass needs), or NULL
+ *   amax_out    receives max |D| as stored, NaN-propagating (what the cast of
+ *               D needs; enqueues a 4-byte memset), or NULL
+ *   sm_count    0: all SMs; else a cap on the persistent grid (a call short
+ *               enough to split k over a cluster takes its own grid)
+ * Accumulates in fp32; each output is rounded once.  Results repeat bit for
+ * bit.  k % 32 == 0 and k > 0; A and B 16-byte aligned; m, n any size (0: a
+ * no-op but for *amax_out = 0); m, n, k <= 2^30. */
+NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
+                         const float* amax_a, const void* B, const void* SFB, const float* amax_b,
+                         void* D, int64_t ldd, int out_dtype, const void* bias, int bias_dtype,
+                         const void* residual, int64_t ldr, int activation, void* aux,
+                         int64_t ldaux, float* amax_out, uint32_t sm_count,
+                         nvfp4_stream_t stream);
+
+/* The product in the backward pass of an activation: D = (A B^T) act'(aux)
+ * with the aux that nvfp4_gemm wrote (type out_dtype; may be D itself), and
+ * dbias[j] = sum_i D[i, j] (fp32, before D is rounded; NULL: not computed).
+ * `workspace` is scratch of nvfp4_gemm_dact_workspace_bytes(m, n, k) bytes,
+ * needed with dbias only; it needs no initial state and keeps none. */
+NVFP4_API size_t nvfp4_gemm_dact_workspace_bytes(int64_t m, int64_t n, int64_t k);
+NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
+                              const float* amax_a, const void* B, const void* SFB,
+                              const float* amax_b, const void* aux, int64_t ldaux, int activation,
+                              void* D, int64_t ldd, int out_dtype, float* dbias, float* amax_out,
+                              void* workspace, size_t workspace_bytes, uint32_t sm_count,
+                              nvfp4_stream_t stream);
+
+/* Layer norm of `rows` rows of `cols` elements (row strides ldx, ldy in
+ * elements): y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps).
+ * x and y of dtype, gamma and beta (NULL: 0) of weight_dtype, which is dtype
+ * or fp32.  mean and rstd (rows floats each) may be NULL.  amax_out as in
+ * nvfp4_gemm, of y.  y may be x.  cols <= 2^24. */
+NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                                  const void* gamma, const void* beta, int dtype,
+                                  int weight_dtype, float eps, void* y, int64_t ldy, float* mean,
+                                  float* rstd, float* amax_out, nvfp4_stream_t stream);
+
+/* Its backward pass, with mean and rstd from the forward call:
+ *   dx = rstd (u - mean(u) - h mean(u h)) + residual,  u = dy gamma, h = (x - mean) rstd
+ *   dgamma = sum_rows dy h,  dbeta = sum_rows dy      (of weight_dtype, added in fp32)
+ * residual (NULL: none) is the gradient that reaches x past the norm.  dx may
+ * be dy or residual.  dgamma, dbeta may be NULL.  `workspace`: scratch of
+ * nvfp4_layernorm_bwd_workspace_bytes(rows, cols) bytes without initial or
+ * kept state.  rows == 0 clears dgamma and dbeta.  Results repeat bit for bit. */
+NVFP4_API size_t nvfp4_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
+NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, int64_t lddy,
+                                  const void* x, int64_t ldx, const float* mean,
+                                  const float* rstd, const void* gamma, const void* residual,
+                                  int64_t ldr, int dtype, int weight_dtype, void* dx,
+                                  int64_t lddx, void* dgamma, void* dbeta, void* workspace,
+                                  size_t workspace_bytes, nvfp4_stream_t stream);
+
+/* How the two moments of AdamW are held: fp32, or 8 bits with one scale byte
+ * for each 128 elements.  Scale byte s stands for 2^(s - 127) (255: the block
+ * held a value that was not finite and reads as NaN).  exp_avg: sign and E4M3.
+ * exp_avg_sq: E4M4 without sign, bias 7 (0: 0; e = 0: f / 16 * 2^-6; else
+ * (1 + f / 16) 2^(e - 7)).  All bytes zero is the state before the first step. */
+enum { NVFP4_STATE_F32 = 0, NVFP4_STATE_8BIT = 1 };
+enum { NVFP4_EXP_AVG = 0, NVFP4_EXP_AVG_SQ = 1 };
+
+/* One parameter tensor of a step.  Its elements are contiguous. */
+typedef struct nvfp4_adamw_tensor {
+  void* param;               /* n of param_dtype, updated in place */
+  const void* grad;          /* n of grad_dtype */
+  void* exp_avg;             /* n floats, or n bytes */
+  void* exp_avg_sq;
+  uint8_t* exp_avg_scale;    /* ceil(n / 128) bytes with 8-bit states, else unused */
+  uint8_t* exp_avg_sq_scale;
+  void* copy;                /* n bf16: the updated parameters rounded (fp32 parameters
+                                only), or NULL */
+  uint64_t n;
+  uint64_t offset;           /* position of the first element in the numbering that the
+                                random bits go by (8-bit states; % 128 == 0): distinct
+                                tensors get distinct ranges, and a shard of a tensor
+                                its place in the whole, so that shards repeat the
+                                unsharded result */
+  double weight_decay;
+} nvfp4_adamw_tensor;
+
+/* One AdamW step (decoupled weight decay, bias-corrected) over `count`
+ * tensors, described by a HOST array that the call has read when it returns:
+ *   g = grad * *grad_scale (device float; NULL: 1)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr wd) p - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in fp32.  param_dtype: fp32 or bf16 (rounded to nearest); grad_dtype: any.
+ * step counts from 1.  scalars (device, NULL or 3 floats {lr, 1 - beta1^step,
+ * 1 - beta2^step}) takes the place of lr and step, so that a captured call can
+ * be replayed.
+ * 8-bit moments are rounded stochastically with Philox4x32-10: key =
+ * rng_state.seed, counter = {rng_state.offset + step, (offset + i) / 4} for
+ * element i; word i % 4 of the result gives exp_avg its low and exp_avg_sq its
+ * high 16 bits.  (A replayed call repeats `step`: advance rng_state.)  An
+ * exp_avg_sq above zero stays above zero.  Their noise averages out over
+ * 1 / (1 - beta2) steps: with beta2 <= 0.98 the standard deviation of
+ * exp_avg_sq stays below 10 %; for longer memories take fp32.
+ * amax_out (NULL or `count` floats): max |p| of each tensor rounded to bf16,
+ * NaN-propagating: what the cast of the new weights needs.
+ * count == 0 and tensors with n == 0 are skipped.  The tensors of one call
+ * must not overlap. */
+NVFP4_API int nvfp4_adamw_step(const nvfp4_adamw_tensor* tensors, int count, int param_dtype,
+                               int grad_dtype, int state_format, double lr, double beta1,
+                               double beta2, double eps, int64_t step, const float* grad_scale,
+                               const float* scalars, float* amax_out, const size_t* rng_state,
+                               nvfp4_stream_t stream);
+
+/* The values of n 8-bit moments (moment: NVFP4_EXP_AVG or NVFP4_EXP_AVG_SQ;
+ * out_dtype fp32, or bf16, which holds them exactly down to its subnormals). */
+NVFP4_API int nvfp4_adamw_unpack_state(const void* codes, const uint8_t* scales, size_t n,
+                                       int moment, void* out, int out_dtype,
+                                       nvfp4_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
 /* Diagnostics                                                             */
 /* ---------------------------------------------------------------------- */
 

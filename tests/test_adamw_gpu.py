@@ -1,0 +1,328 @@
+"""AdamW against 64 bits, and its 8-bit moments bit for bit.
+
+Tolerances of the 32-bit form: each moment is two products and a sum, each
+rounded (3 steps of 2^-24 of its TERMS |beta1 m| + |(1 - beta1) g|, which may
+cancel in m).  p's update passes m's error on, magnified by lr / (bias
+correction * denominator), and adds a root, a quotient and two products (2^-20
+of the update).  The decayed p has the factor's rounding, the product's and the
+final sum's: 3 steps of 2^-24 of |p| and one of the result."""
+import math
+
+import pytest
+import torch
+
+from tests import training_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+H = dict(lr=1e-2, beta1=0.9, beta2=0.95, eps=1e-8)
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def close(got, want, tol, what):
+    err = (got.double().cpu() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((err - tol).max()))
+
+
+def make(sizes, param, grad, seed):
+    g = torch.Generator().manual_seed(seed)
+    ps = [(torch.randn(n, generator=g) * 0.05).to(param) for n in sizes]
+    gs = [(torch.randn(n, generator=g) * 0.01).to(grad) for n in sizes]
+    ms = [torch.randn(n, generator=g) * 0.003 for n in sizes]
+    vs = [(torch.randn(n, generator=g) * 0.01) ** 2 for n in sizes]
+    return ps, gs, ms, vs
+
+
+def check_param(p, p0, g, m0, v, step, want, copies, amax, i):
+    terms = H["beta1"] * m0.double().abs() + (1 - H["beta1"]) * g.double().abs()
+    gain = H["lr"] / (1 - H["beta1"] ** step) / (
+        torch.sqrt(v / (1 - H["beta2"] ** step)) + H["eps"])
+    tol = (gain * terms * (3 * 2.0 ** -24 + 2.0 ** -20)
+           + 2.0 ** -24 * (3 * p0.double().abs() + want.abs()))
+    if p.dtype == torch.bfloat16:
+        tol = tol + orc.half_step(torch.bfloat16) * want.abs() * (1 + 2.0 ** -8)
+    close(p, want, tol, f"p[{i}]")
+    if copies is not None:
+        assert torch.equal(copies[i], p.to(torch.bfloat16))
+    if amax is not None:
+        top = p.to(torch.bfloat16).float().abs().max() if p.numel() else torch.zeros(())
+        assert float(amax[i]) == float(top)
+
+
+SIZES = [[1], [5, 3, 1000], [4096], [4097, 0, 129, 8192, 127, 128], [33] * 70, [300] * 800]
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("param,grad", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"),
+                                        ("bf16", "bf16"), ("bf16", "f32")])
+def test_32_bit(nvlib, sizes, param, grad):
+    ps, gs, ms, vs = make(sizes, TYPES[param], TYPES[grad], len(sizes))
+    dp, dg, dm, dv = ([t.cuda() for t in x] for x in (ps, gs, ms, vs))
+    copies = ([torch.empty(n, dtype=torch.bfloat16, device="cuda") for n in sizes]
+              if param == "f32" else None)
+    amax = torch.full((len(sizes),), 9.0, device="cuda")
+    wds = [0.1 * (i % 3) for i in range(len(sizes))]
+    scale = torch.tensor([0.5], device="cuda")
+    opt = nvlib.AdamW(dp, dg, dm, dv, copies=copies, weight_decays=wds, amax_out=amax)
+    opt.step(7, grad_scale=scale, **H)
+    for i in range(len(sizes)):
+        p, m, v = orc.adamw(ps[i], gs[i], ms[i], vs[i], step=7, wd=wds[i], grad_scale=0.5, **H)
+        g = gs[i].double() * 0.5
+        close(dm[i], m, 3 * 2.0 ** -24 * (0.9 * ms[i].double().abs() + 0.1 * g.abs()), "m")
+        close(dv[i], v, 4 * 2.0 ** -24 * v, "v")
+        check_param(dp[i], ps[i], g, ms[i], v, 7, p, copies, amax, i)
+
+
+def zeros8(sizes):
+    blocks = [-(-n // 128) for n in sizes]
+    return ([torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes],
+            [torch.zeros(b, dtype=torch.uint8, device="cuda") for b in blocks])
+
+
+def f32(x):
+    return x.to(torch.float32)
+
+
+def expect8(x, moment, words):
+    """Codes and scale bytes of fp32 values, step by step as the format says."""
+    n = x.numel()
+    drop, levels = (20, 8) if moment == "exp_avg" else (19, 16)
+    pad = -(-n // 128) * 128 - n
+    bits = torch.cat([x, torch.zeros(pad)]).abs().view(torch.int32).view(-1, 128)
+    top = bits.amax(1) >> 23
+    scale = torch.where(top == 255, top, (top - 7).clamp_min(1))
+    inv = ((254 - scale).clamp_min(0) << 23).view(torch.float32)
+    y = torch.cat([x, torch.zeros(pad)]).abs().view(-1, 128) * inv[:, None]
+    low = y < 2.0 ** -6
+    r = torch.cat([words, torch.zeros(pad, dtype=torch.int32)]).view(-1, 128)
+    t = torch.where(low, y + 2.0 ** -6, y).view(torch.int32) + (r << (drop - 16))
+    code = (t >> drop) - ((120 + low.int()) << (23 - drop))
+    code = torch.where(scale[:, None] == 255, torch.zeros_like(code), code).view(-1)[:n]
+    if moment == "exp_avg":
+        code = code | ((x < 0).int() << 7)
+    else:
+        finite = (scale != 255).repeat_interleave(128)[:n]
+        code = torch.where((x > 0) & finite, code.clamp_min(1), code)
+    return code.to(torch.uint8), scale.to(torch.uint8)
+
+
+def moment_words(n, offset, seed, counter):
+    lo, hi = torch.empty(n, dtype=torch.int32), torch.empty(n, dtype=torch.int32)
+    for i in range(0, n, 4):
+        w = orc.philox(seed, counter, (offset + i) // 4)
+        for k in range(min(4, n - i)):
+            lo[i + k], hi[i + k] = w[k] & 0xFFFF, w[k] >> 16
+    return lo, hi
+
+
+@pytest.mark.parametrize("sizes", [[1], [128], [4, 300, 127, 4096 + 37], [513] * 40])
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_8_bit(nvlib, sizes, grad):
+    """Three steps from zero states: codes and scales bit for bit, parameters
+    against 64 bits from the decoded states."""
+    ps, _, _, _ = make(sizes, torch.float32, TYPES[grad], 3)
+    dp = [p.cuda() for p in ps]
+    (dm, ms), (dv, vs) = zeros8(sizes), zeros8(sizes)
+    dg = [torch.zeros(n, dtype=TYPES[grad], device="cuda") for n in sizes]
+    seed, off = 0x123456789ABCDEF, 0xFFFFFFFE
+    rng = torch.tensor([seed, off], device="cuda")
+    amax = torch.empty(len(sizes), device="cuda")
+    opt = nvlib.AdamW(dp, dg, dm, dv, exp_avg_scales=ms, exp_avg_sq_scales=vs, amax_out=amax,
+                      rng_state=rng)
+    offsets = [0]
+    for n in sizes:
+        offsets.append(offsets[-1] + -(-n // 128) * 128)
+    for step in (1, 2, 3):
+        gs = make(sizes, torch.float32, TYPES[grad], 100 + step)[1]
+        if sizes[-1] > 200:
+            gs[-1][7] = 30.0        # an outlier pushes its block into the lowest binade
+        for d, g in zip(dg, gs):
+            d.copy_(g)
+        before = [(p.cpu(), orc.unpack8(m.cpu(), s.cpu(), "exp_avg"),
+                   orc.unpack8(v.cpu(), t.cpu(), "exp_avg_sq"))
+                  for p, m, s, v, t in zip(dp, dm, ms, dv, vs)]
+        opt.step(step, **H)
+        torch.cuda.synchronize()
+        for i, n in enumerate(sizes):
+            p0, m0, v0 = before[i]
+            g = f32(gs[i])
+            m = f32(m0) * torch.tensor(0.9) + g * torch.tensor(1 - 0.9)
+            v = f32(v0) * torch.tensor(0.95) + (g * g) * torch.tensor(1 - 0.95)
+            lo, hi = moment_words(n, offsets[i], seed, off + step)
+            code, scale = expect8(m, "exp_avg", lo)
+            assert torch.equal(ms[i].cpu(), scale) and torch.equal(dm[i].cpu(), code), (step, i)
+            code, scale = expect8(v, "exp_avg_sq", hi)
+            assert torch.equal(vs[i].cpu(), scale) and torch.equal(dv[i].cpu(), code), (step, i)
+            want, _, wv = orc.adamw(p0, g, m0, v0, step=step, wd=0.0, **H)
+            check_param(dp[i], p0, g, m0, wv, step, want, None, amax, i)
+
+
+def test_8_bit_shards_repeat_the_whole(nvlib):
+    """A tensor in two pieces with their offsets: the bits of the whole."""
+    n, cut = 5000, 2048
+    ps, gs, _, _ = make([n], torch.float32, torch.float32, 9)
+    rng = torch.tensor([11, 5], device="cuda")
+    out = []
+    for pieces in ([slice(0, n)], [slice(0, cut), slice(cut, n)]):
+        p, g = ps[0].cuda(), gs[0].cuda()
+        (m,), (ms,) = zeros8([n])
+        (v,), (vs,) = zeros8([n])
+
+        def cutb(t):
+            return [t[s.start // 128:-(-s.stop // 128)] for s in pieces]
+
+        def cute(t):
+            return [t[s] for s in pieces]
+        opt = nvlib.AdamW(cute(p), cute(g), cute(m), cute(v), exp_avg_scales=cutb(ms),
+                          exp_avg_sq_scales=cutb(vs), offsets=[s.start for s in pieces],
+                          rng_state=rng)
+        for step in (1, 2):
+            opt.step(step, **H)
+        out.append((p, m, v, ms, vs))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_8_bit_special_values(nvlib):
+    """A value that is not finite marks its block; a second moment above zero
+    stays above zero; zero gradients from zero states change nothing but the decay."""
+    n = 384
+    p = torch.ones(n, device="cuda")
+    g = torch.zeros(n, device="cuda")
+    g[5] = math.inf
+    g[128] = 1.0
+    g[129] = 1e-12            # far below its block's lowest step
+    (m,), (ms,) = zeros8([n])
+    (v,), (vs,) = zeros8([n])
+    amax = torch.empty(1, device="cuda")
+    opt = nvlib.AdamW([p], [g], [m], [v], exp_avg_scales=[ms], exp_avg_sq_scales=[vs],
+                      rng_state=torch.tensor([1, 2], device="cuda"), amax_out=amax,
+                      weight_decays=[0.5])
+    opt.step(1, **H)
+    um, uv = (nvlib.adamw_unpack_state(c, s, k).cpu() for c, s, k in
+              ((m, ms, "exp_avg"), (v, vs, "exp_avg_sq")))
+    assert bool(torch.isnan(um[:128]).all()) and bool(torch.isnan(uv[:128]).all())
+    assert bool(torch.isfinite(um[128:]).all()) and bool(torch.isfinite(uv[128:]).all())
+    assert float(uv[129]) > 0 and bool((uv[256:] == 0).all()) and bool((um[256:] == 0).all())
+    pc = p.cpu()
+    assert math.isnan(float(pc[5])) and math.isnan(float(amax))
+    assert bool((pc[256:] == float(torch.tensor(1.0) * torch.tensor(1 - 0.01 * 0.5))).all())
+
+
+@pytest.mark.parametrize("moment", ["exp_avg", "exp_avg_sq"])
+@pytest.mark.parametrize("n,shift", [(1, 0), (128, 0), (256 * 3 + 5, 0), (1000, 1)])
+def test_unpack(nvlib, moment, n, shift):
+    """All codes under scales from the smallest to the largest."""
+    raw = (torch.arange(n + shift) * 37 % 256).to(torch.uint8)
+    if moment == "exp_avg":
+        raw[(raw & 127) == 127] = 0        # E4M3's NaN code is never written
+    codes = raw.cuda()[shift:]
+    blocks = -(-n // 128)
+    scales = torch.tensor([1, 120, 127, 255, 0, 121, 3, 60] * blocks, dtype=torch.uint8)[:blocks]
+    want = orc.unpack8(codes.cpu(), scales, moment)
+    got = nvlib.adamw_unpack_state(codes, scales.cuda(), moment, torch.float32).double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+    b16 = nvlib.adamw_unpack_state(codes, scales.cuda(), moment).double().cpu()
+    assert torch.equal(b16.nan_to_num(), got.float().to(torch.bfloat16).double().nan_to_num())
+
+
+def test_stochastic_rounding_is_unbiased(nvlib):
+    """Mean over many draws of one second moment between two codes: within 5
+    standard deviations of its value."""
+    n = 128 * 512
+    g = torch.full((n,), math.sqrt(1.37), device="cuda")
+    p = torch.zeros(n, device="cuda")
+    (m,), (ms,) = zeros8([n])
+    (v,), (vs,) = zeros8([n])
+    opt = nvlib.AdamW([p], [g], [m], [v], exp_avg_scales=[ms], exp_avg_sq_scales=[vs],
+                      rng_state=torch.tensor([77, 0], device="cuda"))
+    opt.step(1, **H)
+    u = nvlib.adamw_unpack_state(v, vs, "exp_avg_sq", torch.float32).double()
+    want = float(torch.tensor(0.05) * (g[0].cpu() * g[0].cpu()))
+    values = u.unique()
+    assert values.numel() == 2 and float(values[0]) < want < float(values[1])
+    sd = float(values[1] - values[0]) / 2 / math.sqrt(n)
+    assert abs(float(u.mean()) - want) < 5 * sd + 2.0 ** -16 * float(values[1] - values[0])
+
+
+def test_unaligned_views_and_neighbours(nvlib):
+    """Tensors at odd places of flat buffers; what lies around them stays."""
+    cuts = [(1, 200), (203, 777), (1001, 64)]
+    flat = {k: torch.full((1100,), 2.5, device="cuda") for k in "pgmv"}
+    copies = torch.full((1100,), 2.5, dtype=torch.bfloat16, device="cuda")
+    ps, gs, ms, vs = make([n for _, n in cuts], torch.float32, torch.float32, 12)
+    for k, seq in zip("pgmv", (ps, gs, ms, vs)):
+        for (a, n), t in zip(cuts, seq):
+            flat[k][a:a + n] = t.cuda()
+    view = lambda t: [t[a:a + n] for a, n in cuts]  # noqa: E731
+    opt = nvlib.AdamW(view(flat["p"]), view(flat["g"]), view(flat["m"]), view(flat["v"]),
+                      copies=view(copies))
+    opt.step(3, **H)
+    for i, (a, n) in enumerate(cuts):
+        p, m, v = orc.adamw(ps[i], gs[i], ms[i], vs[i], step=3, wd=0.0, **H)
+        check_param(flat["p"][a:a + n], ps[i], gs[i], ms[i], v, 3, p, view(copies), None, i)
+    mask = torch.ones(1100, dtype=torch.bool, device="cuda")
+    for a, n in cuts:
+        mask[a:a + n] = False
+    for t in [*flat.values(), copies]:
+        assert bool((t[mask] == 2.5).all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_captured_step_takes_its_scalars_from_the_device(nvlib, eight):
+    """A captured step replayed with new scalars, gradients and rng_state gives
+    the bits of eager steps with the same."""
+    sizes = [1000, 260]
+    ps, _, ms, vs = make(sizes, torch.float32, torch.float32, 4)
+
+    def build():
+        p, g = [t.cuda() for t in ps], [torch.empty(n, device="cuda") for n in sizes]
+        rng = torch.tensor([3, 0], device="cuda")
+        if eight:
+            (m, a), (v, b) = zeros8(sizes), zeros8(sizes)
+            opt = nvlib.AdamW(p, g, m, v, exp_avg_scales=a, exp_avg_sq_scales=b, rng_state=rng,
+                              weight_decays=[0.1, 0.0])
+        else:
+            m, v = [t.cuda() for t in ms], [t.cuda() for t in vs]
+            opt = nvlib.AdamW(p, g, m, v, weight_decays=[0.1, 0.0])
+        return opt, p, g, m, v, rng, torch.empty(3, device="cuda")
+    runs = [build(), build()]
+    graph = torch.cuda.CUDAGraph()
+    opt, _, _, _, _, _, sc = runs[1]
+    with torch.cuda.graph(graph):
+        opt.step(0, lr=0.0, beta1=0.9, beta2=0.95, eps=1e-8, scalars=sc)
+    for step in (1, 2, 3):
+        gs = make(sizes, torch.float32, torch.float32, 50 + step)[1]
+        lr = 0.01 / step
+        for which, (opt, p, g, m, v, rng, sc) in enumerate(runs):
+            for d, t in zip(g, gs):
+                d.copy_(t)
+            sc.copy_(torch.tensor([lr, 1 - 0.9 ** step, 1 - 0.95 ** step]))
+            rng[1] = step
+            if which:
+                graph.replay()
+            else:
+                opt.step(0, lr=0.0, beta1=0.9, beta2=0.95, eps=1e-8, scalars=sc)
+        torch.cuda.synchronize()
+        for a, b in zip(runs[0][1:5], runs[1][1:5]):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # and the device scalars mean what lr and step mean
+    opt, p, g, m, v, rng, _ = build()
+    for step in (1, 2, 3):
+        gs = make(sizes, torch.float32, torch.float32, 50 + step)[1]
+        for d, t in zip(g, gs):
+            d.copy_(t)
+        rng[1] = 0                         # the counter is offset + step
+        opt.step(step, lr=0.01 / step, beta1=0.9, beta2=0.95, eps=1e-8)
+    for x, y in zip(p, runs[0][1]):
+        close(x, y.double().cpu(), 2.0 ** -18 * 0.03 + 2.0 ** -22 * x.abs().cpu(), "scalars")
+
+
+def test_first_step_by_differences(nvlib):
+    """From zero states the first update is lr sign(g) for gradients far above eps."""
+    g = torch.tensor([3.0, -0.25, 1e-3, -2e4], device="cuda")
+    p = torch.zeros(4, device="cuda")
+    opt = nvlib.AdamW([p], [g], [torch.zeros(4, device="cuda")], [torch.zeros(4, device="cuda")])
+    opt.step(1, lr=0.5, beta1=0.9, beta2=0.95, eps=1e-12)
+    close(p, -0.5 * g.sign().double().cpu(), torch.full((4,), 0.5 * 2.0 ** -20), "p")

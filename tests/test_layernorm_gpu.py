@@ -1,0 +1,224 @@
+"""Layer norm forward and backward against 64 bits.
+
+Tolerances.  A row's sums are taken by threads of at most L elements each and
+joined over lanes and warps: off by (L + 16) 2^-24 of the mean magnitude.
+Each output is a short chain of fp32 operations (counted as 2^-20 of its
+terms) and one rounding to its type.  A column sum over r rows is off by at
+most (r + 64) 2^-24 of its sum of magnitudes, and by its terms' own errors."""
+import math
+
+import pytest
+import torch
+
+from tests import training_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+EPS = 1e-5
+
+
+def close(got, want, tol, what):
+    err = (got.double().cpu() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((err - tol).max()),
+                           bad.nonzero()[:4].tolist())
+
+
+def make(rows, cols, dtype, weight, seed, offset=0.5):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, cols, generator=g) * (torch.rand(cols, generator=g) + 0.3)
+         + offset).to(dtype)
+    gamma = (torch.randn(cols, generator=g) * 0.2 + 1).to(weight)
+    beta = (torch.randn(cols, generator=g) * 0.2).to(weight)
+    dy = torch.randn(rows, cols, generator=g).to(dtype)
+    res = torch.randn(rows, cols, generator=g).to(dtype)
+    return x, gamma, beta, dy, res
+
+
+def check_forward(nvlib, x, gamma, beta, xd=None, eps=EPS):
+    rows, cols = x.shape
+    amax = torch.empty(1, device="cuda")
+    y, mean, rstd = nvlib.layernorm(x.cuda() if xd is None else xd, gamma.cuda(),
+                                    None if beta is None else beta.cuda(), eps, amax_out=amax)
+    wy, wm, wr = orc.layernorm(x, gamma, beta, eps)
+    L = max(32, cols // 256) + 16
+    size = x.double().abs().amax(1)
+    em = L * 2.0 ** -24 * size
+    close(mean, wm, em + 2.0 ** -24 * wm.abs(), "mean")
+    # var = mean (x - mean)^2: relative 2 em^2-free error of L 2^-24, halved by the root
+    close(rstd, wr, L * 2.0 ** -23 * wr + wr ** 3 * em ** 2, "rstd")
+    h = (x.double() - wm[:, None]) * wr[:, None]
+    g = gamma.double().abs()
+    tol = (wr[:, None] * g * em[:, None] + L * 2.0 ** -22 * h.abs() * g
+           + 2.0 ** -23 * (0 if beta is None else beta.double().abs()))
+    close(y, wy, tol + (orc.half_step(x.dtype) + 2.0 ** -23) * wy.abs()
+          + orc.least_step(x.dtype), "y")
+    assert float(amax) == float(y.float().abs().max())
+    return mean, rstd
+
+
+def check_backward(nvlib, x, gamma, dy, res, mean, rstd, dev=None):
+    rows, cols = x.shape
+    xd, dyd, resd = dev or (x.cuda(), dy.cuda(), None if res is None else res.cuda())
+    dx, dg, db = nvlib.layernorm_backward(dyd, xd, mean, rstd, gamma.cuda(), residual=resd)
+    m, r = mean.cpu(), rstd.cpu()
+    wdx, wdg, wdb = orc.layernorm_backward(dy, x, m, r, gamma, res)
+    L = max(32, cols // 256) + 16
+    h = (x.double() - m.double()[:, None]) * r.double()[:, None]
+    u = (dy.double() * gamma.double()).abs()
+    part = r.double()[:, None] * (u + u.mean(1, keepdim=True)
+                                  + h.abs() * (u * h.abs()).mean(1, keepdim=True))
+    tol = L * 2.0 ** -22 * part + 2.0 ** -23 * (0 if res is None else res.double().abs())
+    close(dx, wdx, tol + orc.half_step(x.dtype) * wdx.abs()
+          + orc.least_step(x.dtype), "dx")
+    hw = orc.half_step(gamma.dtype)
+    sub = orc.least_step(gamma.dtype)
+    t = (dy.double() * h).abs().sum(0)
+    close(dg, wdg, (rows + 64) * 2.0 ** -24 * t + 2.0 ** -22 * t + hw * wdg.abs() + sub, "dgamma")
+    t = dy.double().abs().sum(0)
+    close(db, wdb, (rows + 64) * 2.0 ** -24 * t + hw * wdb.abs() + sub, "dbeta")
+
+
+SHAPES = [(1, 1), (1, 8), (3, 7), (2, 16), (5, 64), (17, 129), (4, 256), (33, 1000), (7, 1024),
+          (300, 520), (9, 4099), (2, 5120), (400, 2048), (3, 8192), (2, 8200), (2, 12288),
+          (2, 16384), (3, 16392), (1, 16411), (2, 40000), (1200, 24)]
+
+
+@pytest.mark.parametrize("dtype,weight", [("bf16", "f32"), ("bf16", "bf16"), ("f16", "f16"),
+                                          ("f16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_both_passes(nvlib, rows, cols, dtype, weight):
+    x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], TYPES[weight], rows * 3 + cols)
+    mean, rstd = check_forward(nvlib, x, gamma, beta if cols % 2 else None)
+    check_backward(nvlib, x, gamma, dy, res if rows % 2 else None, mean, rstd)
+    check_backward(nvlib, x, gamma, dy, None if rows % 2 else res, mean, rstd)
+    assert nvlib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("pad,shift", [(8, 0), (8, 8), (3, 1)])
+def test_strides(nvlib, dtype, pad, shift):
+    """Rows inside a wider buffer, at aligned and odd places."""
+    rows, cols = 37, 192
+    x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], torch.float32, 5)
+
+    def place(t):
+        buf = torch.full((rows, cols + pad + shift), 9.0, dtype=t.dtype, device="cuda")
+        buf[:, shift:shift + cols] = t.cuda()
+        return buf[:, shift:shift + cols]
+    px, pdy, pres = place(x), place(dy), place(res)
+    mean, rstd = check_forward(nvlib, x, gamma, beta, xd=px)
+    check_backward(nvlib, x, gamma, dy, res, mean, rstd, dev=(px, pdy, pres))
+
+
+def test_offset_and_outliers(nvlib):
+    """A common offset far above the spread, and a first element far off: the
+    statistics keep their digits."""
+    x, gamma, beta, _, _ = make(20, 3000, torch.float32, torch.float32, 8, offset=1000.0)
+    check_forward(nvlib, x, gamma, beta)
+    x, gamma, beta, _, _ = make(20, 4096, torch.bfloat16, torch.float32, 9)
+    x[:, 0] = 500.0
+    check_forward(nvlib, x, gamma, beta)
+
+
+def test_constant_rows_and_nan(nvlib):
+    x, gamma, beta, _, _ = make(6, 512, torch.float32, torch.float32, 4)
+    x[1] = 3.25
+    x[2] = 0.0
+    check_forward(nvlib, x, gamma, beta)
+    x[4, 100] = math.nan
+    x[5, 7] = math.inf
+    amax = torch.empty(1, device="cuda")
+    y, mean, rstd = nvlib.layernorm(x.cuda(), gamma.cuda(), beta.cuda(), EPS, amax_out=amax)
+    y = y.cpu()
+    assert bool(torch.isnan(y[4:]).all()) and bool(torch.isfinite(y[:4]).all())
+    assert math.isnan(float(amax))
+
+
+def test_in_place(nvlib):
+    """y over x, dx over dy and over the residual, through the pointer-level calls."""
+    for rows, cols in ((50, 640), (50, 641), (3, 20001)):
+        x, gamma, beta, dy, res = make(rows, cols, torch.float32, torch.float32, cols)
+        x, gamma, beta, dy, res = (t.cuda() for t in (x, gamma, beta, dy, res))
+        y, mean, rstd = nvlib.layernorm(x, gamma, beta)
+        xx = x.clone()
+        nvlib.layernorm_fwd(rows, cols, xx, cols, gamma, beta, x.dtype, gamma.dtype, EPS, xx, cols,
+                            None, None, None)
+        assert torch.equal(xx, y)
+        dx, dg, db = nvlib.layernorm_backward(dy, x, mean, rstd, gamma, residual=res)
+        nb = nvlib.layernorm_bwd_workspace_bytes(rows, cols)
+        ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+        for over in (dy, res):
+            keep = over.clone()
+            g2, b2 = torch.empty_like(dg), torch.empty_like(db)
+            nvlib.layernorm_bwd(rows, cols, dy, cols, x, cols, mean, rstd, gamma, res, cols,
+                                x.dtype, gamma.dtype, over, cols, g2, b2, ws, nb)
+            assert torch.equal(over, dx) and torch.equal(g2, dg) and torch.equal(b2, db)
+            over.copy_(keep)
+
+
+def test_empty(nvlib):
+    gamma = torch.ones(40, device="cuda")
+    x = torch.empty(0, 40, device="cuda")
+    amax = torch.full((1,), 3.0, device="cuda")
+    y, mean, rstd = nvlib.layernorm(x, gamma, amax_out=amax)
+    assert y.shape == (0, 40) and float(amax) == 0.0
+    dx, dg, db = nvlib.layernorm_backward(x, x, mean, rstd, gamma)
+    assert float(dg.abs().max()) == 0.0 and float(db.abs().max()) == 0.0 and dx.shape == (0, 40)
+
+
+def test_gradient_by_differences(nvlib):
+    """The backward pass is the derivative of the forward pass: central
+    differences of sum(y w) in 64 bits around the fp32 inputs.  With step
+    2^-8 the third-order term is below 2^-16 of the terms' size here."""
+    rows, cols = 3, 24
+    x, gamma, beta, dy, _ = make(rows, cols, torch.float32, torch.float32, 77)
+    _, mean, rstd = nvlib.layernorm(x.cuda(), gamma.cuda(), beta.cuda())
+    dx, dg, db = (t.double().cpu() for t in
+                  nvlib.layernorm_backward(dy.cuda(), x.cuda(), mean, rstd, gamma.cuda()))
+    step = 2.0 ** -8
+
+    def loss(a, ga, be):
+        return float((orc.layernorm(a, ga, be, EPS)[0] * dy.double()).sum())
+    for r, c in ((0, 0), (1, 5), (2, 23)):
+        e = torch.zeros(rows, cols, dtype=torch.float64)
+        e[r, c] = step
+        num = (loss(x.double() + e, gamma, beta) - loss(x.double() - e, gamma, beta)) / (2 * step)
+        assert abs(num - float(dx[r, c])) < 2.0 ** -10
+        v = torch.zeros(cols, dtype=torch.float64)
+        v[c] = step
+        num = (loss(x, gamma.double() + v, beta) - loss(x, gamma.double() - v, beta)) / (2 * step)
+        assert abs(num - float(dg[c])) < 2.0 ** -16
+        num = (loss(x, gamma, beta.double() + v) - loss(x, gamma, beta.double() - v)) / (2 * step)
+        assert abs(num - float(db[c])) < 2.0 ** -16
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 1024), (300, 777)])
+def test_streams_and_capture(nvlib, rows, cols):
+    x, gamma, beta, dy, res = (t.cuda() for t in make(rows, cols, torch.bfloat16, torch.float32, 6))
+    y, mean, rstd = nvlib.layernorm(x, gamma, beta)
+    want = nvlib.layernorm_backward(dy, x, mean, rstd, gamma, residual=res)
+    torch.cuda.synchronize()
+    got = []
+    for s in [torch.cuda.Stream() for _ in range(2)]:
+        with torch.cuda.stream(s):
+            got += [nvlib.layernorm_backward(dy, x, mean, rstd, gamma, residual=res)
+                    for _ in range(3)]
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(p, q) for p, q in zip(g, want))
+    amax = torch.empty(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gy, gm, gr = nvlib.layernorm(x, gamma, beta, amax_out=amax)
+        gg = nvlib.layernorm_backward(dy, x, gm, gr, gamma, residual=res)
+    for k in range(2):
+        x.mul_(0.5)       # the amax of the second replay is not the first one's
+        gamma.mul_(0.5)
+        graph.replay()
+        y, mean, rstd = nvlib.layernorm(x, gamma, beta)
+        want = nvlib.layernorm_backward(dy, x, mean, rstd, gamma, residual=res)
+        torch.cuda.synchronize()
+        assert torch.equal(gy, y) and all(torch.equal(p, q) for p, q in zip(gg, want))
+        assert float(amax) == float(y.float().abs().max())

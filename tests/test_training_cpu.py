@@ -1,0 +1,160 @@
+"""Refusals of the operators around the cast: argument checks that run before
+any CUDA call (placeholder pointers, never used), and the tensor-level checks
+that need no device."""
+import ctypes
+
+import pytest
+import torch
+
+OK, SHAPE, ARG, ALIGN = 0, 1, 2, 3
+P = 4096        # an aligned placeholder address
+
+
+def gemm(lib, m=4, n=8, k=64, A=P, SFA=P, aa=P, B=P, SFB=P, ab=P, D=P, ldd=None, out=1, bias=None,
+         bt=0, res=None, ldr=None, act=0, aux=None, ldaux=None, amax=None):
+    return lib.nvfp4_gemm(m, n, k, A, SFA, aa, B, SFB, ab, D, n if ldd is None else ldd, out, bias,
+                          bt, res, n if ldr is None else ldr, act, aux,
+                          n if ldaux is None else ldaux, amax, 0, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(k=48), SHAPE), (dict(k=16), SHAPE), (dict(k=0), SHAPE), (dict(m=-1), SHAPE),
+    (dict(n=-8), SHAPE), (dict(ldd=7), SHAPE), (dict(res=P, ldr=7), SHAPE),
+    (dict(aux=P, ldaux=7), SHAPE), (dict(m=2**31), SHAPE), (dict(k=2**31), SHAPE),
+    (dict(m=2**30, n=2**30, k=32), SHAPE),
+    (dict(A=None), ARG), (dict(SFA=None), ARG), (dict(aa=None), ARG), (dict(B=None), ARG),
+    (dict(SFB=None), ARG), (dict(ab=None), ARG), (dict(D=None), ARG), (dict(out=3), ARG),
+    (dict(out=-1), ARG), (dict(bias=P, bt=5), ARG), (dict(act=4), ARG), (dict(act=-1), ARG),
+    (dict(A=P + 8), ALIGN), (dict(B=P + 8), ALIGN), (dict(D=P + 1), ALIGN),
+    (dict(D=P + 2, out=0), ALIGN), (dict(res=P + 1), ALIGN), (dict(aux=P + 1), ALIGN),
+    (dict(bias=P + 2), ALIGN), (dict(aa=P + 2), ALIGN), (dict(amax=P + 2), ALIGN),
+    (dict(m=0), OK), (dict(n=0), OK), (dict(m=0, A=None, D=None), OK),
+])
+def test_gemm_refuses(nvlib, kw, want):
+    assert gemm(nvlib.load(), **kw) == want
+
+
+def test_gemm_dact_refuses(nvlib):
+    lib = nvlib.load()
+
+    def call(aux=P, ldaux=8, act=2, dbias=None, ws=None, nbytes=0, m=4, n=8, k=64, amax=None):
+        return lib.nvfp4_gemm_dact(m, n, k, P, P, P, P, P, P, aux, ldaux, act, P, n, 1, dbias,
+                                   amax, ws, nbytes, 0, None)
+    need = lib.nvfp4_gemm_dact_workspace_bytes(4, 8, 64)
+    assert need >= 8 * 4
+    assert call(aux=None) == ARG
+    assert call(ldaux=7) == SHAPE
+    assert call(act=9) == ARG
+    assert call(dbias=P) == ARG                                # no workspace
+    assert call(dbias=P, ws=P, nbytes=need - 1) == ARG         # a short one
+    assert call(dbias=P + 2, ws=P, nbytes=need) == ALIGN
+    assert call(dbias=P, ws=P + 1, nbytes=need) == ALIGN
+    assert lib.nvfp4_gemm_dact_workspace_bytes(0, 8, 64) == 0
+
+
+def test_layernorm_refuses(nvlib):
+    lib = nvlib.load()
+
+    def fwd(rows=4, cols=8, x=P, ldx=8, gamma=P, beta=P, dt=1, wt=0, eps=1e-5, y=P, ldy=8, mean=P,
+            rstd=P, amax=None):
+        return lib.nvfp4_layernorm_fwd(rows, cols, x, ldx, gamma, beta, dt, wt, eps, y, ldy, mean,
+                                       rstd, amax, None)
+    assert fwd(rows=-1) == SHAPE and fwd(cols=-1) == SHAPE and fwd(cols=2**25, ldx=2**25,
+                                                                    ldy=2**25) == SHAPE
+    assert fwd(ldx=7) == SHAPE and fwd(ldy=7) == SHAPE
+    assert fwd(x=None) == ARG and fwd(gamma=None) == ARG and fwd(y=None) == ARG
+    assert fwd(dt=3) == ARG and fwd(dt=1, wt=2) == ARG and fwd(dt=0, wt=1) == ARG
+    assert fwd(eps=-1.0) == ARG and fwd(eps=float("nan")) == ARG
+    assert fwd(x=P + 1) == ALIGN and fwd(gamma=P + 2) == ALIGN and fwd(mean=P + 2) == ALIGN
+    assert fwd(rows=0) == OK and fwd(cols=0) == OK
+
+    need = lib.nvfp4_layernorm_bwd_workspace_bytes(4, 8)
+
+    def bwd(rows=4, cols=8, dy=P, lddy=8, x=P, ldx=8, mean=P, rstd=P, gamma=P, res=None, ldr=8,
+            dt=1, wt=0, dx=P, lddx=8, dg=P, db=P, ws=P, nb=need):
+        return lib.nvfp4_layernorm_bwd(rows, cols, dy, lddy, x, ldx, mean, rstd, gamma, res, ldr,
+                                       dt, wt, dx, lddx, dg, db, ws, nb, None)
+    for kw in (dict(rows=-1), dict(lddy=7), dict(ldx=7), dict(lddx=7), dict(res=P, ldr=7)):
+        assert bwd(**kw) == SHAPE, kw
+    for kw in (dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(gamma=None),
+               dict(dx=None), dict(ws=None), dict(nb=need - 1), dict(dt=7), dict(wt=2)):
+        assert bwd(**kw) == ARG, kw
+    for kw in (dict(dy=P + 1), dict(res=P + 1), dict(dg=P + 2), dict(ws=P + 2)):
+        assert bwd(**kw) == ALIGN, kw
+    assert bwd(cols=0) == OK
+
+
+def test_adamw_refuses(nvlib):
+    from fp4_sm120a_b200._native import AdamWTensor
+    lib = nvlib.load()
+
+    def step(count=1, pt=0, gt=0, st=0, lr=0.1, b1=0.9, b2=0.95, eps=1e-8, t=1, scale=None,
+             scalars=None, amax=None, rng=None, table=True, **fields):
+        base = dict(param=P, grad=P, exp_avg=P, exp_avg_sq=P, exp_avg_scale=None,
+                    exp_avg_sq_scale=None, copy=None, n=10, offset=0, weight_decay=0.0)
+        base.update(fields)
+        arr = (AdamWTensor * 1)(AdamWTensor(**base))
+        return lib.nvfp4_adamw_step(arr if table else None, count, pt, gt, st, lr, b1, b2, eps, t,
+                                    scale, scalars, amax, rng, None)
+    assert step(count=0) == OK and step(count=-1) == SHAPE and step(table=False) == ARG
+    nan = float("nan")
+    for kw in (dict(pt=2), dict(pt=-1), dict(gt=3), dict(st=2), dict(b1=1.0), dict(b1=-0.1),
+               dict(b2=1.0), dict(b2=nan), dict(eps=-1.0), dict(eps=nan), dict(t=0), dict(lr=nan),
+               dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None),
+               dict(weight_decay=nan), dict(pt=1, copy=P),
+               dict(st=1), dict(st=1, rng=P),
+               dict(st=1, rng=P, exp_avg_scale=P, exp_avg_sq_scale=P, offset=64)):
+        assert step(**kw) == ARG, kw
+    for kw in (dict(param=P + 2), dict(grad=P + 2), dict(exp_avg=P + 1), dict(exp_avg_sq=P + 2),
+               dict(copy=P + 1), dict(amax=P + 1), dict(scale=P + 2), dict(scalars=P + 2),
+               dict(rng=P + 4)):
+        assert step(**kw) == ALIGN, kw
+    assert step(n=2**43) == SHAPE
+
+    def unpack(codes=P, scales=P, n=4, moment=0, out=P, dt=0):
+        return lib.nvfp4_adamw_unpack_state(codes, scales, n, moment, out, dt, None)
+    assert unpack(n=0) == OK and unpack(moment=2) == ARG and unpack(dt=2) == ARG
+    assert unpack(codes=None) == ARG and unpack(scales=None) == ARG and unpack(out=None) == ARG
+    assert unpack(out=P + 2) == ALIGN
+
+
+def test_descriptor_layout(nvlib):
+    """The ctypes mirror has the C struct's layout (8 bytes a field)."""
+    from fp4_sm120a_b200._native import AdamWTensor
+    assert ctypes.sizeof(AdamWTensor) == 80
+    assert AdamWTensor.n.offset == 56 and AdamWTensor.weight_decay.offset == 72
+
+
+def test_tensor_level_refuses_host_tensors(nvlib):
+    x, w = torch.zeros(2, 32), torch.ones(32)
+    with pytest.raises(ValueError):
+        nvlib.layernorm(x, w)
+    with pytest.raises(ValueError):
+        nvlib.matmul_nvfp4(x, x, x, x, x, x)
+    with pytest.raises(ValueError):
+        nvlib.adamw_unpack_state(torch.zeros(4, dtype=torch.uint8), torch.zeros(1), "exp_avg")
+    with pytest.raises(ValueError):
+        nvlib.AdamW([w], [w], [w], [w])
+    with pytest.raises(ValueError):
+        nvlib.AdamW([], [], [], [])
+
+
+def test_unknown_names(nvlib):
+    from fp4_sm120a_b200 import ops
+    with pytest.raises(ValueError):
+        ops.gemm_nvfp4(1, 1, 32, None, None, None, None, None, None, None, 1, torch.float32, None,
+                       torch.float32, None, 1, "tanh", None, 1, None, stream=0)
+    with pytest.raises(ValueError):
+        ops.adamw_unpack_state(None, None, 0, "momentum", None, torch.float32, stream=0)
+
+
+def test_workspaces_follow_the_sizes(nvlib):
+    lib = nvlib.load()
+    w = lib.nvfp4_gemm_dact_workspace_bytes
+    for m in (1, 16, 17, 64, 65, 128, 129, 4099, 100000):
+        for n in (1, 128, 5120):
+            b = w(m, n, 4096)
+            assert b % (4 * n) == 0 and b >= 2 * 4 * n
+            assert b <= 4 * n * 2 * 8 * (m // 16 + 1)
+    assert lib.nvfp4_layernorm_bwd_workspace_bytes(10, 7) == 10 * 2 * 7 * 4
+    assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 296 * 2 * 7 * 4
