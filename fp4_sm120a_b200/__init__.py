@@ -13,6 +13,7 @@ from .ops import (  # noqa: F401
     gemm_nvfp4,
     gemm_nvfp4_dact,
     gemm_nvfp4_dact_workspace_bytes,
+    gemm_nvfp4_workspace_bytes,
     hadamard16,
     layernorm_bwd,
     layernorm_bwd_workspace_bytes,

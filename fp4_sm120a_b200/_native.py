@@ -77,7 +77,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                                                    c_int, c_int, c_void_p], c_int),
     "nvfp4_gemm": ([c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                     c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64, c_int,
-                    c_void_p, c_int64, c_void_p, c_uint32, c_void_p], c_int),
+                    c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_uint32, c_void_p], c_int),
+    "nvfp4_gemm_workspace_bytes": ([c_int64, c_int64, c_int64], c_size_t),
     "nvfp4_gemm_dact_workspace_bytes": ([c_int64, c_int64, c_int64], c_size_t),
     "nvfp4_gemm_dact": ([c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int,

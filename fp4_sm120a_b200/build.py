@@ -20,7 +20,7 @@ OBJDIR = PKG / "_build"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["rht_gemm_sm100.cu", "sr_kernels.cu", "fp8_kernels.cu", "fp8_kernels_loose.cu",
-           "gemm_nvfp4_sm100.cu", "layernorm.cu", "adamw.cu"]
+           "gemm_nvfp4_sm100.cu", "gemm_nvfp4_wide_sm100.cu", "layernorm.cu", "adamw.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

@@ -24,7 +24,7 @@
 //               into a ring of 128-byte-swizzled stages
 //   warp  9     MMA issuer: copies a stage's scales to TMEM (tcgen05.cp),
 //               issues four K = 64 MMAs; owns the TMEM columns
-//   warps 10-12 scale loaders: the casts' row-major scales into the 32 x 16
+//   warps 10-   scale loaders: the casts' row-major scales into the 32 x 16
 //               byte atoms that tcgen05.cp spreads over the lanes.  A lane
 //               takes 16 bytes (one k-slice) of rows l, l + 32, l + 64, l + 96,
 //               so the transpose is a choice of registers.
@@ -36,32 +36,14 @@
 #include <cstdint>
 #include <mutex>
 
-#include <cuda.h>
 #include <cudaTypedefs.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
 
-#include "element_io.cuh"
-#include "launch_common.h"
-#include "nvfp4_b200.h"
-#include "nvfp4_device.cuh"
+#include "gemm_nvfp4.cuh"
 
 namespace nvfp4 {
 namespace gemm {
 
-__device__ uint32_t g_gemm_error_word;
-
-constexpr int kTileF = 128;                  // n side: TMEM lanes
-constexpr int kSliceK = 256;                 // codes per k-slice (128 bytes)
-constexpr int kSteps = kSliceK / 64;         // MMAs per k-slice
-constexpr int kEpiWarps = 8;
-constexpr int kEpiThreads = 32 * kEpiWarps;
 constexpr int kWarpTma = 8, kWarpMma = 9, kWarpScales = 10;
-constexpr int kThreads = 32 * 13;
-constexpr uint32_t kAtomBytes = 512;         // scales of 128 rows x one MMA step
-constexpr uint32_t kSmemMax = 227 * 1024;
-constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr int kMaxSplit = 8;
 
 // Tile widths and what follows from them.
@@ -84,7 +66,13 @@ struct Tile {
   static constexpr uint32_t kColsUsed = kAccStages * TN + 2 * kSfCols;
   static constexpr uint32_t kTmemCols = kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;   // + alignment
-  static constexpr int kSfWarps = 1 + kAtomsT;
+  // Scale loaders.  A whole SM's registers pay for two warps a part and turns
+  // of two slices (32 bytes of a row: one sector, not half of one twice).
+  static constexpr int kSfParts = 1 + kAtomsT;
+  static constexpr int kSfPerPart = kCtasPerSm == 1 ? 2 : 1;
+  static constexpr int kSfGroup = kCtasPerSm == 1 ? 2 : 1;
+  static constexpr int kSfAhead = kCtasPerSm == 1 ? 1 : 2;
+  static constexpr int kThreads = 32 * (kWarpScales + kSfParts * kSfPerPart);
   static_assert(kStages >= 3, "the scale columns of slice g - 2 are checked through its stage");
   static_assert(kColsUsed <= 512, "TMEM");
   static_assert(kTmemCols * kCtasPerSm <= 512, "TMEM of all CTAs of an SM");
@@ -93,173 +81,6 @@ struct Tile {
   static constexpr uint32_t kIdesc =
       (1u << 7) | (1u << 10) | ((uint32_t)(TN / 8) << 17) | ((uint32_t)(kTileF / 16) << 24);
 };
-
-enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
-
-struct Params {
-  int m, n, k;
-  int slices;                 // ceil(k / 256)
-  int tiles_f, tiles_t;
-  const uint8_t* sf_f;        // scales of the n side (B), pitch k / 16
-  const uint8_t* sf_t;        // scales of the m side (A)
-  int sf_pitch;
-  int sf_width_f, sf_width_t;   // bytes per scale load: 16, 4 or 1
-  const float* amax_f;
-  const float* amax_t;
-  void* d;
-  int64_t ldd;
-  const void* bias;
-  int bias_dtype;
-  const void* res;            // forward: residual; backward: the activation's argument
-  int64_t ldr;
-  void* aux;
-  int64_t ldaux;
-  int act;
-  float* dbias_partial;       // [partial rows][n]
-  uint32_t* amax;
-};
-
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                     uint32_t err) {
-  return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, err, &g_gemm_error_word);
-}
-
-// tcgen05.mma, block-scaled: D (+)= (A sfa) (B sfb)^T, one E4M3 scale for each
-// 16 elements of a row.
-__device__ __forceinline__ void mma_nvfp4(uint32_t d, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
-      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-// 32 rows of 16 bytes to 32 lanes x 4 columns, repeated for the four warps' lanes.
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-               : "memory");
-}
-
-__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z,
-                                       uint32_t w) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z),
-               "r"(w)
-               : "memory");
-}
-__device__ __forceinline__ void sts_f32(uint32_t addr, float v) {
-  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
-// 16 scale bytes (one k-slice) of a row; bytes behind the row's end are zero.
-__device__ __forceinline__ uint4 load_scales(const uint8_t* sf, int pitch, int width, int row,
-                                             int rows, int slice) {
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-  if (row < rows) {
-    const uint8_t* p = sf + (int64_t)row * pitch + slice * 16;
-    const int left = pitch - slice * 16;
-    if (width == 16) {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      return q;
-    }
-    if (width == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * i < left) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// COLS consecutive fp32 columns of this thread's TMEM lane.
-template <int COLS>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[COLS]) {
-  if constexpr (COLS == 32) {
-    tmem_ld_32cols(taddr, v);
-  } else if constexpr (COLS == 16) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-  } else {
-    static_assert(COLS == 8, "8, 16 or 32 columns");
-    uint32_t r[8];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-  }
-}
-
-// 1 / (1 + exp(-x)) from the hardware's exponential and reciprocal.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
-
-constexpr float kGeluC = 1.5957691216057308f;    // 2 sqrt(2 / pi)
-constexpr float kGeluA = 0.044715f;
-
-// 0.5 z (1 + tanh(c z (1 + a z^2))) = z sigmoid(2 c z (1 + a z^2))
-template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == kRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if constexpr (ACT == kGelu) return z * sigmoid(kGeluC * z * (1.0f + kGeluA * z * z));
-  if constexpr (ACT == kSilu) return z * sigmoid(z);
-  return z;
-}
-template <int ACT>
-__device__ __forceinline__ float slope(float z) {
-  if constexpr (ACT == kRelu) return z > 0.0f ? 1.0f : 0.0f;
-  // Beyond |z| = 64 both slopes are 0 or 1 to the last bit; the clamp keeps
-  // powers of a huge argument from overflowing (and lets NaN through).
-  const float c = fmax_nan(fmin_nan(z, 64.0f), -64.0f);
-  if constexpr (ACT == kGelu) {
-    const float q = sigmoid(kGeluC * c * (1.0f + kGeluA * c * c));
-    return q + c * q * (1.0f - q) * kGeluC * (1.0f + 3.0f * kGeluA * c * c);
-  }
-  if constexpr (ACT == kSilu) {
-    const float q = sigmoid(c);
-    return q + c * q * (1.0f - q);
-  }
-  return 1.0f;
-}
 
 // A thread's share of a tile: one feature (lane) and COLS columns from
 // column c0 on, the accumulator's values in v.
@@ -311,27 +132,8 @@ __device__ __forceinline__ void finish(const Params& p, Out& o, float (&v)[COLS]
   }
 }
 
-__device__ __forceinline__ float load_bias(const Params& p, int f) {
-  if (!p.bias) return 0.0f;
-  if (p.bias_dtype == NVFP4_DTYPE_F32) return reinterpret_cast<const float*>(p.bias)[f];
-  if (p.bias_dtype == NVFP4_DTYPE_BF16)
-    return to_f32(reinterpret_cast<const __nv_bfloat16*>(p.bias)[f]);
-  return to_f32(reinterpret_cast<const __half*>(p.bias)[f]);
-}
-
-// Tiles in an order that keeps a wave's tiles near a square: groups of
-// kGroup column tiles, walked feature tile by feature tile.
-constexpr int kGroup = 8;
-__device__ __forceinline__ void tile_at(const Params& p, int i, int& tf, int& tt) {
-  const int per = kGroup * p.tiles_f;
-  const int g = i / per, in = i - g * per;
-  const int wide = min(kGroup, p.tiles_t - g * kGroup);
-  tf = in / wide;
-  tt = g * kGroup + in - tf * wide;
-}
-
 template <int TN, typename T, bool DACT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
+__global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     k_gemm(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUtensorMap tm_t,
            const Params p) {
   using C = Tile<TN>;
@@ -339,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 2 * C::kAccStages + 1];
   __shared__ uint32_t tmem_holder;
   __shared__ uint32_t abort_word;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar0 = smem_addr(bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };
@@ -351,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 1 + C::kSfWarps);
+      mbar_init(full(s), 1 + C::kSfParts);
       mbar_init(empty(s), 1);
     }
     for (int a = 0; a < C::kAccStages; ++a) {
@@ -418,107 +220,161 @@ __global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
     }
     __syncwarp();
   } else if (warp == kWarpMma) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, g = 0;
-      bool ok = true;
-      for (int i = first; i < tiles && ok; i += stride) {
-        if (!wait(acc_empty(acc), acc_phase ^ 1u, abort_flag, kErrTimeoutMma)) break;
+    // The whole warp walks the loop, so that addresses and descriptors stay
+    // uniform; one elected lane issues.
+    const bool leader = elect_one();
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, set = 0;
+    uint32_t old_stage = 0, old_phase = 0, g = 0;     // of slice g - 2
+    bool ok = true;
+    for (int i = first; i < tiles && ok; i += stride) {
+      if (!wait_warp(acc_empty(acc), acc_phase ^ 1u, abort_flag, kErrTimeoutMma)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + acc * TN;
+      for (int s = s_begin; s < s_end; ++s, ++g) {
+        ok = wait_warp(full(stage), phase, abort_flag, kErrTimeoutMma);
+        // The scale columns alternate between two sets: the MMAs of slice
+        // g - 2 are done with this one when they have freed their stage.
+        // (That stage's next phase needs a commit still to come, so the parity
+        // cannot have moved on.)
+        if (ok && g >= 2) {
+          ok = wait_warp(empty(old_stage), old_phase, abort_flag, kErrTimeoutMma);
+          if (++old_stage == (uint32_t)C::kStages) { old_stage = 0; old_phase ^= 1u; }
+        }
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem + acc * TN;
-        for (int s = s_begin; s < s_end; ++s, ++g) {
-          if (!wait(full(stage), phase, abort_flag, kErrTimeoutMma)) { ok = false; break; }
-          // The scale columns of slice g alternate between two sets: the MMAs
-          // of slice g - 2 are done with this one when they have freed their
-          // stage.  (That stage's next phase needs a commit still to come, so
-          // the parity cannot have moved on.)
-          if (g >= 2) {
-            const uint32_t h = g - 2;
-            if (!wait(empty(h % C::kStages), (h / C::kStages) & 1u, abort_flag, kErrTimeoutMma)) {
-              ok = false;
-              break;
-            }
-          }
-          tc_fence_after();
-          const uint32_t base = ring + stage * C::kStageBytes;
-          const uint32_t sf = base + C::kBytesF + C::kBytesT;
-          const uint32_t sf_f = tmem_sf + (g & 1u) * C::kSfCols, sf_t = sf_f + kSteps * 4;
-          const int steps = min(kSteps, (p.k - s * kSliceK + 63) / 64);
-          for (int q = 0; q < steps; ++q) {
-            cp_scales(sf_f + 4 * q, umma_smem_desc(sf + q * kAtomBytes, 128, 128, 0));
+        const uint32_t base = ring + stage * C::kStageBytes;
+        const uint32_t sf_f = tmem_sf + set * C::kSfCols, sf_t = sf_f + kSteps * 4;
+        const uint64_t desc_f = umma_smem_desc(base, 16, 1024, 2);
+        const uint64_t desc_t = umma_smem_desc(base + C::kBytesF, 16, 1024, 2);
+        const uint64_t desc_s = umma_smem_desc(base + C::kBytesF + C::kBytesT, 128, 128, 0);
+        const int steps = min(kSteps, (p.k - s * kSliceK + 63) / 64);
+        if (leader) {
+          // Addresses within a stage add to the descriptors' address field
+          // (16-byte units; the ring ends below its 18 bits).
+#pragma unroll
+          for (int q = 0; q < kSteps; ++q) {
+            cp_scales(sf_f + 4 * q, desc_s + q * (kAtomBytes / 16));
 #pragma unroll
             for (int b = 0; b < C::kAtomsT; ++b)
               cp_scales(sf_t + 4 * (q * C::kAtomsT + b),
-                        umma_smem_desc(sf + (kSteps * (1 + b) + q) * kAtomBytes, 128, 128, 0));
+                        desc_s + (kSteps * (1 + b) + q) * (kAtomBytes / 16));
           }
-          for (int q = 0; q < steps; ++q)
-            mma_nvfp4(d, umma_smem_desc(base + 32 * q, 16, 1024, 2),
-                      umma_smem_desc(base + C::kBytesF + 32 * q, 16, 1024, 2), C::kIdesc,
-                      sf_f + 4 * q, sf_t + 4 * q * C::kAtomsT, s > s_begin || q > 0);
+#pragma unroll
+          for (int q = 0; q < kSteps; ++q)
+            if (q < steps)
+              mma_nvfp4(d, desc_f + 2 * q, desc_t + 2 * q, C::kIdesc, sf_f + 4 * q,
+                        sf_t + 4 * q * C::kAtomsT, s > s_begin || q > 0);
           tc_commit(empty(stage));
-          if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) break;
-        tc_commit(acc_full(acc));
-        if (++acc == (uint32_t)C::kAccStages) { acc = 0; acc_phase ^= 1u; }
+        __syncwarp();
+        set ^= 1u;
+        if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
       }
-      // All issued work completes before TMEM is released.
-      tc_commit(drain);
-      volatile uint32_t never = 0u;
-      wait(drain, 0, &never, kErrTimeoutDrain);
+      if (!ok) break;
+      if (leader) tc_commit(acc_full(acc));
+      __syncwarp();
+      if (++acc == (uint32_t)C::kAccStages) { acc = 0; acc_phase ^= 1u; }
     }
+    // All issued work completes before TMEM is released.
+    if (leader) tc_commit(drain);
     __syncwarp();
+    volatile uint32_t never = 0u;
+    wait_warp(drain, 0, &never, kErrTimeoutDrain);
   } else if (warp >= kWarpScales) {
-    const int part = warp - kWarpScales;      // 0: n side; 1, 2: m side
-    if (part < C::kSfWarps) {
-      const bool f_side = part == 0;
-      const uint8_t* sf = f_side ? p.sf_f : p.sf_t;
-      const int width = f_side ? p.sf_width_f : p.sf_width_t;
-      const int rows = f_side ? p.n : p.m;
-      const int tile_rows = f_side ? kTileF : min(TN - (part - 1) * 128, 128);
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      // Two k-slices of scales in flight ahead of the one being stored.
-      uint4 buf[3][4];
-      int li = first, ls = s_begin;           // next (tile, slice) to load
-      auto load = [&](uint4 (&b)[4]) {
-        if (li >= tiles) return;
+    // kSfPerPart warps share a part (0: n side; 1, 2: 128 rows each of the m
+    // side) by taking turns; a turn is kSfGroup k-slices of one tile, whose
+    // scales lie side by side in memory.  Each warp keeps kSfAhead turns in
+    // flight ahead of the one it stores.
+    constexpr int G = C::kSfGroup, W = C::kSfPerPart, D = C::kSfAhead;
+    const int part = (warp - kWarpScales) / W, turn0 = (warp - kWarpScales) % W;
+    const bool f_side = part == 0;
+    const uint8_t* sf = f_side ? p.sf_f : p.sf_t;
+    const int width = f_side ? p.sf_width_f : p.sf_width_t;
+    const int rows = f_side ? p.n : p.m;
+    const int tile_rows = f_side ? kTileF : min(TN - (part - 1) * 128, 128);
+    const int per_tile = s_end - s_begin;           // slices
+    const int turns = (per_tile + G - 1) / G;       // a tile's
+    // A cursor over this warp's turns.
+    struct Cursor {
+      int tile, turn;
+    };
+    auto advance = [&](Cursor& c) {
+      for (c.turn += W; c.turn >= turns && c.tile < tiles; c.turn -= turns) c.tile += stride;
+    };
+    uint4 buf[D + 1][G][4];
+    const uint8_t* row[4];                          // this lane's rows, null behind the end
+    int row_tile = -1;
+    auto load = [&](Cursor& c, uint4 (&b)[G][4]) {
+      if (c.tile >= tiles) return;
+      if (c.tile != row_tile) {
+        row_tile = c.tile;
         int tf, tt;
-        tile_at(p, li, tf, tt);
+        tile_at(p, c.tile, tf, tt);
         const int row0 = f_side ? tf * kTileF : tt * TN + (part - 1) * 128;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r = q * 32 + lane;
-          b[q] = load_scales(sf, p.sf_pitch, width, r < tile_rows ? row0 + r : rows, rows, ls);
+          row[q] = r < tile_rows && row0 + r < rows ? sf + (int64_t)(row0 + r) * p.sf_pitch
+                                                    : nullptr;
         }
-        if (++ls == s_end) { ls = s_begin; li += stride; }
-      };
-      auto store = [&](const uint4 (&b)[4]) {
-        if (!__all_sync(0xFFFFFFFFu, wait(empty(stage), phase ^ 1u, abort_flag,
-                                          kErrTimeoutProducer))) {
-          ok = false;
-          return;
+      }
+      const int s = s_begin + c.turn * G;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+          if (s + j < s_end) b[j][q] = load_scales(row[q], p.sf_pitch, width, s + j);
+      }
+      advance(c);
+    };
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    auto skip = [&](int n) {                        // n stages on
+      stage += n;
+      while (stage >= (uint32_t)C::kStages) { stage -= C::kStages; phase ^= 1u; }
+    };
+    Cursor out = {first, 0};                        // the turn whose stage `stage` is
+    auto store = [&](const Cursor& c, const uint4 (&b)[G][4]) {
+      // Stages of the turns in between belong to the other warps.
+      while (out.tile != c.tile || out.turn != c.turn) {
+        skip(min(G, per_tile - out.turn * G));
+        if (++out.turn == turns) { out.turn = 0; out.tile += stride; }
+      }
+      const int n = min(G, per_tile - c.turn * G);
+      uint32_t st = stage, ph = phase;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        if (j < n) {
+          if (!wait_warp(empty(st), ph ^ 1u, abort_flag, kErrTimeoutProducer)) {
+            ok = false;
+            return;
+          }
+          const uint32_t dst = ring + st * C::kStageBytes + C::kBytesF + C::kBytesT +
+                               part * kSteps * kAtomBytes + lane * 16;
+          sts128(dst, b[j][0].x, b[j][1].x, b[j][2].x, b[j][3].x);
+          sts128(dst + kAtomBytes, b[j][0].y, b[j][1].y, b[j][2].y, b[j][3].y);
+          sts128(dst + 2 * kAtomBytes, b[j][0].z, b[j][1].z, b[j][2].z, b[j][3].z);
+          sts128(dst + 3 * kAtomBytes, b[j][0].w, b[j][1].w, b[j][2].w, b[j][3].w);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full(st));
+          if (++st == (uint32_t)C::kStages) { st = 0; ph ^= 1u; }
         }
-        const uint32_t dst = ring + stage * C::kStageBytes + C::kBytesF + C::kBytesT +
-                             part * kSteps * kAtomBytes + lane * 16;
-        sts128(dst, b[0].x, b[1].x, b[2].x, b[3].x);
-        sts128(dst + kAtomBytes, b[0].y, b[1].y, b[2].y, b[3].y);
-        sts128(dst + 2 * kAtomBytes, b[0].z, b[1].z, b[2].z, b[3].z);
-        sts128(dst + 3 * kAtomBytes, b[0].w, b[1].w, b[2].w, b[3].w);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full(stage));
-        if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
-      };
-      const int per_tile = s_end - s_begin;
-      const int64_t total =
-          first < tiles ? (int64_t)((tiles - first + stride - 1) / stride) * per_tile : 0;
-      load(buf[0]);
-      load(buf[1]);
-      for (int64_t j = 0; j < total && ok; j += 3) {
-        load(buf[2]);
-        store(buf[0]);
-        if (j + 1 < total && ok) { load(buf[0]); store(buf[1]); }
-        if (j + 2 < total && ok) { load(buf[1]); store(buf[2]); }
+      }
+    };
+    Cursor in = {first, turn0 - W};                 // the next turn to load
+    advance(in);
+    Cursor done = in;                               // the next turn to store
+#pragma unroll
+    for (int j = 0; j < D; ++j) load(in, buf[j]);
+    while (done.tile < tiles && ok) {
+#pragma unroll
+      for (int u = 0; u <= D; ++u) {
+        if (done.tile < tiles && ok) {
+          load(in, buf[(u + D) % (D + 1)]);
+          store(done, buf[u]);
+          advance(done);
+        }
       }
     }
     __syncwarp();
@@ -540,9 +396,7 @@ __global__ void __launch_bounds__(kThreads, Tile<TN>::kCtasPerSm)
       int tf, tt;
       tile_at(p, i, tf, tt);
       const int f = tf * kTileF + quad * 32 + lane;
-      if (!__all_sync(0xFFFFFFFFu, wait(acc_full(acc), acc_phase, abort_flag,
-                                        kErrTimeoutEpilogue)))
-        break;
+      if (!wait_warp(acc_full(acc), acc_phase, abort_flag, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * TN + group * kHalf;
       if constexpr (SPLIT) {
@@ -654,6 +508,8 @@ __global__ void __launch_bounds__(256) k_dbias(const float* __restrict__ partial
 // Host side
 // ---------------------------------------------------------------------------
 
+namespace {
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -668,24 +524,37 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// Packed codes [rows, k / 2] as bytes, box 128 bytes x `box_rows`, 128-byte swizzle.
-int encode_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t k, int box_rows) {
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, int64_t d0, int64_t d1,
+               int64_t pitch, int b0, int b1, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (!fn) return cuda_status(cudaErrorNotSupported);
-  const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)d0, (cuuint64_t)d1};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)b0, (cuuint32_t)b1};
   const cuuint32_t es[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims,
-                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const CUresult r = fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? NVFP4_OK : cuda_status(cudaErrorInvalidValue);
 }
 
+}  // namespace
+
+int encode_codes_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t k, int box_rows) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, k / 2, rows, k / 2, 128, box_rows,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int encode_words_map(CUtensorMap* map, const void* ptr, int64_t rows) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, ptr, 256, rows, 1024, 256, 2,
+                    CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+namespace {
+
 // Tile width and split, from the sizes alone (148 SMs), so that a workspace
 // can be sized without a device.
 struct Plan {
+  bool wide;
   int tn, split;
   int64_t tiles_f, tiles_t;
   int64_t partial_rows() const { return tiles_t * split * 2; }
@@ -694,21 +563,37 @@ constexpr int kSms = 148;
 
 Plan make_plan(int64_t m, int64_t n, int64_t k) {
   Plan p;
-  p.tiles_f = (n + kTileF - 1) / kTileF;
   const int64_t slices = (k + kSliceK - 1) / kSliceK;
-  if (m <= 16) p.tn = 16;
-  else if (m <= 32) p.tn = 32;
-  else if (m <= 64) p.tn = 64;
-  else if (m <= 128 || p.tiles_f * ((m + 255) / 256) < kSms) p.tn = 128;
-  else p.tn = 256;
-  p.tiles_t = (m + p.tn - 1) / p.tn;
+  p.wide = m > 128;
+  if (p.wide) {
+    // Pairs of CTAs; the narrower tile while the wider leaves pairs without one.
+    p.tiles_f = (n + 255) / 256;
+    p.tn = p.tiles_f * ((m + 255) / 256) < kSms / 2 ? 128 : 256;
+    p.tiles_t = (m + p.tn - 1) / p.tn;
+    p.split = 1;
+    return p;
+  }
+  p.tiles_f = (n + kTileF - 1) / kTileF;
+  p.tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  p.tiles_t = 1;
   // Split k while the tiles leave CTA slots empty and every part keeps at
   // least two slices.
   const int64_t slots = (p.tn < 128 ? 2 : 1) * kSms;
-  int64_t s = p.tn == 256 ? 1 : slots / (p.tiles_f * p.tiles_t);
+  int64_t s = slots / p.tiles_f;
   if (s > slices / 2) s = slices / 2;
   p.split = (int)(s < 1 ? 1 : s > kMaxSplit ? kMaxSplit : s);
   return p;
+}
+
+// Workspace: the bias gradient's partial rows, then the ordered scales.
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+size_t partial_bytes(const Plan& p, int64_t n, bool dbias) {
+  return dbias ? align256((size_t)p.partial_rows() * (size_t)n * sizeof(float)) : 0;
+}
+size_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool dbias) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const Plan p = make_plan(m, n, k);
+  return partial_bytes(p, n, dbias) + (p.wide ? wide_scale_bytes(m, n, k) : 0);
 }
 
 template <int TN, typename T, bool DACT>
@@ -717,7 +602,7 @@ int launch_tile(const Plan& plan, const Params& p, const CUtensorMap& f, const C
   using C = Tile<TN>;
   const int64_t tiles = plan.tiles_f * plan.tiles_t;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -731,13 +616,11 @@ int launch_tile(const Plan& plan, const Params& p, const CUtensorMap& f, const C
     if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, f, t, p)) return cuda_status(e);
     return cuda_status(cudaGetLastError());
   };
-  if constexpr (TN <= 128) {
-    if (plan.split > 1) {
-      cfg.gridDim = dim3((unsigned)(tiles * plan.split));
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      return go(k_gemm<TN, T, DACT, true>);
-    }
+  if (plan.split > 1) {
+    cfg.gridDim = dim3((unsigned)(tiles * plan.split));
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return go(k_gemm<TN, T, DACT, true>);
   }
   const int64_t slots = (int64_t)sms * C::kCtasPerSm;
   cfg.gridDim = dim3((unsigned)(tiles < slots ? tiles : slots));
@@ -751,15 +634,8 @@ int launch_type(const Plan& plan, const Params& p, const CUtensorMap& f, const C
     case 16: return launch_tile<16, T, DACT>(plan, p, f, t, sms, st);
     case 32: return launch_tile<32, T, DACT>(plan, p, f, t, sms, st);
     case 64: return launch_tile<64, T, DACT>(plan, p, f, t, sms, st);
-    case 128: return launch_tile<128, T, DACT>(plan, p, f, t, sms, st);
-    default: return launch_tile<256, T, DACT>(plan, p, f, t, sms, st);
+    default: return launch_tile<128, T, DACT>(plan, p, f, t, sms, st);
   }
-}
-
-int scale_width(const void* sf, int64_t pitch) {
-  if ((uintptr_t)sf % 16 == 0 && pitch % 16 == 0) return 16;
-  if ((uintptr_t)sf % 4 == 0 && pitch % 4 == 0) return 4;
-  return 1;
 }
 
 struct Call {
@@ -800,7 +676,7 @@ int run(const Call& c) {
   if ((uintptr_t)c.a % 16 || (uintptr_t)c.b % 16 || (uintptr_t)c.d % es ||
       (uintptr_t)c.res % es || (uintptr_t)c.aux % es || (c.bias && (uintptr_t)c.bias % bs) ||
       (uintptr_t)c.amax_a % 4 || (uintptr_t)c.amax_b % 4 || (uintptr_t)c.amax_out % 4 ||
-      (uintptr_t)c.dbias % 4 || (uintptr_t)c.ws % 4)
+      (uintptr_t)c.dbias % 4)
     return NVFP4_ERR_MISALIGNED;
   const bool empty = c.m == 0 || c.n == 0;
   // k = 0 would be an empty sum; no cast writes such an operand.
@@ -810,9 +686,9 @@ int run(const Call& c) {
       return NVFP4_ERR_INVALID_ARGUMENT;
     const Plan plan = make_plan(c.m, c.n, c.k);
     if (plan.tiles_f * plan.tiles_t > (1ll << 28)) return NVFP4_ERR_INVALID_SHAPE;
-    if (c.dbias &&
-        (!c.ws || c.ws_bytes < (size_t)plan.partial_rows() * (size_t)c.n * sizeof(float)))
-      return NVFP4_ERR_INVALID_ARGUMENT;
+    const size_t need = workspace_bytes(c.m, c.n, c.k, c.dbias != nullptr);
+    if (need && (!c.ws || c.ws_bytes < need)) return NVFP4_ERR_INVALID_ARGUMENT;
+    if (need && (uintptr_t)c.ws % 256) return NVFP4_ERR_MISALIGNED;
   }
   if (empty && !c.amax_out && !(c.dbias && c.n)) return NVFP4_OK;
   int sms = 0;
@@ -827,9 +703,6 @@ int run(const Call& c) {
     return NVFP4_OK;
   }
   const Plan plan = make_plan(c.m, c.n, c.k);
-  CUtensorMap map_f, map_t;
-  if (int e = encode_map(&map_f, c.b, c.n, c.k, kTileF)) return e;
-  if (int e = encode_map(&map_t, c.a, c.m, c.k, plan.tn)) return e;
   Params p = {};
   p.m = (int)c.m;
   p.n = (int)c.n;
@@ -855,30 +728,43 @@ int run(const Call& c) {
   p.act = c.act;
   p.dbias_partial = c.dbias ? reinterpret_cast<float*>(c.ws) : nullptr;
   p.amax = reinterpret_cast<uint32_t*>(c.amax_out);
+  const int64_t per16 = 16 / (int64_t)es;
+  p.vec = ((uintptr_t)c.d % 16 | (uintptr_t)c.res % 16 | (uintptr_t)c.aux % 16 |
+           (uintptr_t)(c.ldd % per16) | (uintptr_t)(c.res ? c.ldr % per16 : 0) |
+           (uintptr_t)(c.aux ? c.ldaux % per16 : 0)) == 0;
+  CUtensorMap map_f, map_t;
   auto typed = [&](auto t) {
     using T = decltype(t);
     return c.dact ? launch_type<T, true>(plan, p, map_f, map_t, sms, c.st)
                   : launch_type<T, false>(plan, p, map_f, map_t, sms, c.st);
   };
-  const int e = c.dtype == NVFP4_DTYPE_F32    ? typed(float())
-                : c.dtype == NVFP4_DTYPE_BF16 ? typed(__nv_bfloat16())
-                                              : typed(__half());
+  int e;
+  if (plan.wide) {
+    e = launch_wide(c.dtype, c.dact, plan.tn, p, c.a, c.b,
+                    reinterpret_cast<unsigned char*>(c.ws) +
+                        partial_bytes(plan, c.n, c.dbias != nullptr),
+                    sms, c.st);
+  } else {
+    if (int r = encode_codes_map(&map_f, c.b, c.n, c.k, kTileF)) return r;
+    if (int r = encode_codes_map(&map_t, c.a, c.m, c.k, plan.tn)) return r;
+    e = c.dtype == NVFP4_DTYPE_F32    ? typed(float())
+        : c.dtype == NVFP4_DTYPE_BF16 ? typed(__nv_bfloat16())
+                                      : typed(__half());
+  }
   if (e || !c.dbias) return e;
   k_dbias<<<(unsigned)((c.n + 31) / 32), 256, 0, c.st>>>(p.dbias_partial,
                                                          (int)plan.partial_rows(), p.n, c.dbias);
   return cuda_status(cudaGetLastError());
 }
 
+}  // namespace
 }  // namespace gemm
 
 int gemm_device_error(uint32_t* code, int clear) {
-  if (cudaError_t e = cudaMemcpyFromSymbol(code, gemm::g_gemm_error_word, sizeof(uint32_t)))
-    return cuda_status(e);
-  if (clear && *code) {
-    const uint32_t zero = 0;
-    if (cudaError_t e = cudaMemcpyToSymbol(gemm::g_gemm_error_word, &zero, sizeof(uint32_t)))
-      return cuda_status(e);
-  }
+  uint32_t wide = 0;
+  if (int e = gemm::read_error_word(code, clear)) return e;
+  if (int e = gemm::wide_device_error(&wide, clear)) return e;
+  if (*code == 0) *code = wide;
   return NVFP4_OK;
 }
 
@@ -890,8 +776,8 @@ NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const v
                          const float* amax_a, const void* B, const void* SFB, const float* amax_b,
                          void* D, int64_t ldd, int out_dtype, const void* bias, int bias_dtype,
                          const void* residual, int64_t ldr, int activation, void* aux,
-                         int64_t ldaux, float* amax_out, uint32_t sm_count,
-                         nvfp4_stream_t stream) {
+                         int64_t ldaux, float* amax_out, void* workspace, size_t workspace_bytes,
+                         uint32_t sm_count, nvfp4_stream_t stream) {
   nvfp4::gemm::Call c = {};
   c.m = m; c.n = n; c.k = k;
   c.a = A; c.sfa = SFA; c.amax_a = amax_a;
@@ -902,14 +788,18 @@ NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const v
   c.act = activation;
   c.aux = aux; c.ldaux = ldaux;
   c.amax_out = amax_out;
+  c.ws = workspace; c.ws_bytes = workspace_bytes;
   c.sm_count = sm_count;
   c.st = (cudaStream_t)stream;
   return nvfp4::gemm::run(c);
 }
 
+NVFP4_API size_t nvfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  return nvfp4::gemm::workspace_bytes(m, n, k, false);
+}
+
 NVFP4_API size_t nvfp4_gemm_dact_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
-  return (size_t)nvfp4::gemm::make_plan(m, n, k).partial_rows() * (size_t)n * sizeof(float);
+  return nvfp4::gemm::workspace_bytes(m, n, k, true);
 }
 
 NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,

@@ -230,13 +230,17 @@ def _activation(name: str) -> int:
 
 def gemm_nvfp4(m: int, n: int, k: int, A: Ptr, SFA: Ptr, amax_a: Ptr, B: Ptr, SFB: Ptr,
                amax_b: Ptr, D: Ptr, ldd: int, out_dtype, bias: Ptr, bias_dtype, residual: Ptr,
-               ldr: int, activation: str, aux: Ptr, ldaux: int, amax_out: Ptr, sm_count: int = 0,
-               stream=None) -> None:
+               ldr: int, activation: str, aux: Ptr, ldaux: int, amax_out: Ptr, workspace: Ptr,
+               workspace_bytes: int, sm_count: int = 0, stream=None) -> None:
     """nvfp4_gemm: D = act(A B^T + bias) + residual of two NVFP4 operands."""
     call("nvfp4_gemm", m, n, k, _ptr(A), _ptr(SFA), _ptr(amax_a), _ptr(B), _ptr(SFB),
          _ptr(amax_b), _ptr(D), ldd, _dtype_code(out_dtype), _ptr(bias), _dtype_code(bias_dtype),
-         _ptr(residual), ldr, _activation(activation), _ptr(aux), ldaux, _ptr(amax_out), sm_count,
-         _stream(stream))
+         _ptr(residual), ldr, _activation(activation), _ptr(aux), ldaux, _ptr(amax_out),
+         _ptr(workspace), workspace_bytes, sm_count, _stream(stream))
+
+
+def gemm_nvfp4_workspace_bytes(m: int, n: int, k: int) -> int:
+    return load().nvfp4_gemm_workspace_bytes(m, n, k)
 
 
 def gemm_nvfp4_dact_workspace_bytes(m: int, n: int, k: int) -> int:

@@ -112,9 +112,11 @@ def matmul_nvfp4(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Tensor, 
     ldr = n if residual is None else _rows(residual, (m, n), out.dtype, "residual")
     _word(amax_out, "amax_out")
     aux = torch.empty((m, n), dtype=out.dtype, device=a.device) if with_aux else None
+    nbytes = ops.gemm_nvfp4_workspace_bytes(m, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     ops.gemm_nvfp4(m, n, k, a, a_scales, a_amax, b, b_scales, b_amax, out, ldd, out.dtype, bias,
                    torch.float32 if bias is None else bias.dtype, residual, ldr, activation, aux,
-                   n, amax_out)
+                   n, amax_out, ws, nbytes)
     return out, aux
 
 
@@ -132,12 +134,13 @@ def matmul_nvfp4_dact(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Ten
     ldaux = _rows(aux, (m, n), aux.dtype, "aux")
     _word(amax_out, "amax_out")
     d = torch.empty((m, n), dtype=aux.dtype, device=a.device)
-    dbias = ws = None
-    nbytes = 0
+    dbias = None
     if with_dbias:
         dbias = torch.empty(n, dtype=torch.float32, device=a.device)
         nbytes = ops.gemm_nvfp4_dact_workspace_bytes(m, n, k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+    else:
+        nbytes = ops.gemm_nvfp4_workspace_bytes(m, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     ops.gemm_nvfp4_dact(m, n, k, a, a_scales, a_amax, b, b_scales, b_amax, aux, ldaux, activation,
                         d, n, d.dtype, dbias, amax_out, ws, nbytes)
     return d, dbias

@@ -289,23 +289,27 @@ enum { NVFP4_ACT_NONE = 0, NVFP4_ACT_RELU = 1, NVFP4_ACT_GELU = 2, NVFP4_ACT_SIL
  *   aux         receives z (what the backward pass needs), or NULL
  *   amax_out    receives max |D| as stored, NaN-propagating (what the cast of
  *               D needs; enqueues a 4-byte memset), or NULL
+ *   workspace   scratch of nvfp4_gemm_workspace_bytes(m, n, k) bytes, 256-byte
+ *               aligned (0 bytes: may be NULL); it needs no initial state and
+ *               keeps none, but no two calls may use it at the same time
  *   sm_count    0: all SMs; else a cap on the persistent grid (a call short
  *               enough to split k over a cluster takes its own grid)
- * Accumulates in fp32; each output is rounded once.  Results repeat bit for
- * bit.  k % 32 == 0 and k > 0; A and B 16-byte aligned; m, n any size (0: a
+ * Accumulates in fp32; each output is rounded once.  The same call gives the
+ * same bits.  k % 32 == 0 and k > 0; A and B 16-byte aligned; m, n any size (0: a
  * no-op but for *amax_out = 0); m, n, k <= 2^30. */
+NVFP4_API size_t nvfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
                          const float* amax_a, const void* B, const void* SFB, const float* amax_b,
                          void* D, int64_t ldd, int out_dtype, const void* bias, int bias_dtype,
                          const void* residual, int64_t ldr, int activation, void* aux,
-                         int64_t ldaux, float* amax_out, uint32_t sm_count,
-                         nvfp4_stream_t stream);
+                         int64_t ldaux, float* amax_out, void* workspace, size_t workspace_bytes,
+                         uint32_t sm_count, nvfp4_stream_t stream);
 
 /* The product in the backward pass of an activation: D = (A B^T) act'(aux)
  * with the aux that nvfp4_gemm wrote (type out_dtype; may be D itself), and
  * dbias[j] = sum_i D[i, j] (fp32, before D is rounded; NULL: not computed).
- * `workspace` is scratch of nvfp4_gemm_dact_workspace_bytes(m, n, k) bytes,
- * needed with dbias only; it needs no initial state and keeps none. */
+ * `workspace` as in nvfp4_gemm, of nvfp4_gemm_dact_workspace_bytes(m, n, k)
+ * bytes (without dbias nvfp4_gemm_workspace_bytes suffices). */
 NVFP4_API size_t nvfp4_gemm_dact_workspace_bytes(int64_t m, int64_t n, int64_t k);
 NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
                               const float* amax_a, const void* B, const void* SFB,

@@ -264,8 +264,9 @@ def test_empty(nvlib):
 
 @pytest.mark.parametrize("m,n,k", [(3, 700, 4096), (700, 300, 256), (2400, 2304, 512)])
 def test_repeats_and_sm_cap(nvlib, m, n, k):
-    """The same bits on every call, on another stream, two calls at once, and
-    with a capped grid; a captured call replays on new inputs."""
+    """The same bits on every call, on another stream and two calls at once; with
+    a capped grid the same D, and a bias gradient added in another order; a
+    captured call replays on new inputs."""
     a, b, _, _ = problem(m, n, k, 21)
     a, b = cuda(a), cuda(b)
     aux = torch.randn(m, n, device="cuda").to(torch.bfloat16)
@@ -287,7 +288,10 @@ def test_repeats_and_sm_cap(nvlib, m, n, k):
     db = torch.empty_like(wb)
     nvlib.gemm_nvfp4_dact(m, n, k, *a, *b, aux, n, "gelu", d, n, d.dtype, db, None, ws, nb,
                           sm_count=5)
-    assert torch.equal(d, want) and torch.equal(db, wb)
+    assert torch.equal(d, want)
+    # fewer CTAs give a tile another accumulator, whose columns are taken in the
+    # other direction: m additions of fp32 values either way
+    close(db, wb.double().cpu(), (m + 40) * 2.0 ** -23 * want.double().abs().sum(0).cpu(), "dbias, capped grid")
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         gd, gb = nvlib.matmul_nvfp4_dact(*a, *b, aux, activation="gelu", with_dbias=True)

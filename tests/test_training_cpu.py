@@ -11,10 +11,10 @@ P = 4096        # an aligned placeholder address
 
 
 def gemm(lib, m=4, n=8, k=64, A=P, SFA=P, aa=P, B=P, SFB=P, ab=P, D=P, ldd=None, out=1, bias=None,
-         bt=0, res=None, ldr=None, act=0, aux=None, ldaux=None, amax=None):
+         bt=0, res=None, ldr=None, act=0, aux=None, ldaux=None, amax=None, ws=None, nb=0):
     return lib.nvfp4_gemm(m, n, k, A, SFA, aa, B, SFB, ab, D, n if ldd is None else ldd, out, bias,
                           bt, res, n if ldr is None else ldr, act, aux,
-                          n if ldaux is None else ldaux, amax, 0, None)
+                          n if ldaux is None else ldaux, amax, ws, nb, 0, None)
 
 
 @pytest.mark.parametrize("kw,want", [
@@ -28,6 +28,8 @@ def gemm(lib, m=4, n=8, k=64, A=P, SFA=P, aa=P, B=P, SFB=P, ab=P, D=P, ldd=None,
     (dict(A=P + 8), ALIGN), (dict(B=P + 8), ALIGN), (dict(D=P + 1), ALIGN),
     (dict(D=P + 2, out=0), ALIGN), (dict(res=P + 1), ALIGN), (dict(aux=P + 1), ALIGN),
     (dict(bias=P + 2), ALIGN), (dict(aa=P + 2), ALIGN), (dict(amax=P + 2), ALIGN),
+    (dict(m=500, n=512), ARG), (dict(m=500, n=512, ws=P, nb=1024), ARG),
+    (dict(m=500, n=512, ws=P + 16, nb=1 << 20), ALIGN),
     (dict(m=0), OK), (dict(n=0), OK), (dict(m=0, A=None, D=None), OK),
 ])
 def test_gemm_refuses(nvlib, kw, want):
@@ -143,18 +145,24 @@ def test_unknown_names(nvlib):
     from fp4_sm120a_b200 import ops
     with pytest.raises(ValueError):
         ops.gemm_nvfp4(1, 1, 32, None, None, None, None, None, None, None, 1, torch.float32, None,
-                       torch.float32, None, 1, "tanh", None, 1, None, stream=0)
+                       torch.float32, None, 1, "tanh", None, 1, None, None, 0, stream=0)
     with pytest.raises(ValueError):
         ops.adamw_unpack_state(None, None, 0, "momentum", None, torch.float32, stream=0)
 
 
 def test_workspaces_follow_the_sizes(nvlib):
     lib = nvlib.load()
-    w = lib.nvfp4_gemm_dact_workspace_bytes
+    plain, dact = lib.nvfp4_gemm_workspace_bytes, lib.nvfp4_gemm_dact_workspace_bytes
     for m in (1, 16, 17, 64, 65, 128, 129, 4099, 100000):
         for n in (1, 128, 5120):
-            b = w(m, n, 4096)
-            assert b % (4 * n) == 0 and b >= 2 * 4 * n
-            assert b <= 4 * n * 2 * 8 * (m // 16 + 1)
+            for k in (32, 4096):
+                a, b = plain(m, n, k), dact(m, n, k)
+                assert a % 256 == 0 and b % 256 == 0
+                # two partial rows at least; scales: 8 bytes for 128 codes, in
+                # whole blocks of 128 rows x 256 codes
+                assert b - a >= 2 * 4 * n
+                assert a in (0, (-(-m // 128) + -(-n // 128)) * -(-k // 256) * 2048)
+    assert plain(128, 5120, 4096) == 0
+    assert plain(0, 8, 64) == dact(4, 0, 64) == 0
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10, 7) == 10 * 2 * 7 * 4
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 296 * 2 * 7 * 4
