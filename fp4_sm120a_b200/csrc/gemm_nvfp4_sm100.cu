@@ -557,7 +557,7 @@ struct Plan {
   bool wide;
   int tn, split;
   int64_t tiles_f, tiles_t;
-  int64_t partial_rows() const { return tiles_t * split * 2; }
+  int64_t partial_rows() const { return tiles_t * (wide ? 4 : 2 * split); }
 };
 constexpr int kSms = 148;
 

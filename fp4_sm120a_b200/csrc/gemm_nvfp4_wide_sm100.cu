@@ -19,9 +19,9 @@
 // epilogue of a tile takes the shared columns first, and the next tile's
 // products start when these (not the whole accumulator) have been read.
 //
-// Warps: 0-7 epilogue, 8 TMA producer, 9 MMA issuer (of the pair's first CTA).
-// Epilogue: a warp's 32 lanes (features) x 32 columns (tokens) are turned
-// around through 4 KB of shared memory, after which a thread holds eight
+// Warps: 0-15 epilogue, 16 TMA producer, 17 MMA issuer (of the pair's first
+// CTA).  Epilogue: a warp's 32 lanes (features) x 32 columns (tokens) are turned
+// around through 2 KB of shared memory, after which a thread holds eight
 // consecutive features of a token: bias, activation, residual and the stores
 // work on 16-byte vectors.
 #include "gemm_nvfp4.cuh"
@@ -30,8 +30,12 @@ namespace nvfp4 {
 namespace gemm {
 namespace {
 
-constexpr int kWarpTma = 8, kWarpMma = 9;
-constexpr int kThreads = 32 * 10;
+// Sixteen epilogue warps: four column groups of four warps (TMEM lane quarters).
+constexpr int kPairEpiWarps = 16, kGroups = kPairEpiWarps / 4;
+constexpr int kWarpTma = kPairEpiWarps, kWarpMma = kPairEpiWarps + 1;
+constexpr int kThreads = 32 * (kPairEpiWarps + 2);
+constexpr int kTurnRows = 16;                                // tokens turned around at once
+constexpr uint32_t kTurnWarp = kTurnRows * 128;
 
 template <int TN>
 struct Wide {
@@ -40,7 +44,7 @@ struct Wide {
   static constexpr uint32_t kBytesT = TN / 2 * 128;          // this CTA's half
   static constexpr uint32_t kBytesSf = kSteps * (1 + kAtomsT) * kAtomBytes;
   static constexpr uint32_t kStageBytes = kBytesF + kBytesT + kBytesSf;
-  static constexpr uint32_t kTurnBytes = kEpiWarps * 4096;
+  static constexpr uint32_t kTurnBytes = kPairEpiWarps * kTurnWarp;
   static constexpr int kStagesRaw = (int)((kSmemMax - 2048 - kTurnBytes) / kStageBytes);
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kTurnBytes + 1024;
@@ -49,13 +53,13 @@ struct Wide {
   static constexpr int kOverlap = 2 * TN > kFree ? 2 * TN - kFree : 0;
   static constexpr int kAcc1 = TN - kOverlap;                // second accumulator's first column
   static constexpr int kChunks = TN / 32;
-  static constexpr int kTurns = kChunks / 2;                 // per column group
+  static constexpr int kTurns = kChunks / kGroups;           // per column group
   // Turns whose columns the next tile's products overwrite.
-  static constexpr int kEarly = (kOverlap + 63) / 64;
+  static constexpr int kEarly = (kOverlap + 32 * kGroups - 1) / (32 * kGroups);
   static constexpr uint32_t kIdesc =
       (1u << 7) | (1u << 10) | ((uint32_t)(TN / 8) << 17) | ((uint32_t)(256 / 16) << 24);
   static_assert(kStages >= 3, "the scale columns of slice g - 2 are checked through its stage");
-  static_assert(kEarly <= 2, "columns held in registers");
+  static_assert(kEarly <= 1 && kTurns >= 1, "columns held in registers");
 };
 
 // TMA load by a CTA of a pair into its own shared memory, completing on the
@@ -98,15 +102,6 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void grid_dependency_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 // Eight consecutive elements of T as loaded from memory.
 template <typename T>
 struct Raw8 {
@@ -227,56 +222,61 @@ __device__ __forceinline__ void finish8(const Params& p, Acc& o, float (&x)[8], 
 }
 
 // A warp's chunk: lane l holds feature l's accumulators of the tokens t0 ..
-// t0 + 31 in v.  `turn` is the warp's 4 KB: row = token, 16-byte units of a
+// t0 + 31 in v.  `turn` is the warp's 2 KB: row = token, 16-byte units of a
 // row swapped by the token's parity so that neither side meets a bank twice.
 template <typename T, bool DACT>
 __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const float (&v)[32],
-                                             uint32_t turn, int lane, int t0) {
-  Raw8<T> r[4];
-  const int row0 = lane >> 2;
+                                             float* turn, int lane, int t0) {
+  constexpr int kRows = kTurnRows / 8;         // tokens of a thread at a time
   const T* res = reinterpret_cast<const T*>(p.res);
-  if (DACT || p.res) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t t = t0 + row0 + 8 * i;
-      if (t < p.m) {
-        if (p.vec && o.f + 8 <= p.n) {
-          r[i].load(res + t * p.ldr + o.f);
-        } else {
-          float e[8];
+  for (int h = 0; h < 32; h += kTurnRows) {
+    Raw8<T> r[kRows];
+    const int row0 = lane >> 2;
+    if (DACT || p.res) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            e[j] = o.f + j < p.n ? to_f32(res[t * p.ldr + o.f + j]) : 0.0f;
-          r[i].set(e);
+      for (int i = 0; i < kRows; ++i) {
+        const int64_t t = t0 + h + row0 + 8 * i;
+        if (t < p.m) {
+          if (p.vec && o.f + 8 <= p.n) {
+            r[i].load(res + t * p.ldr + o.f);
+          } else {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              e[j] = o.f + j < p.n ? to_f32(res[t * p.ldr + o.f + j]) : 0.0f;
+            r[i].set(e);
+          }
         }
       }
     }
-  }
-  __syncwarp();
+    __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    sts_f32(turn + j * 128 + ((((lane >> 2) ^ (j & 1)) << 4) | ((lane & 3) << 2)), v[j]);
-  __syncwarp();
-  auto all = [&](auto act) {
+    for (int j = 0; j < kTurnRows; ++j)
+      turn[j * 32 + ((((lane >> 2) ^ (j & 1)) << 2) | (lane & 3))] = v[h + j];
+    __syncwarp();
+    float x[kRows][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + 8 * i;
-      const uint32_t at = turn + row * 128;
-      const uint32_t u = (lane & 3) * 2;
-      const uint4 a = lds128(at + ((u ^ (row & 1)) << 4));
-      const uint4 b = lds128(at + (((u + 1) ^ (row & 1)) << 4));
-      float x[8] = {__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z),
-                    __uint_as_float(a.w), __uint_as_float(b.x), __uint_as_float(b.y),
-                    __uint_as_float(b.z), __uint_as_float(b.w)};
-      if (t0 + row < p.m && o.f < p.n)
-        finish8<T, DACT, decltype(act)::value>(p, o, x, r[i], t0 + row);
+    for (int i = 0; i < kRows; ++i) {
+      const int row = row0 + 8 * i, u = (lane & 3) * 2;
+      const float4 a = *reinterpret_cast<const float4*>(turn + row * 32 + ((u ^ (row & 1)) << 2));
+      const float4 b =
+          *reinterpret_cast<const float4*>(turn + row * 32 + (((u + 1) ^ (row & 1)) << 2));
+      x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+      x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
     }
-  };
-  switch (p.act) {
-    case kRelu: all(Const<kRelu>()); break;
-    case kGelu: all(Const<kGelu>()); break;
-    case kSilu: all(Const<kSilu>()); break;
-    default: all(Const<kNone>()); break;
+    auto all = [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        if (t0 + h + row0 + 8 * i < p.m && o.f < p.n)
+          finish8<T, DACT, decltype(act)::value>(p, o, x[i], r[i], t0 + h + row0 + 8 * i);
+    };
+    switch (p.act) {
+      case kRelu: all(Const<kRelu>()); break;
+      case kGelu: all(Const<kGelu>()); break;
+      case kSilu: all(Const<kSilu>()); break;
+      default: all(Const<kNone>()); break;
+    }
   }
 }
 
@@ -308,7 +308,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full(a), 1);
-      mbar_init(acc_free(a), 2 * kEpiWarps);   // both CTAs' epilogue warps
+      mbar_init(acc_free(a), 2 * kPairEpiWarps);   // both CTAs' epilogue warps
     }
     mbar_init(drain, 1);
     abort_word = 0u;
@@ -448,7 +448,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else {
     const int group = warp >> 2, quad = warp & 3;
-    const uint32_t turn = ring + C::kStages * C::kStageBytes + warp * 4096;
+    float* turn = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) +
+                                           C::kStages * C::kStageBytes + warp * kTurnWarp);
     Acc o;
     o.top = 0u;
     {
@@ -472,31 +473,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // Chunk of this group's turn u: the first accumulator shares its last
       // columns with the second, the second its first ones.
       auto chunk = [&](int u) {
-        const int c = 2 * u + group;
+        const int c = kGroups * u + group;
         return a ? c : C::kChunks - 1 - c;
       };
-      auto release = [&]() {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_cluster(map_rank(acc_free(a), 0));
-      };
-      if constexpr (C::kEarly > 0) {
-        // The shared columns to registers first.
-        float v[C::kEarly][32];
-#pragma unroll
-        for (int u = 0; u < C::kEarly; ++u) tmem_ld_32cols(src + 32 * chunk(u), v[u]);
-        tc_wait_ld();
-        release();
-#pragma unroll
-        for (int u = 0; u < C::kEarly; ++u)
-          finish_chunk<T, DACT>(p, o, v[u], turn, lane, tt * TN + 32 * chunk(u));
-      }
+      // The accumulator's columns are free for the next products once the last
+      // turn (or, with an overlap, the last shared one) is in registers.
+      constexpr int kLast = C::kEarly > 0 ? C::kEarly - 1 : C::kTurns - 1;
 #pragma unroll 1
-      for (int u = C::kEarly; u < C::kTurns; ++u) {
+      for (int u = 0; u < C::kTurns; ++u) {
         float v[32];
         tmem_ld_32cols(src + 32 * chunk(u), v);
         tc_wait_ld();
-        if (C::kEarly == 0 && u == C::kTurns - 1) release();
+        if (u == kLast) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_cluster(map_rank(acc_free(a), 0));
+        }
         finish_chunk<T, DACT>(p, o, v, turn, lane, tt * TN + 32 * chunk(u));
       }
       if (DACT && p.dbias_partial) {
@@ -507,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int k = 4; k < 32; k <<= 1)
             o.dbias[j] += __shfl_xor_sync(0xFFFFFFFFu, o.dbias[j], k);
           if (lane < 4 && o.f + j < p.n)
-            p.dbias_partial[(int64_t)(tt * 2 + group) * p.n + o.f + j] = o.dbias[j];
+            p.dbias_partial[(int64_t)(tt * kGroups + group) * p.n + o.f + j] = o.dbias[j];
         }
       }
     }
