@@ -62,6 +62,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack_one(float x) {
+  if constexpr (sizeof(T) == 4) return __float_as_uint(x);
+  else return pack2<T>(x, 0.0f);
+}
+
 // VEC consecutive elements: 16 bytes, or one element.
 template <typename T, int VEC>
 struct Pack {
@@ -105,14 +111,44 @@ __device__ __forceinline__ Pack<T, VEC> zero_pack() {
   return r;
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store_global(T* p, const float (&x)[VEC]) {
+__device__ __forceinline__ Pack<T, VEC> pack(const float (&x)[VEC]) {
+  Pack<T, VEC> r;
   if constexpr (VEC == 1) {
-    *p = from_f32<T>(x[0]);
+    r.w[0] = pack_one<T>(x[0]);
   } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = __float_as_uint(x[k]);
   } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                              pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = pack2<T>(x[2 * k], x[2 * k + 1]);
+  }
+  return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_global(T* p, const Pack<T, VEC>& r) {
+  if constexpr (VEC == 1) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = r.w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)r.w[0];
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  }
+}
+// Unsigned maximum of the magnitudes' bit patterns, per 16-bit half or per
+// word (NaN patterns are above infinity's), and its value as fp32 bits.
+template <typename T, int VEC>
+__device__ __forceinline__ uint32_t pack_top(uint32_t m, const Pack<T, VEC>& r) {
+#pragma unroll
+  for (int k = 0; k < Pack<T, VEC>::kWords; ++k)
+    m = sizeof(T) == 4 ? max(m, r.w[k] & 0x7FFFFFFFu) : __vmaxu2(m, r.w[k] & 0x7FFF7FFFu);
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  else {
+    float lo, hi;
+    unpack2<T>(m, lo, hi);
+    return max(__float_as_uint(lo), __float_as_uint(hi));
   }
 }
 
@@ -124,20 +160,35 @@ struct Ring {
 
 struct Shared {
   uint64_t bar[kMaxStages];
-  float red[2][2][kMaxWarps];
+  float2 red[2][kMaxWarps];
   uint32_t abort_flag;
   uint32_t pad[3];
 };
 
-// Stage of the block's k-th row and the parity its barrier completes with.
-__device__ __forceinline__ uint32_t ring_stage(const Ring& r, uint32_t k) { return k % r.stages; }
-__device__ __forceinline__ uint32_t ring_parity(const Ring& r, uint32_t k) {
-  return (k / r.stages) & 1u;
-}
-__device__ __forceinline__ bool ring_wait(const Ring& r, uint32_t k,
+// Position of a row in the ring: its stage and the parity its barrier completes
+// with.
+struct RingAt {
+  uint32_t stage = 0, parity = 0;
+  __device__ __forceinline__ void next(const Ring& r) {
+    if (++stage == (uint32_t)r.stages) { stage = 0; parity ^= 1u; }
+  }
+};
+__device__ __forceinline__ bool ring_wait(const Ring& r, const RingAt& at,
                                           volatile uint32_t* abort_flag) {
-  return mbar_wait_bounded(r.bar + 8 * ring_stage(r, k), ring_parity(r, k), abort_flag,
-                           kWaitLimitNs, kErrTimeoutProducer, &g_layernorm_error_word);
+  return mbar_wait_bounded(r.bar + 8 * at.stage, at.parity, abort_flag, kWaitLimitNs,
+                           kErrTimeoutProducer, &g_layernorm_error_word);
+}
+// A launch that gave up: the loads in flight land before the block ends.
+__device__ __forceinline__ void ring_drain(const Ring& r, RingAt at, int64_t rows_left) {
+  volatile uint32_t never = 0u;
+  for (int j = 0; j < r.stages && j < rows_left; ++j, at.next(r)) ring_wait(r, at, &never);
+}
+
+// Eight weights or one as fp32.
+template <typename W, int VEC>
+__device__ __forceinline__ void load_weights(const W* w, float (&x)[VEC]) {
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) x[k] = to_f32(w[k]);
 }
 
 struct FwdArgs {
@@ -169,61 +220,62 @@ __global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
   ring.bar = smem_addr(sh.bar);
   ring.stages = BULK ? a.stages : 1;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
-  auto issue = [&](int64_t k) {
-    const uint32_t s = ring_stage(ring, (uint32_t)k);
-    mbar_arrive_expect_tx(ring.bar + 8 * s, ring.row_bytes);
-    bulk_load(ring.base + s * ring.stage_bytes, x + (blockIdx.x + k * gridDim.x) * a.ldx,
-              ring.row_bytes, ring.bar + 8 * s);
+  auto issue = [&](int64_t k, uint32_t stage) {
+    mbar_arrive_expect_tx(ring.bar + 8 * stage, ring.row_bytes);
+    bulk_load(ring.base + stage * ring.stage_bytes, x + (blockIdx.x + k * gridDim.x) * a.ldx,
+              ring.row_bytes, ring.bar + 8 * stage);
   };
   if constexpr (BULK) {
     if (tid == 0) {
       for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
       sh.abort_flag = 0u;
       fence_barrier_init();
-      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k);
+      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
     }
   }
-  float gamma[ITEMS][VEC], beta[ITEMS][VEC];
+  const W* wg = reinterpret_cast<const W*>(a.gamma);
+  const W* wb = reinterpret_cast<const W*>(a.beta);
+  // Weights stay in registers while there is room for them.
+  constexpr bool kKeep = ITEMS * VEC <= 16;
+  float gamma[kKeep ? ITEMS : 1][VEC], beta[kKeep ? ITEMS : 1][VEC];
+  auto weights = [&](int v, float (&g)[VEC], float (&b)[VEC]) {
 #pragma unroll
-  for (int it = 0; it < ITEMS; ++it) {
-    const int v = tid + it * nthr;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      gamma[it][k] = v < nvec ? to_f32(reinterpret_cast<const W*>(a.gamma)[v * VEC + k]) : 0.0f;
-      beta[it][k] = v < nvec && a.beta ? to_f32(reinterpret_cast<const W*>(a.beta)[v * VEC + k])
-                                       : 0.0f;
+    for (int k = 0; k < VEC; ++k) g[k] = b[k] = 0.0f;
+    if (v < nvec) {
+      load_weights<W, VEC>(wg + v * VEC, g);
+      if (wb) load_weights<W, VEC>(wb + v * VEC, b);
     }
+  };
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) weights(tid + it * nthr, gamma[it], beta[it]);
   }
   if constexpr (BULK) __syncthreads();
-  // Elements this warp holds of a row.
-  int nw = 0;
+  // Elements that warp `lane` holds of a row (0 for lanes without a warp).
+  float nw = 0.0f;
+  if (lane < nwarps) {
 #pragma unroll
-  for (int it = 0; it < ITEMS; ++it) {
-    const int first = warp * 32 + it * nthr;
-    nw += min(max(nvec - first, 0), 32) * VEC;
+    for (int it = 0; it < ITEMS; ++it)
+      nw += (float)(min(max(nvec - lane * 32 - it * nthr, 0), 32) * VEC);
   }
-  const float inv_nw = nw > 0 ? 1.0f / (float)nw : 0.0f;
+  const float own = __shfl_sync(0xFFFFFFFFu, nw, warp);
+  const float inv_own = own > 0.0f ? 1.0f / own : 0.0f;
   const float inv_n = 1.0f / (float)a.cols;
   uint32_t top = 0;
   int64_t k = 0;
-  for (; k < mine; ++k) {
+  RingAt at;
+  for (; k < mine; ++k, at.next(ring)) {
     const int64_t row = blockIdx.x + k * gridDim.x;
     Pack<T, VEC> raw[ITEMS];
     bool ok = true;
-    if constexpr (BULK) ok = ring_wait(ring, (uint32_t)k, &sh.abort_flag);
+    if constexpr (BULK) ok = ring_wait(ring, at, &sh.abort_flag);
     if (ok) {
+      const T* src = BULK ? reinterpret_cast<const T*>(smem + at.stage * ring.stage_bytes)
+                          : x + row * a.ldx;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         const int v = tid + it * nthr;
-        raw[it] = zero_pack<T, VEC>();
-        if (v < nvec) {
-          if constexpr (BULK)
-            raw[it] = load_global<T, VEC>(
-                reinterpret_cast<const T*>(smem + ring_stage(ring, (uint32_t)k) * ring.stage_bytes) +
-                v * VEC);
-          else
-            raw[it] = load_global<T, VEC>(x + row * a.ldx + v * VEC);
-        }
+        raw[it] = v < nvec ? load_global<T, VEC>(src + v * VEC) : zero_pack<T, VEC>();
       }
       float s = 0.0f;
 #pragma unroll
@@ -233,7 +285,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += f[j];
       }
-      const float mw = warp_sum(s) * inv_nw;
+      const float mw = warp_sum(s) * inv_own;
       float q = 0.0f;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
@@ -245,32 +297,20 @@ __global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
         }
       }
       q = warp_sum(q);
-      if (lane == 0) {
-        sh.red[k & 1][0][warp] = mw;
-        sh.red[k & 1][1][warp] = q;
-      }
+      if (lane == 0) sh.red[k & 1][warp] = make_float2(mw, q);
     }
-    // Everybody has taken its part of the stage and written its sums; the
-    // sums' other copy was last read before the previous barrier's successor.
+    // Everybody has taken its part of the stage and written its sums.  (The
+    // sums alternate between two copies: those written next were last read
+    // before this barrier.)
     __syncthreads();
     if constexpr (BULK) {
       if (*(volatile uint32_t*)&sh.abort_flag) break;
-      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages);
+      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     }
-    float mean = 0.0f, m2 = 0.0f;
-    for (int w = 0; w < nwarps; ++w) {
-      int n = 0;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) n += min(max(nvec - w * 32 - it * nthr, 0), 32) * VEC;
-      mean += sh.red[k & 1][0][w] * ((float)n * inv_n);
-    }
-    for (int w = 0; w < nwarps; ++w) {
-      int n = 0;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) n += min(max(nvec - w * 32 - it * nthr, 0), 32) * VEC;
-      const float d = sh.red[k & 1][0][w] - mean;
-      m2 += sh.red[k & 1][1][w] + (float)n * d * d;
-    }
+    // Lane w joins warp w's share; every warp does so by itself.
+    const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
+    const float mean = warp_sum(part.x * (nw * inv_n));
+    const float m2 = warp_sum(part.y + nw * (part.x - mean) * (part.x - mean));
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(m2 * inv_n + a.eps));
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
@@ -279,28 +319,25 @@ __global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
       const int v = tid + it * nthr;
+      if (!kKeep) weights(v, gamma[0], beta[0]);
+      const int w = kKeep ? it : 0;
       if (v < nvec) {
         float f[VEC];
         unpack<T, VEC>(raw[it], f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          f[j] = (f[j] - mean) * rstd * gamma[it][j] + beta[it][j];
-          if (a.amax) top = max(top, __float_as_uint(round_to<T>(f[j])) & 0x7FFFFFFFu);
-        }
-        store_global<T, VEC>(y + row * a.ldy + v * VEC, f);
+        for (int j = 0; j < VEC; ++j) f[j] = (f[j] - mean) * rstd * gamma[w][j] + beta[w][j];
+        const Pack<T, VEC> o = pack<T, VEC>(f);
+        if (a.amax) top = pack_top<T, VEC>(top, o);
+        store_global<T, VEC>(y + row * a.ldy + v * VEC, o);
       }
     }
   }
   if constexpr (BULK) {
-    // Given up: the copies in flight land before the block ends.
-    if (k < mine && tid == 0) {
-      volatile uint32_t never = 0u;
-      for (int64_t j = k; j < k + ring.stages && j < mine; ++j) ring_wait(ring, (uint32_t)j, &never);
-    }
+    if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
   }
   if (a.amax) {
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if (lane == 0 && top) atomicMax(a.amax, top);
+    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, top_bits<T>(top));
+    if (lane == 0 && bits) atomicMax(a.amax, bits);
   }
 }
 
@@ -386,9 +423,8 @@ __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
   ring.bar = smem_addr(sh.bar);
   ring.stages = BULK ? a.stages : 1;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
-  auto issue = [&](int64_t k) {
-    const uint32_t s = ring_stage(ring, (uint32_t)k), bar = ring.bar + 8 * s;
-    const uint32_t dst = ring.base + s * ring.stage_bytes;
+  auto issue = [&](int64_t k, uint32_t stage) {
+    const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
     const int64_t row = blockIdx.x + k * gridDim.x;
     mbar_arrive_expect_tx(bar, ring.stage_bytes);
     bulk_load(dst, x + row * a.ldx, ring.row_bytes, bar);
@@ -401,60 +437,67 @@ __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
       for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
       sh.abort_flag = 0u;
       fence_barrier_init();
-      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k);
+      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
     }
   }
-  float gamma[ITEMS][VEC], dg[ITEMS][VEC], db[ITEMS][VEC];
+  const W* wg = reinterpret_cast<const W*>(a.gamma);
+  constexpr bool kKeep = ITEMS * VEC <= 16;      // gamma stays in registers
+  float gamma[kKeep ? ITEMS : 1][VEC], dg[ITEMS][VEC], db[ITEMS][VEC];
+  auto weights = [&](int v, float (&g)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) g[k] = 0.0f;
+    if (v < nvec) load_weights<W, VEC>(wg + v * VEC, g);
+  };
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it) {
-    const int v = tid + it * nthr;
+    if constexpr (kKeep) weights(tid + it * nthr, gamma[it]);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      gamma[it][k] = v < nvec ? to_f32(reinterpret_cast<const W*>(a.gamma)[v * VEC + k]) : 0.0f;
-      dg[it][k] = db[it][k] = 0.0f;
-    }
+    for (int k = 0; k < VEC; ++k) dg[it][k] = db[it][k] = 0.0f;
   }
   if constexpr (BULK) __syncthreads();
   const float inv_n = 1.0f / (float)a.cols;
   int64_t k = 0;
-  for (; k < mine; ++k) {
+  RingAt at;
+  // A row's statistics are fetched a row ahead.
+  float next_mean = mine > 0 ? a.mean[blockIdx.x] : 0.0f;
+  float next_rstd = mine > 0 ? a.rstd[blockIdx.x] : 0.0f;
+  for (; k < mine; ++k, at.next(ring)) {
     const int64_t row = blockIdx.x + k * gridDim.x;
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    const float mean = next_mean, rstd = next_rstd;
+    if (k + 1 < mine) {
+      next_mean = a.mean[row + gridDim.x];
+      next_rstd = a.rstd[row + gridDim.x];
+    }
     Pack<T, VEC> px[ITEMS], pd[ITEMS], pr[RES ? ITEMS : 1];
     bool ok = true;
-    if constexpr (BULK) ok = ring_wait(ring, (uint32_t)k, &sh.abort_flag);
+    if constexpr (BULK) ok = ring_wait(ring, at, &sh.abort_flag);
     if (ok) {
-      const unsigned char* st = smem + ring_stage(ring, (uint32_t)k) * ring.stage_bytes;
+      const unsigned char* st = smem + at.stage * ring.stage_bytes;
+      const T* sx = BULK ? reinterpret_cast<const T*>(st) : x + row * a.ldx;
+      const T* sd = BULK ? reinterpret_cast<const T*>(st + ring.row_bytes) : dy + row * a.lddy;
+      const T* sr = BULK ? reinterpret_cast<const T*>(st + 2 * ring.row_bytes) : res + row * a.ldr;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         const int v = tid + it * nthr;
-        px[it] = pd[it] = zero_pack<T, VEC>();
-        if constexpr (RES) pr[it] = zero_pack<T, VEC>();
-        if (v < nvec) {
-          if constexpr (BULK) {
-            px[it] = load_global<T, VEC>(reinterpret_cast<const T*>(st) + v * VEC);
-            pd[it] = load_global<T, VEC>(reinterpret_cast<const T*>(st + ring.row_bytes) + v * VEC);
-            if constexpr (RES)
-              pr[it] = load_global<T, VEC>(reinterpret_cast<const T*>(st + 2 * ring.row_bytes) +
-                                           v * VEC);
-          } else {
-            px[it] = load_global<T, VEC>(x + row * a.ldx + v * VEC);
-            pd[it] = load_global<T, VEC>(dy + row * a.lddy + v * VEC);
-            if constexpr (RES) pr[it] = load_global<T, VEC>(res + row * a.ldr + v * VEC);
-          }
-        }
+        const bool in = v < nvec;
+        px[it] = in ? load_global<T, VEC>(sx + v * VEC) : zero_pack<T, VEC>();
+        pd[it] = in ? load_global<T, VEC>(sd + v * VEC) : zero_pack<T, VEC>();
+        if constexpr (RES) pr[it] = in ? load_global<T, VEC>(sr + v * VEC) : zero_pack<T, VEC>();
       }
       float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        if (tid + it * nthr < nvec) {
+        const int v = tid + it * nthr;
+        if (!kKeep) weights(v, gamma[0]);
+        const int w = kKeep ? it : 0;
+        if (v < nvec) {
           float fx[VEC], fd[VEC];
           unpack<T, VEC>(px[it], fx);
           unpack<T, VEC>(pd[it], fd);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             const float h = (fx[j] - mean) * rstd;
-            const float u = fd[j] * gamma[it][j];
+            const float u = fd[j] * gamma[w][j];
             s1 += u;
             s2 += u * h;
             dg[it][j] += fd[j] * h;
@@ -464,26 +507,20 @@ __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
       }
       s1 = warp_sum(s1);
       s2 = warp_sum(s2);
-      if (lane == 0) {
-        sh.red[k & 1][0][warp] = s1;
-        sh.red[k & 1][1][warp] = s2;
-      }
+      if (lane == 0) sh.red[k & 1][warp] = make_float2(s1, s2);
     }
     __syncthreads();
     if constexpr (BULK) {
       if (*(volatile uint32_t*)&sh.abort_flag) break;
-      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages);
+      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     }
-    float c1 = 0.0f, c2 = 0.0f;
-    for (int w = 0; w < nwarps; ++w) {
-      c1 += sh.red[k & 1][0][w];
-      c2 += sh.red[k & 1][1][w];
-    }
-    c1 *= inv_n;
-    c2 *= inv_n;
+    const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
+    const float c1 = warp_sum(part.x) * inv_n, c2 = warp_sum(part.y) * inv_n;
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
       const int v = tid + it * nthr;
+      if (!kKeep) weights(v, gamma[0]);
+      const int w = kKeep ? it : 0;
       if (v < nvec) {
         float fx[VEC], fd[VEC], fr[VEC];
         unpack<T, VEC>(px[it], fx);
@@ -492,18 +529,15 @@ __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float h = (fx[j] - mean) * rstd;
-          fx[j] = rstd * (fd[j] * gamma[it][j] - c1 - h * c2);
+          fx[j] = rstd * (fd[j] * gamma[w][j] - c1 - h * c2);
           if constexpr (RES) fx[j] += fr[j];
         }
-        store_global<T, VEC>(dx + row * a.lddx + v * VEC, fx);
+        store_global<T, VEC>(dx + row * a.lddx + v * VEC, pack<T, VEC>(fx));
       }
     }
   }
   if constexpr (BULK) {
-    if (k < mine && tid == 0) {
-      volatile uint32_t never = 0u;
-      for (int64_t j = k; j < k + ring.stages && j < mine; ++j) ring_wait(ring, (uint32_t)j, &never);
-    }
+    if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
   }
   float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
