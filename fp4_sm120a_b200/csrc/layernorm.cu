@@ -24,6 +24,7 @@
 // its sum of squares about that mean, combined over warps by
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
 // so a large common offset or an outlier costs no digits.
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,11 +41,10 @@ namespace {
 __device__ uint32_t g_layernorm_error_word;
 
 constexpr int kMaxThreads = 512;
-constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxStages = 8;
-constexpr uint32_t kRingBytes = 96 * 1024;     // per block: two blocks fit one SM
+constexpr size_t kRingBytes = 200 * 1024;      // of an SM, over its blocks
+constexpr size_t kRingMost = 226 * 1024;       // dynamic shared memory a block may ask for
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
-constexpr int kMaxPartials = 296;              // partial rows of dgamma and dbeta
 constexpr int kWideThreads = 256;
 
 __device__ __forceinline__ float warp_sum(float x) {
@@ -62,105 +62,216 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack_one(float x) {
-  if constexpr (sizeof(T) == 4) return __float_as_uint(x);
-  else return pack2<T>(x, 0.0f);
+// Pairs of fp32 in one instruction (add / mul / fma.rn.f32x2).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum2(uint64_t p) {
+  float a, b;
+  split(p, a, b);
+  return a + b;
 }
 
-// VEC consecutive elements: 16 bytes, or one element.
-template <typename T, int VEC>
-struct Pack {
-  static constexpr int kWords = VEC == 1 ? 1 : 4;
-  uint32_t w[kWords];
+// A row over the threads.  kAligned: thread t holds the 16-byte vectors t,
+// t + threads, ...; otherwise the elements t, t + threads, ...
+template <typename T, bool ALIGNED>
+struct Layout {
+  static constexpr int kVec = ALIGNED ? 16 / (int)sizeof(T) : 1;
 };
-template <typename T, int VEC>
-__device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&x)[VEC]) {
-  if constexpr (VEC == 1) {
-    if constexpr (sizeof(T) == 4) {
-      x[0] = __uint_as_float(p.w[0]);
-    } else {
-      float hi;
-      unpack2<T>(p.w[0], x[0], hi);
-    }
-  } else if constexpr (sizeof(T) == 4) {
+
+// 16 bytes as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& q, float* x) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(p.w[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) unpack2<T>(p.w[k], x[2 * k], x[2 * k + 1]);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) x[k] = __uint_as_float(w[k]);
+    else unpack2<T>(w[k], x[2 * k], x[2 * k + 1]);
   }
 }
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_global(const T* p) {
-  Pack<T, VEC> r;
-  if constexpr (VEC == 1) {
-    if constexpr (sizeof(T) == 4) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
-    else r.w[0] = *reinterpret_cast<const uint16_t*>(p);
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-  }
-  return r;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> zero_pack() {
-  Pack<T, VEC> r;
-#pragma unroll
-  for (int k = 0; k < Pack<T, VEC>::kWords; ++k) r.w[k] = 0u;
-  return r;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> pack(const float (&x)[VEC]) {
-  Pack<T, VEC> r;
-  if constexpr (VEC == 1) {
-    r.w[0] = pack_one<T>(x[0]);
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r.w[k] = __float_as_uint(x[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r.w[k] = pack2<T>(x[2 * k], x[2 * k + 1]);
-  }
-  return r;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_global(T* p, const Pack<T, VEC>& r) {
-  if constexpr (VEC == 1) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = r.w[0];
-    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)r.w[0];
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
-  }
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* x) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                      __float_as_uint(x[3]));
+  else
+    return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                      pack2<T>(x[6], x[7]));
 }
 // Unsigned maximum of the magnitudes' bit patterns, per 16-bit half or per
 // word (NaN patterns are above infinity's), and its value as fp32 bits.
-template <typename T, int VEC>
-__device__ __forceinline__ uint32_t pack_top(uint32_t m, const Pack<T, VEC>& r) {
-#pragma unroll
-  for (int k = 0; k < Pack<T, VEC>::kWords; ++k)
-    m = sizeof(T) == 4 ? max(m, r.w[k] & 0x7FFFFFFFu) : __vmaxu2(m, r.w[k] & 0x7FFF7FFFu);
-  return m;
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, uint32_t w) {
+  return sizeof(T) == 4 ? max(m, w & 0x7FFFFFFFu) : __vmaxu2(m, w & 0x7FFF7FFFu);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
-  if constexpr (sizeof(T) == 4) return m;
-  else {
+  if constexpr (sizeof(T) == 4) {
+    return m;
+  } else {
     float lo, hi;
     unpack2<T>(m, lo, hi);
     return max(__float_as_uint(lo), __float_as_uint(hi));
   }
 }
 
-// The ring of bulk copies: ARRAYS rows a stage (x, dy, residual).
+// The part of a row that bulk copies can take: whole 16-byte units.  The few
+// elements before and behind them (unaligned rows) are read directly, so
+// nothing outside the row is touched.
+struct Span {
+  uint32_t lead;     // bytes from the 16-byte boundary below the row to the row
+  uint32_t skip;     // ... to the first whole unit (0 or 16)
+  uint32_t bytes;    // of whole units
+};
+template <bool ALIGNED>
+__device__ __forceinline__ Span span_of(const void* row, uint32_t row_bytes) {
+  if constexpr (ALIGNED) return {0u, 0u, row_bytes};
+  const uint32_t lead = (uint32_t)((uintptr_t)row & 15u), skip = lead ? 16u : 0u;
+  const uint32_t end = (lead + row_bytes) & ~15u;
+  return {lead, skip, end > skip ? end - skip : 0u};
+}
+// Starts a row's copy; returns the bytes to expect.
+template <bool ALIGNED>
+__device__ __forceinline__ void span_load(const Span& s, uint32_t slot, const void* row,
+                                          uint32_t bar) {
+  if (ALIGNED || s.bytes)
+    bulk_load(slot + s.skip, reinterpret_cast<const unsigned char*>(row) - s.lead + s.skip, s.bytes,
+              bar);
+}
+// Which of a thread's items lie within the row.
+template <typename T, bool ALIGNED, int ITEMS>
+struct Mine {
+  uint32_t in;
+  __device__ __forceinline__ explicit Mine(int cols) : in(0) {
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it)
+      if ((int)threadIdx.x + it * (int)blockDim.x < cols / Layout<T, ALIGNED>::kVec) in |= 1u << it;
+  }
+  __device__ __forceinline__ bool has(int it) const { return (in >> it) & 1u; }
+};
+// The elements of an unaligned row outside its whole 16-byte units lie among
+// its first and last eight.  Lanes 0-15 of the first warp look after one each:
+// they load it a row ahead of the row's copy and store it into the slot when
+// the copy starts, two barriers before the slot is read.
+template <typename T, bool ALIGNED>
+struct Edge {
+  int e;       // this lane's element, -1: none
+  T value;
+  __device__ __forceinline__ explicit Edge(int cols) : e(-1), value() {
+    if (!ALIGNED && threadIdx.x < 16) {
+      const int lane = (int)threadIdx.x;
+      e = cols >= 16 && lane >= 8 ? cols - 16 + lane : lane;
+      if (e >= cols) e = -1;
+    }
+  }
+  __device__ __forceinline__ void load(const T* row) {
+    if (!ALIGNED && e >= 0) value = row[e];
+  }
+  __device__ __forceinline__ void store(unsigned char* slot, const Span& s) const {
+    if (!ALIGNED && e >= 0) {
+      const uint32_t off = s.lead + (uint32_t)e * (uint32_t)sizeof(T);
+      if (off - s.skip >= s.bytes) *reinterpret_cast<T*>(slot + off) = value;
+    }
+  }
+};
+// This thread's elements of a row that has arrived in `slot`.
+template <typename T, bool ALIGNED, int ITEMS>
+__device__ __forceinline__ void fetch(const Mine<T, ALIGNED, ITEMS>& my, const unsigned char* slot,
+                                      const T* row, uint32_t row_bytes, float* f) {
+  constexpr int VEC = Layout<T, ALIGNED>::kVec;
+  const int tid = threadIdx.x, nthr = blockDim.x;
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const uint4 q = my.has(it) ? reinterpret_cast<const uint4*>(slot)[tid + it * nthr]
+                                 : make_uint4(0, 0, 0, 0);
+      unpack16<T>(q, f + it * VEC);
+    }
+  } else {
+    // Loads without branches: what lies behind the row's end reads its first element.
+    const T* in = reinterpret_cast<const T*>(slot + span_of<false>(row, row_bytes).lead);
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const T v = in[my.has(it) ? tid + it * nthr : 0];
+      f[it] = my.has(it) ? to_f32(v) : 0.0f;
+    }
+  }
+}
+// Stores this thread's elements; with TOP returns the magnitudes' maximum
+// joined to `top`.
+template <bool TOP, typename T, bool ALIGNED, int ITEMS>
+__device__ __forceinline__ uint32_t put(const Mine<T, ALIGNED, ITEMS>& my, T* row, const float* f,
+                                        uint32_t top) {
+  constexpr int VEC = Layout<T, ALIGNED>::kVec;
+  const int nthr = blockDim.x;
+  if constexpr (ALIGNED) {
+    uint4* out = reinterpret_cast<uint4*>(row) + threadIdx.x;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const uint4 q = pack16<T>(f + it * VEC);
+      if (my.has(it)) out[it * nthr] = q;
+      if (TOP && my.has(it)) {
+        top = max_bits<T>(max_bits<T>(top, q.x), q.y);
+        top = max_bits<T>(max_bits<T>(top, q.z), q.w);
+      }
+    }
+  } else {
+    T* out = row + threadIdx.x;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const T o = from_f32<T>(f[it]);
+      if (my.has(it)) out[it * nthr] = o;
+      if (TOP && my.has(it))
+        top = max_bits<T>(top, sizeof(T) == 4
+                                   ? __float_as_uint(to_f32(o))
+                                   : (uint32_t)*reinterpret_cast<const uint16_t*>(&o));
+    }
+  }
+  return top;
+}
+// This thread's weights, zero behind the row's end.
+template <typename T, typename W, bool ALIGNED, int ITEMS>
+__device__ __forceinline__ void fetch_weights(const W* w, int cols, float* f) {
+  constexpr int VEC = Layout<T, ALIGNED>::kVec;
+#pragma unroll
+  for (int it = 0; it < ITEMS; ++it) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int c = ((int)threadIdx.x + it * (int)blockDim.x) * VEC + k;
+      f[it * VEC + k] = w != nullptr && c < cols ? to_f32(w[c]) : 0.0f;
+    }
+  }
+}
+
+// The ring of rows in flight: ARRAYS slots a stage (x, dy, residual).
 struct Ring {
-  uint32_t base, bar, stage_bytes, row_bytes;
+  uint32_t base, bar, stage_bytes, slot_bytes;
   int stages;
 };
 
 struct Shared {
   uint64_t bar[kMaxStages];
-  float2 red[2][kMaxWarps];
+  float2 red[2][32];
   uint32_t abort_flag;
   uint32_t pad[3];
 };
@@ -184,13 +295,6 @@ __device__ __forceinline__ void ring_drain(const Ring& r, RingAt at, int64_t row
   for (int j = 0; j < r.stages && j < rows_left; ++j, at.next(r)) ring_wait(r, at, &never);
 }
 
-// Eight weights or one as fp32.
-template <typename W, int VEC>
-__device__ __forceinline__ void load_weights(const W* w, float (&x)[VEC]) {
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) x[k] = to_f32(w[k]);
-}
-
 struct FwdArgs {
   const void* x;
   const void* gamma;
@@ -201,56 +305,63 @@ struct FwdArgs {
   uint32_t* amax;
   int64_t rows, ldx, ldy;
   int cols, stages;
+  uint32_t slot_bytes;
   float eps;
 };
 
-// One row per block at a time; thread t holds the vectors t, t + blockDim, ...
-// BULK: the row arrives through the ring; otherwise by element-wise loads.
-template <typename T, typename W, int VEC, int ITEMS, bool BULK>
-__global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
+// One row per block at a time; two blocks or more share an SM and hide each
+// other's reductions.
+template <typename T, typename W, bool ALIGNED, int ITEMS>
+__global__ void __launch_bounds__(kMaxThreads, ALIGNED && ITEMS * Layout<T, ALIGNED>::kVec <= 16 ? 2 : 1)
+    k_fwd_rows(const FwdArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared sh;
+  constexpr int VEC = Layout<T, ALIGNED>::kVec, E = ITEMS * VEC;
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int nwarps = nthr >> 5, nvec = a.cols / VEC;
+  const Mine<T, ALIGNED, ITEMS> my(a.cols);
+  const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
   const T* x = reinterpret_cast<const T*>(a.x);
   T* y = reinterpret_cast<T*>(a.y);
   Ring ring;
-  ring.row_bytes = ring.stage_bytes = (uint32_t)a.cols * sizeof(T);
+  ring.slot_bytes = ring.stage_bytes = a.slot_bytes;
   ring.base = smem_addr(smem);
   ring.bar = smem_addr(sh.bar);
-  ring.stages = BULK ? a.stages : 1;
+  ring.stages = a.stages;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  auto row_at = [&](int64_t k) { return (int64_t)blockIdx.x + k * gridDim.x; };
+  Edge<T, ALIGNED> edge(a.cols);
+  // By the first warp; row k's edge elements have been loaded.
   auto issue = [&](int64_t k, uint32_t stage) {
-    mbar_arrive_expect_tx(ring.bar + 8 * stage, ring.row_bytes);
-    bulk_load(ring.base + stage * ring.stage_bytes, x + (blockIdx.x + k * gridDim.x) * a.ldx,
-              ring.row_bytes, ring.bar + 8 * stage);
-  };
-  if constexpr (BULK) {
+    const T* row = x + row_at(k) * a.ldx;
+    const Span s = span_of<ALIGNED>(row, row_bytes);
+    edge.store(smem + stage * ring.stage_bytes, s);
     if (tid == 0) {
-      for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
-      sh.abort_flag = 0u;
-      fence_barrier_init();
-      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
+      mbar_arrive_expect_tx(ring.bar + 8 * stage, s.bytes);
+      span_load<ALIGNED>(s, ring.base + stage * ring.stage_bytes, row, ring.bar + 8 * stage);
     }
+    if (k + 1 < mine) edge.load(x + row_at(k + 1) * a.ldx);
+  };
+  if (tid == 0) {
+    for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
+    sh.abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    edge.load(x + row_at(0) * a.ldx);
+    for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   const W* wb = reinterpret_cast<const W*>(a.beta);
   // Weights stay in registers while there is room for them.
-  constexpr bool kKeep = ITEMS * VEC <= 16;
-  float gamma[kKeep ? ITEMS : 1][VEC], beta[kKeep ? ITEMS : 1][VEC];
-  auto weights = [&](int v, float (&g)[VEC], float (&b)[VEC]) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) g[k] = b[k] = 0.0f;
-    if (v < nvec) {
-      load_weights<W, VEC>(wg + v * VEC, g);
-      if (wb) load_weights<W, VEC>(wb + v * VEC, b);
-    }
-  };
+  constexpr bool kKeep = E <= 16;
+  float gamma[E], beta[E];
   if constexpr (kKeep) {
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) weights(tid + it * nthr, gamma[it], beta[it]);
+    fetch_weights<T, W, ALIGNED, ITEMS>(wg, a.cols, gamma);
+    fetch_weights<T, W, ALIGNED, ITEMS>(wb, a.cols, beta);
   }
-  if constexpr (BULK) __syncthreads();
+  __syncthreads();
   // Elements that warp `lane` holds of a row (0 for lanes without a warp).
   float nw = 0.0f;
   if (lane < nwarps) {
@@ -265,76 +376,60 @@ __global__ void __launch_bounds__(kMaxThreads) k_fwd_rows(const FwdArgs a) {
   int64_t k = 0;
   RingAt at;
   for (; k < mine; ++k, at.next(ring)) {
-    const int64_t row = blockIdx.x + k * gridDim.x;
-    Pack<T, VEC> raw[ITEMS];
-    bool ok = true;
-    if constexpr (BULK) ok = ring_wait(ring, at, &sh.abort_flag);
-    if (ok) {
-      const T* src = BULK ? reinterpret_cast<const T*>(smem + at.stage * ring.stage_bytes)
-                          : x + row * a.ldx;
+    const int64_t row = row_at(k);
+    float f[E];
+    if (ring_wait(ring, at, &sh.abort_flag)) {
+      fetch<T, ALIGNED, ITEMS>(my, smem + at.stage * ring.stage_bytes, x + row * a.ldx, row_bytes,
+                               f);
+      uint64_t s = pair(0.0f, 0.0f);
 #pragma unroll
-      for (int it = 0; it < ITEMS; ++it) {
-        const int v = tid + it * nthr;
-        raw[it] = v < nvec ? load_global<T, VEC>(src + v * VEC) : zero_pack<T, VEC>();
+      for (int e = 0; e < E; e += 2) s = add2(s, pair(f[e], f[e + 1]));
+      const float mw = warp_sum(sum2(s)) * inv_own;
+      const uint64_t minus = pair(-mw, -mw);
+      s = pair(0.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        // What lies behind the row's end counts as the mean.
+        const float u = my.has(e / VEC) ? f[e] : mw, v = my.has((e + 1) / VEC) ? f[e + 1] : mw;
+        const uint64_t d = add2(pair(u, v), minus);
+        s = fma2(d, d, s);
       }
-      float s = 0.0f;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) {
-        float f[VEC];
-        unpack<T, VEC>(raw[it], f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += f[j];
-      }
-      const float mw = warp_sum(s) * inv_own;
-      float q = 0.0f;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) {
-        if (tid + it * nthr < nvec) {
-          float f[VEC];
-          unpack<T, VEC>(raw[it], f);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) q += (f[j] - mw) * (f[j] - mw);
-        }
-      }
-      q = warp_sum(q);
+      const float q = warp_sum(sum2(s));
       if (lane == 0) sh.red[k & 1][warp] = make_float2(mw, q);
     }
     // Everybody has taken its part of the stage and written its sums.  (The
     // sums alternate between two copies: those written next were last read
     // before this barrier.)
     __syncthreads();
-    if constexpr (BULK) {
-      if (*(volatile uint32_t*)&sh.abort_flag) break;
-      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
-    }
+    if (*(volatile uint32_t*)&sh.abort_flag) break;
+    if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     // Lane w joins warp w's share; every warp does so by itself.
     const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
     const float mean = warp_sum(part.x * (nw * inv_n));
-    const float m2 = warp_sum(part.y + nw * (part.x - mean) * (part.x - mean));
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(m2 * inv_n + a.eps));
+    const float d = part.x - mean;
+    const float rstd = rsqrtf(warp_sum(part.y + nw * d * d) * inv_n + a.eps);
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
     }
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-      const int v = tid + it * nthr;
-      if (!kKeep) weights(v, gamma[0], beta[0]);
-      const int w = kKeep ? it : 0;
-      if (v < nvec) {
-        float f[VEC];
-        unpack<T, VEC>(raw[it], f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = (f[j] - mean) * rstd * gamma[w][j] + beta[w][j];
-        const Pack<T, VEC> o = pack<T, VEC>(f);
-        if (a.amax) top = pack_top<T, VEC>(top, o);
-        store_global<T, VEC>(y + row * a.ldy + v * VEC, o);
-      }
+    if constexpr (!kKeep) {
+      fetch_weights<T, W, ALIGNED, ITEMS>(wg, a.cols, gamma);
+      fetch_weights<T, W, ALIGNED, ITEMS>(wb, a.cols, beta);
     }
+    // (x - mean) first: a constant row's difference is zero exactly, whatever
+    // rstd makes of a rounding error.
+    const uint64_t scale = pair(rstd, rstd), minus = pair(-mean, -mean);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const uint64_t h = mul2(add2(pair(f[e], f[e + 1]), minus), scale);
+      split(fma2(h, pair(gamma[e], gamma[e + 1]), pair(beta[e], beta[e + 1])), f[e], f[e + 1]);
+    }
+    if (a.amax)
+      top = put<true, T, ALIGNED, ITEMS>(my, y + row * a.ldy, f, top);
+    else
+      put<false, T, ALIGNED, ITEMS>(my, y + row * a.ldy, f, 0u);
   }
-  if constexpr (BULK) {
-    if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
-  }
+  if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
   if (a.amax) {
     const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, top_bits<T>(top));
     if (lane == 0 && bits) atomicMax(a.amax, bits);
@@ -403,58 +498,74 @@ struct BwdArgs {
   float* partial;       // [partials][2][cols]: sums of dy h, sums of dy
   int64_t rows, lddy, ldx, ldr, lddx;
   int cols, stages, partials;
+  uint32_t slot_bytes;
 };
 
-template <typename T, typename W, int VEC, int ITEMS, bool BULK, bool RES>
+template <typename T, typename W, bool ALIGNED, int ITEMS, bool RES>
 __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
+  // k_bwd_reduce may be scheduled; it waits for this kernel to complete.
+  asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared sh;
+  constexpr int VEC = Layout<T, ALIGNED>::kVec, E = ITEMS * VEC;
   constexpr int kArrays = RES ? 3 : 2;
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int nwarps = nthr >> 5, nvec = a.cols / VEC;
+  const int nwarps = nthr >> 5;
+  const Mine<T, ALIGNED, ITEMS> my(a.cols);
+  const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* dy = reinterpret_cast<const T*>(a.dy);
   const T* res = reinterpret_cast<const T*>(a.res);
   T* dx = reinterpret_cast<T*>(a.dx);
   Ring ring;
-  ring.row_bytes = (uint32_t)a.cols * sizeof(T);
-  ring.stage_bytes = kArrays * ring.row_bytes;
+  ring.slot_bytes = a.slot_bytes;
+  ring.stage_bytes = kArrays * a.slot_bytes;
   ring.base = smem_addr(smem);
   ring.bar = smem_addr(sh.bar);
-  ring.stages = BULK ? a.stages : 1;
+  ring.stages = a.stages;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  Edge<T, ALIGNED> ex(a.cols), ed(a.cols), er(a.cols);
+  auto edges = [&](int64_t row) {
+    ex.load(x + row * a.ldx);
+    ed.load(dy + row * a.lddy);
+    if constexpr (RES) er.load(res + row * a.ldr);
+  };
+  // By the first warp; row k's edge elements have been loaded.
   auto issue = [&](int64_t k, uint32_t stage) {
     const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
     const int64_t row = blockIdx.x + k * gridDim.x;
-    mbar_arrive_expect_tx(bar, ring.stage_bytes);
-    bulk_load(dst, x + row * a.ldx, ring.row_bytes, bar);
-    bulk_load(dst + ring.row_bytes, dy + row * a.lddy, ring.row_bytes, bar);
-    if constexpr (RES)
-      bulk_load(dst + 2 * ring.row_bytes, res + row * a.ldr, ring.row_bytes, bar);
-  };
-  if constexpr (BULK) {
+    const Span s0 = span_of<ALIGNED>(x + row * a.ldx, row_bytes);
+    const Span s1 = span_of<ALIGNED>(dy + row * a.lddy, row_bytes);
+    const Span s2 = RES ? span_of<ALIGNED>(res + row * a.ldr, row_bytes) : Span{0u, 0u, 0u};
+    unsigned char* slot = smem + stage * ring.stage_bytes;
+    ex.store(slot, s0);
+    ed.store(slot + ring.slot_bytes, s1);
+    if constexpr (RES) er.store(slot + 2 * ring.slot_bytes, s2);
     if (tid == 0) {
-      for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
-      sh.abort_flag = 0u;
-      fence_barrier_init();
-      for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
+      mbar_arrive_expect_tx(bar, s0.bytes + s1.bytes + s2.bytes);
+      span_load<ALIGNED>(s0, dst, x + row * a.ldx, bar);
+      span_load<ALIGNED>(s1, dst + ring.slot_bytes, dy + row * a.lddy, bar);
+      if constexpr (RES) span_load<ALIGNED>(s2, dst + 2 * ring.slot_bytes, res + row * a.ldr, bar);
     }
+    if (k + 1 < mine) edges(row + gridDim.x);
+  };
+  if (tid == 0) {
+    for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
+    sh.abort_flag = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    edges(blockIdx.x);
+    for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
-  constexpr bool kKeep = ITEMS * VEC <= 16;      // gamma stays in registers
-  float gamma[kKeep ? ITEMS : 1][VEC], dg[ITEMS][VEC], db[ITEMS][VEC];
-  auto weights = [&](int v, float (&g)[VEC]) {
+  constexpr bool kKeep = E <= 16;      // gamma stays in registers
+  float gamma[E], dg[E], db[E];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) g[k] = 0.0f;
-    if (v < nvec) load_weights<W, VEC>(wg + v * VEC, g);
-  };
-#pragma unroll
-  for (int it = 0; it < ITEMS; ++it) {
-    if constexpr (kKeep) weights(tid + it * nthr, gamma[it]);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) dg[it][k] = db[it][k] = 0.0f;
-  }
-  if constexpr (BULK) __syncthreads();
+  for (int e = 0; e < E; ++e) dg[e] = db[e] = 0.0f;
+  if constexpr (kKeep) fetch_weights<T, W, ALIGNED, ITEMS>(wg, a.cols, gamma);
+  __syncthreads();
   const float inv_n = 1.0f / (float)a.cols;
   int64_t k = 0;
   RingAt at;
@@ -468,86 +579,58 @@ __global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
       next_mean = a.mean[row + gridDim.x];
       next_rstd = a.rstd[row + gridDim.x];
     }
-    Pack<T, VEC> px[ITEMS], pd[ITEMS], pr[RES ? ITEMS : 1];
-    bool ok = true;
-    if constexpr (BULK) ok = ring_wait(ring, at, &sh.abort_flag);
+    float h[E], u[E], fr[RES ? E : 2];
+    const bool ok = ring_wait(ring, at, &sh.abort_flag);
     if (ok) {
       const unsigned char* st = smem + at.stage * ring.stage_bytes;
-      const T* sx = BULK ? reinterpret_cast<const T*>(st) : x + row * a.ldx;
-      const T* sd = BULK ? reinterpret_cast<const T*>(st + ring.row_bytes) : dy + row * a.lddy;
-      const T* sr = BULK ? reinterpret_cast<const T*>(st + 2 * ring.row_bytes) : res + row * a.ldr;
+      fetch<T, ALIGNED, ITEMS>(my, st, x + row * a.ldx, row_bytes, h);
+      fetch<T, ALIGNED, ITEMS>(my, st + ring.slot_bytes, dy + row * a.lddy, row_bytes, u);
+      if constexpr (RES)
+        fetch<T, ALIGNED, ITEMS>(my, st + 2 * ring.slot_bytes, res + row * a.ldr, row_bytes, fr);
+      if constexpr (!kKeep) fetch_weights<T, W, ALIGNED, ITEMS>(wg, a.cols, gamma);
+      const uint64_t scale = pair(rstd, rstd), minus = pair(-mean, -mean);
+      uint64_t t1 = pair(0.0f, 0.0f), t2 = pair(0.0f, 0.0f);
+      // Behind the row's end dy and gamma are zero: nothing is added there.
 #pragma unroll
-      for (int it = 0; it < ITEMS; ++it) {
-        const int v = tid + it * nthr;
-        const bool in = v < nvec;
-        px[it] = in ? load_global<T, VEC>(sx + v * VEC) : zero_pack<T, VEC>();
-        pd[it] = in ? load_global<T, VEC>(sd + v * VEC) : zero_pack<T, VEC>();
-        if constexpr (RES) pr[it] = in ? load_global<T, VEC>(sr + v * VEC) : zero_pack<T, VEC>();
+      for (int e = 0; e < E; e += 2) {
+        const uint64_t hh = mul2(add2(pair(h[e], h[e + 1]), minus), scale);
+        const uint64_t d = pair(u[e], u[e + 1]);
+        const uint64_t uu = mul2(d, pair(gamma[e], gamma[e + 1]));
+        t1 = add2(t1, uu);
+        t2 = fma2(uu, hh, t2);
+        split(fma2(d, hh, pair(dg[e], dg[e + 1])), dg[e], dg[e + 1]);
+        split(add2(d, pair(db[e], db[e + 1])), db[e], db[e + 1]);
+        split(hh, h[e], h[e + 1]);
+        split(uu, u[e], u[e + 1]);
       }
-      float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) {
-        const int v = tid + it * nthr;
-        if (!kKeep) weights(v, gamma[0]);
-        const int w = kKeep ? it : 0;
-        if (v < nvec) {
-          float fx[VEC], fd[VEC];
-          unpack<T, VEC>(px[it], fx);
-          unpack<T, VEC>(pd[it], fd);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float h = (fx[j] - mean) * rstd;
-            const float u = fd[j] * gamma[w][j];
-            s1 += u;
-            s2 += u * h;
-            dg[it][j] += fd[j] * h;
-            db[it][j] += fd[j];
-          }
-        }
-      }
-      s1 = warp_sum(s1);
-      s2 = warp_sum(s2);
+      const float s1 = warp_sum(sum2(t1)), s2 = warp_sum(sum2(t2));
       if (lane == 0) sh.red[k & 1][warp] = make_float2(s1, s2);
     }
     __syncthreads();
-    if constexpr (BULK) {
-      if (*(volatile uint32_t*)&sh.abort_flag) break;
-      if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
-    }
+    if (*(volatile uint32_t*)&sh.abort_flag) break;
+    if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
-    const float c1 = warp_sum(part.x) * inv_n, c2 = warp_sum(part.y) * inv_n;
+    const float c1 = warp_sum(part.x) * inv_n * rstd, c2 = warp_sum(part.y) * inv_n * rstd;
+    const uint64_t scale = pair(rstd, rstd), n1 = pair(-c1, -c1), n2 = pair(-c2, -c2);
 #pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-      const int v = tid + it * nthr;
-      if (!kKeep) weights(v, gamma[0]);
-      const int w = kKeep ? it : 0;
-      if (v < nvec) {
-        float fx[VEC], fd[VEC], fr[VEC];
-        unpack<T, VEC>(px[it], fx);
-        unpack<T, VEC>(pd[it], fd);
-        if constexpr (RES) unpack<T, VEC>(pr[it], fr);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float h = (fx[j] - mean) * rstd;
-          fx[j] = rstd * (fd[j] * gamma[w][j] - c1 - h * c2);
-          if constexpr (RES) fx[j] += fr[j];
-        }
-        store_global<T, VEC>(dx + row * a.lddx + v * VEC, pack<T, VEC>(fx));
-      }
+    for (int e = 0; e < E; e += 2) {
+      uint64_t o = fma2(pair(u[e], u[e + 1]), scale, n1);
+      o = fma2(pair(h[e], h[e + 1]), n2, o);
+      if constexpr (RES) o = add2(o, pair(fr[e], fr[e + 1]));
+      split(o, h[e], h[e + 1]);
     }
+    put<false, T, ALIGNED, ITEMS>(my, dx + row * a.lddx, h, 0u);
   }
-  if constexpr (BULK) {
-    if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
-  }
+  if (k < mine && tid == 0) ring_drain(ring, at, mine - k);
   float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it) {
-    const int v = tid + it * nthr;
-    if (v < nvec) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        out[v * VEC + j] = dg[it][j];
-        out[a.cols + v * VEC + j] = db[it][j];
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (tid + it * nthr) * VEC + j;
+      if (c < a.cols) {
+        out[c] = dg[it * VEC + j];
+        out[a.cols + c] = db[it * VEC + j];
       }
     }
   }
@@ -616,23 +699,33 @@ __global__ void __launch_bounds__(kWideThreads) k_bwd_wide_w(const BwdArgs a) {
 }
 
 // dgamma, dbeta: the partial rows summed in a fixed order.  32 columns of one
-// of the two outputs a block; 8 warps take every eighth partial row.
+// of the two outputs a block; warp w takes the partial rows w, w + 16, ...
+constexpr int kReduceWarps = 16;
 template <typename W>
-__global__ void __launch_bounds__(256) k_bwd_reduce(const float* __restrict__ partial,
-                                                    int partials, int cols, W* dgamma, W* dbeta) {
-  __shared__ float s[8][32];
+__global__ void __launch_bounds__(32 * kReduceWarps) k_bwd_reduce(const float* partial,
+                                                                  int partials, int cols,
+                                                                  W* dgamma, W* dbeta) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float s[kReduceWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane, which = blockIdx.y;
   float v = 0.0f;
   if (c < cols) {
     const float* p = partial + (size_t)which * cols + c;
-    for (int r = warp; r < partials; r += 8) v += p[(size_t)r * 2 * cols];
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int r = warp;
+    for (; r + 3 * kReduceWarps < partials; r += 4 * kReduceWarps) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] += p[(size_t)(r + j * kReduceWarps) * 2 * cols];
+    }
+    for (; r < partials; r += kReduceWarps) t[0] += p[(size_t)r * 2 * cols];
+    v = (t[0] + t[1]) + (t[2] + t[3]);
   }
   s[warp][lane] = v;
   __syncthreads();
   if (warp == 0 && c < cols) {
 #pragma unroll
-    for (int w = 1; w < 8; ++w) v += s[w][lane];
+    for (int w = 1; w < kReduceWarps; ++w) v += s[w][lane];
     W* out = which == 0 ? dgamma : dbeta;
     if (out) out[c] = from_f32<W>(v);
   }
@@ -642,127 +735,138 @@ __global__ void __launch_bounds__(256) k_bwd_reduce(const float* __restrict__ pa
 // Host side
 // ---------------------------------------------------------------------------
 
-// How a row is laid over threads: `items` vectors a thread, few enough threads
-// that none is idle for most of the row.
-struct Shape {
-  int items, threads;
-};
-// items are 1, 2 or 4; false: the row is wider than the registers hold.
-bool row_shape(int64_t nvec, int want, Shape* s) {
-  for (int items : {want, 4}) {
-    while (items > 1 && nvec <= (int64_t)items / 2 * 32) items /= 2;
-    const int64_t threads = ((nvec + items - 1) / items + 31) / 32 * 32;
-    if (threads <= kMaxThreads) {
-      *s = {items, (int)threads};
-      return true;
-    }
-  }
-  return false;
-}
+// Threads for a row of `n` vectors (or elements) at `items` a thread.
+int row_threads(int64_t n, int items) { return (int)(((n + items - 1) / items + 31) / 32 * 32); }
 
-template <typename K>
-int set_smem(K kernel, size_t bytes) {
-  // 48 KB is the default limit of static and dynamic memory together.
-  if (bytes + sizeof(Shared) > 48 * 1024)
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)bytes))
+// Blocks of `kernel` that an SM's registers and threads take, before shared
+// memory (kept: the query costs more than a launch).  Also allows the kernel
+// all of an SM's shared memory, once a device.
+template <auto KERNEL>
+int blocks_of(int threads, int* blocks) {
+  static std::atomic<int> kept[33];
+  static std::atomic<uint64_t> allowed;
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return cuda_status(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev > 63 || !(allowed.load(std::memory_order_acquire) & bit)) {
+    if (cudaError_t e = cudaFuncSetAttribute(
+            KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingMost))
       return cuda_status(e);
-  return NVFP4_OK;
-}
-
-int ring_stages(size_t stage_bytes) {
-  const size_t s = kRingBytes / stage_bytes;
-  return (int)(s < 2 ? 2 : s > kMaxStages ? kMaxStages : s);
-}
-
-// Blocks of a persistent grid: as many as fit at once, at most one a row.
-template <typename K>
-int grid_of(K kernel, int threads, size_t smem, int64_t rows, int sms, int64_t most,
-            unsigned* grid) {
-  int per_sm = 0;
-  if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem))
-    return cuda_status(e);
-  int64_t g = (int64_t)(per_sm < 1 ? 1 : per_sm) * sms;
-  if (g > most) g = most;
-  *grid = (unsigned)(g < rows ? g : rows);
-  return NVFP4_OK;
-}
-
-template <typename T, typename W, int VEC, int ITEMS, bool BULK>
-int launch_fwd_rows(FwdArgs a, int threads, int sms, cudaStream_t st) {
-  auto kernel = k_fwd_rows<T, W, VEC, ITEMS, BULK>;
-  size_t smem = 0;
-  if constexpr (BULK) {
-    a.stages = ring_stages((size_t)a.cols * sizeof(T));
-    smem = (size_t)a.stages * a.cols * sizeof(T);
-    if (int e = set_smem(kernel, smem)) return e;
+    allowed.fetch_or(bit, std::memory_order_release);
   }
+  int n = kept[threads / 32].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0))
+      return cuda_status(e);
+    if (n < 1) n = 1;
+    kept[threads / 32].store(n, std::memory_order_relaxed);
+  }
+  *blocks = n;
+  return NVFP4_OK;
+}
+
+// Ring and grid of a launch: the SM's shared memory over the blocks that fit it
+// otherwise, two stages a block at least (fewer blocks then) while they fit.
+struct Launch {
+  int stages;
+  size_t smem;
   unsigned grid;
-  if (int e = grid_of(kernel, threads, smem, a.rows, sms, INT32_MAX, &grid)) return e;
-  kernel<<<grid, threads, smem, st>>>(a);
+};
+Launch launch_shape(int blocks, size_t stage_bytes, int sms, int64_t rows, int64_t most) {
+  Launch l;
+  const size_t least = 2 * stage_bytes <= kRingMost ? 2 : 1;
+  while (blocks > 1 && kRingBytes / blocks < least * stage_bytes) --blocks;
+  const size_t fit = kRingBytes / blocks / stage_bytes;
+  l.stages = (int)(fit < least ? least : fit > (size_t)kMaxStages ? kMaxStages : fit);
+  l.smem = l.stages * stage_bytes;
+  int64_t g = (int64_t)blocks * sms;
+  if (g > most) g = most;
+  l.grid = (unsigned)(g < rows ? g : rows);
+  return l;
+}
+// Partial rows of the weights' gradients: enough blocks to fill the SMs, more
+// of them where a row takes few threads.
+int64_t most_partials(int64_t rows, int64_t cols) {
+  const int64_t narrow = 2048 / cols;
+  const int64_t p = 296 * (narrow < 1 ? 1 : narrow > 4 ? 4 : narrow);
+  return rows < p ? rows : p;
+}
+uint32_t slot_of(size_t row_bytes, bool aligned) {
+  return (uint32_t)(aligned ? row_bytes : (row_bytes + 15) / 16 * 16 + 16);
+}
+
+template <typename T, typename W, bool ALIGNED, int ITEMS>
+int launch_fwd_rows(FwdArgs a, int threads, int sms, cudaStream_t st) {
+  constexpr auto kernel = k_fwd_rows<T, W, ALIGNED, ITEMS>;
+  int blocks;
+  if (int e = blocks_of<kernel>(threads, &blocks)) return e;
+  a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), ALIGNED);
+  const Launch l = launch_shape(blocks, a.slot_bytes, sms, a.rows, INT32_MAX);
+  a.stages = l.stages;
+  kernel<<<l.grid, threads, l.smem, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
 template <typename T, typename W>
 int launch_fwd(const FwdArgs& a, int sms, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool bulk = ((uintptr_t)a.x % 16 | (uintptr_t)a.y % 16 | (uintptr_t)(a.ldx % V) |
-                     (uintptr_t)(a.ldy % V) | (uintptr_t)(a.cols % V)) == 0;
-  Shape s;
-  if (bulk && row_shape(a.cols / V, 2, &s)) {
-    switch (s.items) {
-      case 1: return launch_fwd_rows<T, W, V, 1, true>(a, s.threads, sms, st);
-      case 2: return launch_fwd_rows<T, W, V, 2, true>(a, s.threads, sms, st);
-      default: return launch_fwd_rows<T, W, V, 4, true>(a, s.threads, sms, st);
-    }
-  }
-  if (a.cols <= 16 * kMaxThreads) {
-    const int threads = ((a.cols + 15) / 16 + 31) / 32 * 32;
-    return launch_fwd_rows<T, W, 1, 16, false>(a, threads, sms, st);
+  const bool aligned = ((uintptr_t)a.x % 16 | (uintptr_t)a.y % 16 | (uintptr_t)(a.ldx % V) |
+                        (uintptr_t)(a.ldy % V) | (uintptr_t)(a.cols % V)) == 0;
+  // 16 columns a thread (its gamma and beta fill half of the 64 registers that
+  // two blocks of 512 threads leave), 8 for a row of one warp, 32 for the widest.
+  if (aligned) {
+    const int64_t n = a.cols / V;
+    if (n <= 32 * (8 / V)) return launch_fwd_rows<T, W, true, 8 / V>(a, 32, sms, st);
+    if (int t = row_threads(n, 16 / V); t <= kMaxThreads)
+      return launch_fwd_rows<T, W, true, 16 / V>(a, t, sms, st);
+    if (int t = row_threads(n, 32 / V); t <= kMaxThreads)
+      return launch_fwd_rows<T, W, true, 32 / V>(a, t, sms, st);
+  } else {
+    if (a.cols <= 32 * 4) return launch_fwd_rows<T, W, false, 4>(a, 32, sms, st);
+    if (int t = row_threads(a.cols, 16); t <= kMaxThreads)
+      return launch_fwd_rows<T, W, false, 16>(a, t, sms, st);
   }
   const int64_t most = (int64_t)sms * 8;
   k_fwd_wide<T, W><<<(unsigned)(a.rows < most ? a.rows : most), kWideThreads, 0, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
-template <typename T, typename W, int VEC, int ITEMS, bool BULK, bool RES>
+template <typename T, typename W, bool ALIGNED, int ITEMS, bool RES>
 int launch_bwd_rows(BwdArgs& a, int threads, int sms, cudaStream_t st) {
-  auto kernel = k_bwd_rows<T, W, VEC, ITEMS, BULK, RES>;
-  size_t smem = 0;
-  if constexpr (BULK) {
-    const size_t stage = (size_t)a.cols * sizeof(T) * (RES ? 3 : 2);
-    a.stages = ring_stages(stage);
-    smem = a.stages * stage;
-    if (int e = set_smem(kernel, smem)) return e;
-  }
-  unsigned grid;
-  if (int e = grid_of(kernel, threads, smem, a.rows, sms, kMaxPartials, &grid)) return e;
-  a.partials = (int)grid;
-  kernel<<<grid, threads, smem, st>>>(a);
+  constexpr auto kernel = k_bwd_rows<T, W, ALIGNED, ITEMS, RES>;
+  int blocks;
+  if (int e = blocks_of<kernel>(threads, &blocks)) return e;
+  a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), ALIGNED);
+  const Launch l = launch_shape(blocks, (RES ? 3 : 2) * (size_t)a.slot_bytes, sms, a.rows,
+                                most_partials(a.rows, a.cols));
+  a.stages = l.stages;
+  a.partials = (int)l.grid;
+  kernel<<<l.grid, threads, l.smem, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
 template <typename T, typename W, bool RES>
 int launch_bwd(BwdArgs& a, int sms, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool bulk = ((uintptr_t)a.x % 16 | (uintptr_t)a.dy % 16 | (uintptr_t)a.dx % 16 |
-                     (uintptr_t)a.res % 16 | (uintptr_t)(a.ldx % V) | (uintptr_t)(a.lddy % V) |
-                     (uintptr_t)(a.lddx % V) | (uintptr_t)(RES ? a.ldr % V : 0) |
-                     (uintptr_t)(a.cols % V)) == 0;
-  Shape s;
-  if (bulk && row_shape(a.cols / V, 2, &s)) {
-    switch (s.items) {
-      case 1: return launch_bwd_rows<T, W, V, 1, true, RES>(a, s.threads, sms, st);
-      case 2: return launch_bwd_rows<T, W, V, 2, true, RES>(a, s.threads, sms, st);
-      default: return launch_bwd_rows<T, W, V, 4, true, RES>(a, s.threads, sms, st);
-    }
-  }
-  if (a.cols <= 16 * kMaxThreads) {
-    const int threads = ((a.cols + 15) / 16 + 31) / 32 * 32;
-    return launch_bwd_rows<T, W, 1, 16, false, RES>(a, threads, sms, st);
+  const bool aligned = ((uintptr_t)a.x % 16 | (uintptr_t)a.dy % 16 | (uintptr_t)a.dx % 16 |
+                        (uintptr_t)a.res % 16 | (uintptr_t)(a.ldx % V) | (uintptr_t)(a.lddy % V) |
+                        (uintptr_t)(a.lddx % V) | (uintptr_t)(RES ? a.ldr % V : 0) |
+                        (uintptr_t)(a.cols % V)) == 0;
+  // 16 columns a thread, 8 for rows of one warp, 32 for the widest.
+  if (aligned) {
+    const int64_t n = a.cols / V;
+    if (n <= 32 * (8 / V)) return launch_bwd_rows<T, W, true, 8 / V, RES>(a, 32, sms, st);
+    if (int t = row_threads(n, 16 / V); t <= kMaxThreads)
+      return launch_bwd_rows<T, W, true, 16 / V, RES>(a, t, sms, st);
+    if (int t = row_threads(n, 32 / V); t <= kMaxThreads)
+      return launch_bwd_rows<T, W, true, 32 / V, RES>(a, t, sms, st);
+  } else {
+    if (a.cols <= 32 * 4) return launch_bwd_rows<T, W, false, 4, RES>(a, 32, sms, st);
+    if (int t = row_threads(a.cols, 16); t <= kMaxThreads)
+      return launch_bwd_rows<T, W, false, 16, RES>(a, t, sms, st);
   }
   // The weights' partial sums first: dx may overwrite dy.
-  a.partials = (int)(a.rows < kMaxPartials ? a.rows : kMaxPartials);
+  a.partials = (int)most_partials(a.rows, a.cols);
   const dim3 grid((unsigned)((a.cols + kWideThreads - 1) / kWideThreads), (unsigned)a.partials);
   k_bwd_wide_w<T><<<grid, kWideThreads, 0, st>>>(a);
   if (cudaError_t e = cudaGetLastError()) return cuda_status(e);
@@ -773,8 +877,20 @@ int launch_bwd(BwdArgs& a, int sms, cudaStream_t st) {
 
 template <typename W>
 int launch_reduce(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t st) {
-  k_bwd_reduce<W><<<dim3((unsigned)((a.cols + 31) / 32), 2), 256, 0, st>>>(
-      a.partial, a.partials, a.cols, reinterpret_cast<W*>(dgamma), reinterpret_cast<W*>(dbeta));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.cols + 31) / 32), 2);
+  cfg.blockDim = dim3(32 * kReduceWarps);
+  cfg.stream = st;
+  // Launched while the rows are still being worked on; waits for them.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, k_bwd_reduce<W>, (const float*)a.partial,
+                                         a.partials, a.cols, reinterpret_cast<W*>(dgamma),
+                                         reinterpret_cast<W*>(dbeta)))
+    return cuda_status(e);
   return cuda_status(cudaGetLastError());
 }
 
@@ -824,7 +940,7 @@ NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int
     if (cudaError_t e = cudaMemsetAsync(amax_out, 0, sizeof(float), st)) return cuda_status(e);
   if (empty) return NVFP4_OK;
   FwdArgs a = {x, gamma, beta, y, mean, rstd, reinterpret_cast<uint32_t*>(amax_out),
-               rows, ldx, ldy, (int)cols, 1, eps};
+               rows, ldx, ldy, (int)cols, 1, 0u, eps};
   if (dtype == NVFP4_DTYPE_F32) return launch_fwd<float, float>(a, sms, st);
   if (dtype == NVFP4_DTYPE_BF16)
     return weight_dtype == NVFP4_DTYPE_F32 ? launch_fwd<__nv_bfloat16, float>(a, sms, st)
@@ -835,7 +951,7 @@ NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int
 
 NVFP4_API size_t nvfp4_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)(rows < kMaxPartials ? rows : kMaxPartials) * 2 * (size_t)cols * sizeof(float);
+  return (size_t)most_partials(rows, cols) * 2 * (size_t)cols * sizeof(float);
 }
 
 NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, int64_t lddy,
@@ -870,7 +986,7 @@ NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, in
     return NVFP4_OK;
   }
   BwdArgs a = {dy, x, mean, rstd, gamma, residual, dx, reinterpret_cast<float*>(workspace),
-               rows, lddy, ldx, ldr, lddx, (int)cols, 1, 0};
+               rows, lddy, ldx, ldr, lddx, (int)cols, 1, 0, 0u};
   auto rows_of = [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);

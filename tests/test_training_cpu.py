@@ -165,4 +165,5 @@ def test_workspaces_follow_the_sizes(nvlib):
     assert plain(128, 5120, 4096) == 0
     assert plain(0, 8, 64) == dact(4, 0, 64) == 0
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10, 7) == 10 * 2 * 7 * 4
-    assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 296 * 2 * 7 * 4
+    assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 4 * 296 * 2 * 7 * 4
+    assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 5120) == 296 * 2 * 5120 * 4
