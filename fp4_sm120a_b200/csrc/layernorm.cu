@@ -40,7 +40,6 @@ namespace {
 
 __device__ uint32_t g_layernorm_error_word;
 
-constexpr int kMaxThreads = 512;
 constexpr int kMaxStages = 8;
 constexpr size_t kRingBytes = 200 * 1024;      // of an SM, over its blocks
 constexpr size_t kRingMost = 226 * 1024;       // dynamic shared memory a block may ask for
@@ -158,16 +157,15 @@ __device__ __forceinline__ void span_load(const Span& s, uint32_t slot, const vo
     bulk_load(slot + s.skip, reinterpret_cast<const unsigned char*>(row) - s.lead + s.skip, s.bytes,
               bar);
 }
-// Which of a thread's items lie within the row.
+// How many of a thread's items lie within the row: the first `count`.
 template <typename T, bool ALIGNED, int ITEMS>
 struct Mine {
-  uint32_t in;
-  __device__ __forceinline__ explicit Mine(int cols) : in(0) {
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it)
-      if ((int)threadIdx.x + it * (int)blockDim.x < cols / Layout<T, ALIGNED>::kVec) in |= 1u << it;
+  int count;
+  __device__ __forceinline__ explicit Mine(int cols) {
+    const int n = cols / Layout<T, ALIGNED>::kVec - (int)threadIdx.x;
+    count = n > 0 ? (n + (int)blockDim.x - 1) / (int)blockDim.x : 0;
   }
-  __device__ __forceinline__ bool has(int it) const { return (in >> it) & 1u; }
+  __device__ __forceinline__ bool has(int it) const { return it < count; }
 };
 // The elements of an unaligned row outside its whole 16-byte units lie among
 // its first and last eight.  Lanes 0-15 of the first warp look after one each:
@@ -209,7 +207,7 @@ __device__ __forceinline__ void fetch(const Mine<T, ALIGNED, ITEMS>& my, const u
     }
   } else {
     // Loads without branches: what lies behind the row's end reads its first element.
-    const T* in = reinterpret_cast<const T*>(slot + span_of<false>(row, row_bytes).lead);
+    const T* in = reinterpret_cast<const T*>(slot + ((uint32_t)(uintptr_t)row & 15u));
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
       const T v = in[my.has(it) ? tid + it * nthr : 0];
@@ -311,9 +309,8 @@ struct FwdArgs {
 
 // One row per block at a time; two blocks or more share an SM and hide each
 // other's reductions.
-template <typename T, typename W, bool ALIGNED, int ITEMS>
-__global__ void __launch_bounds__(kMaxThreads, ALIGNED && ITEMS * Layout<T, ALIGNED>::kVec <= 16 ? 2 : 1)
-    k_fwd_rows(const FwdArgs a) {
+template <typename T, typename W, bool ALIGNED, int ITEMS, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared sh;
   constexpr int VEC = Layout<T, ALIGNED>::kVec, E = ITEMS * VEC;
@@ -501,8 +498,8 @@ struct BwdArgs {
   uint32_t slot_bytes;
 };
 
-template <typename T, typename W, bool ALIGNED, int ITEMS, bool RES>
-__global__ void __launch_bounds__(kMaxThreads) k_bwd_rows(const BwdArgs a) {
+template <typename T, typename W, bool ALIGNED, int ITEMS, int THREADS, bool RES>
+__global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   // k_bwd_reduce may be scheduled; it waits for this kernel to complete.
   asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ __align__(128) unsigned char smem[];
@@ -795,9 +792,9 @@ uint32_t slot_of(size_t row_bytes, bool aligned) {
   return (uint32_t)(aligned ? row_bytes : (row_bytes + 15) / 16 * 16 + 16);
 }
 
-template <typename T, typename W, bool ALIGNED, int ITEMS>
+template <typename T, typename W, bool ALIGNED, int ITEMS, int THREADS, int BLOCKS>
 int launch_fwd_rows(FwdArgs a, int threads, int sms, cudaStream_t st) {
-  constexpr auto kernel = k_fwd_rows<T, W, ALIGNED, ITEMS>;
+  constexpr auto kernel = k_fwd_rows<T, W, ALIGNED, ITEMS, THREADS, BLOCKS>;
   int blocks;
   if (int e = blocks_of<kernel>(threads, &blocks)) return e;
   a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), ALIGNED);
@@ -816,24 +813,26 @@ int launch_fwd(const FwdArgs& a, int sms, cudaStream_t st) {
   // two blocks of 512 threads leave), 8 for a row of one warp, 32 for the widest.
   if (aligned) {
     const int64_t n = a.cols / V;
-    if (n <= 32 * (8 / V)) return launch_fwd_rows<T, W, true, 8 / V>(a, 32, sms, st);
-    if (int t = row_threads(n, 16 / V); t <= kMaxThreads)
-      return launch_fwd_rows<T, W, true, 16 / V>(a, t, sms, st);
-    if (int t = row_threads(n, 32 / V); t <= kMaxThreads)
-      return launch_fwd_rows<T, W, true, 32 / V>(a, t, sms, st);
+    if (n <= 32 * (8 / V)) return launch_fwd_rows<T, W, true, 8 / V, 32, 16>(a, 32, sms, st);
+    if (int t = row_threads(n, 16 / V); t <= 512)
+      return launch_fwd_rows<T, W, true, 16 / V, 512, 2>(a, t, sms, st);
+    if (int t = row_threads(n, 32 / V); t <= 512)
+      return launch_fwd_rows<T, W, true, 32 / V, 512, 1>(a, t, sms, st);
   } else {
-    if (a.cols <= 32 * 4) return launch_fwd_rows<T, W, false, 4>(a, 32, sms, st);
-    if (int t = row_threads(a.cols, 16); t <= kMaxThreads)
-      return launch_fwd_rows<T, W, false, 16>(a, t, sms, st);
+    // Element-wise addressing takes more registers: 80 at two blocks of 384.
+    if (a.cols <= 32 * 4) return launch_fwd_rows<T, W, false, 4, 32, 16>(a, 32, sms, st);
+    const int t = row_threads(a.cols, 16);
+    if (t <= 384) return launch_fwd_rows<T, W, false, 16, 384, 2>(a, t, sms, st);
+    if (t <= 512) return launch_fwd_rows<T, W, false, 16, 512, 1>(a, t, sms, st);
   }
   const int64_t most = (int64_t)sms * 8;
   k_fwd_wide<T, W><<<(unsigned)(a.rows < most ? a.rows : most), kWideThreads, 0, st>>>(a);
   return cuda_status(cudaGetLastError());
 }
 
-template <typename T, typename W, bool ALIGNED, int ITEMS, bool RES>
+template <typename T, typename W, bool ALIGNED, int ITEMS, int THREADS, bool RES>
 int launch_bwd_rows(BwdArgs& a, int threads, int sms, cudaStream_t st) {
-  constexpr auto kernel = k_bwd_rows<T, W, ALIGNED, ITEMS, RES>;
+  constexpr auto kernel = k_bwd_rows<T, W, ALIGNED, ITEMS, THREADS, RES>;
   int blocks;
   if (int e = blocks_of<kernel>(threads, &blocks)) return e;
   a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), ALIGNED);
@@ -852,18 +851,22 @@ int launch_bwd(BwdArgs& a, int sms, cudaStream_t st) {
                         (uintptr_t)a.res % 16 | (uintptr_t)(a.ldx % V) | (uintptr_t)(a.lddy % V) |
                         (uintptr_t)(a.lddx % V) | (uintptr_t)(RES ? a.ldr % V : 0) |
                         (uintptr_t)(a.cols % V)) == 0;
-  // 16 columns a thread, 8 for rows of one warp, 32 for the widest.
+  // 8 columns a thread while a row then takes at most 512 threads (its warps, or
+  // those of several blocks, fill an SM), then 16, then 32.  Unaligned rows stay
+  // with 8 up to 704 threads: their addressing leaves 16 too few registers.
   if (aligned) {
     const int64_t n = a.cols / V;
-    if (n <= 32 * (8 / V)) return launch_bwd_rows<T, W, true, 8 / V, RES>(a, 32, sms, st);
-    if (int t = row_threads(n, 16 / V); t <= kMaxThreads)
-      return launch_bwd_rows<T, W, true, 16 / V, RES>(a, t, sms, st);
-    if (int t = row_threads(n, 32 / V); t <= kMaxThreads)
-      return launch_bwd_rows<T, W, true, 32 / V, RES>(a, t, sms, st);
+    if (int t = row_threads(n, 8 / V); t <= 512)
+      return launch_bwd_rows<T, W, true, 8 / V, 512, RES>(a, t, sms, st);
+    if (int t = row_threads(n, 16 / V); t <= 512)
+      return launch_bwd_rows<T, W, true, 16 / V, 512, RES>(a, t, sms, st);
+    if (int t = row_threads(n, 32 / V); t <= 512)
+      return launch_bwd_rows<T, W, true, 32 / V, 512, RES>(a, t, sms, st);
   } else {
-    if (a.cols <= 32 * 4) return launch_bwd_rows<T, W, false, 4, RES>(a, 32, sms, st);
-    if (int t = row_threads(a.cols, 16); t <= kMaxThreads)
-      return launch_bwd_rows<T, W, false, 16, RES>(a, t, sms, st);
+    if (int t = row_threads(a.cols, 8); t <= 704)
+      return launch_bwd_rows<T, W, false, 8, 704, RES>(a, t, sms, st);
+    if (int t = row_threads(a.cols, 16); t <= 512)
+      return launch_bwd_rows<T, W, false, 16, 512, RES>(a, t, sms, st);
   }
   // The weights' partial sums first: dx may overwrite dy.
   a.partials = (int)most_partials(a.rows, a.cols);
