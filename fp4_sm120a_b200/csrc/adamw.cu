@@ -54,17 +54,17 @@ struct Tensor {
   uint64_t n;
   uint64_t offset;
   float decay;           // lr * weight_decay, or weight_decay alone where lr comes from the device
-  uint32_t first_chunk;  // number of this tensor's first chunk in the launch
+  uint32_t vec;          // takes vector accesses
 };
 
 // The tensors of one launch travel as a kernel parameter: no device table to
 // allocate, copy or keep.  The short form keeps the parameter block small for
-// the usual small call.
+// the usual small call.  The chunk numbers lie side by side for the search.
 template <int CAP>
 struct Args {
   Tensor t[CAP];
+  uint32_t first_chunk[CAP];   // number of a tensor's first chunk in the launch
   int count;
-  uint32_t vec[(CAP + 31) / 32];  // bit t: tensor t takes vector accesses
   float beta1, beta2, omb1, omb2, eps;
   float step_size, rsqrt_bc2;
   const float* grad_scale;
@@ -79,13 +79,28 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
   return __uint_as_float((s << 23) | (s == 255u ? 0x400000u : 0u));
 }
 
-template <int DROP, uint32_t LOW>
-__device__ __forceinline__ float unpack8(uint32_t code, float scale) {
-  // `code` above LOW carries its own exponent (bias 7); below it counts steps
-  // of the lowest binade: 2^-6 (1 + f) - 2^-6.
-  const bool low = code < LOW;
-  const float t = __uint_as_float((code << DROP) + ((low ? 121u : 120u) << 23));
-  return (low ? t - 0.015625f : t) * scale;
+// Four 8-bit moments.  A code moved to the top of an fp16's exponent and
+// mantissa is the code's value times 2^-8 exactly, subnormals included (both
+// formats have a bias of 8 less than fp16's 15), so fp16's conversion decodes it.
+template <bool SIGNED>
+__device__ __forceinline__ void unpack8x4(uint32_t codes, uint32_t scale, float (&x)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t w = __byte_perm(codes, 0u, h ? 0x4342 : 0x4140);   // bytes 2h, 2h + 1 in halves
+    const uint32_t bits =
+        SIGNED ? ((w << 7) & 0x3F803F80u) | ((w << 8) & 0x80008000u) : w << 6;
+    unpack2<__half>(bits, x[2 * h], x[2 * h + 1]);
+  }
+  // 2^(s - 127 + 8); the largest scale takes its last binade in a second step.
+  const float f = scale == 0u ? 0.0f : scale_value(scale >= 247u && scale < 255u ? 254u
+                                                   : scale == 255u               ? 255u
+                                                                                 : scale + 8u);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] *= f;
+  if (scale >= 247u && scale < 255u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] *= __uint_as_float((scale - 246u + 127u) << 23);
+  }
 }
 // |x| scaled into [0, 256), rounded by 16 random bits at the top of the DROP
 // bits that are cut.
@@ -97,51 +112,41 @@ __device__ __forceinline__ uint32_t pack8(float mag, float inv_scale, uint32_t r
   return (t >> DROP) - ((low ? 121u : 120u) << (23 - DROP));
 }
 
-template <typename P, typename G, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Args<CAP> a) {
-  // The tensor of this block's chunk: the last one whose first chunk is not
-  // behind it.
-  int lo = 0, hi = a.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].first_chunk <= blockIdx.x) lo = mid; else hi = mid - 1;
-  }
-  const Tensor& t = a.t[lo];
-  const bool vec = (a.vec[lo >> 5] >> (lo & 31)) & 1u;
+// x / y and sqrt(x) to a few 2^-23: p's update is rounded to p's precision
+// afterwards, and the moments do not depend on it.
+__device__ __forceinline__ float fast_sqrt(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+struct Rates {
+  float keep, step_size, rbc2, gs;
+  uint64_t seed, offset;
+};
+
+// One chunk.  FULL: every element exists and all accesses are vectors.
+template <typename P, typename G, bool EIGHT, bool FULL, int CAP>
+__device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor& t,
+                                                const Rates& r, uint64_t base) {
   const uint64_t n = t.n;
-  const uint64_t base = (uint64_t)(blockIdx.x - t.first_chunk) * kChunk + threadIdx.x * kVec;
-
-  const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
-  float keep = 1.0f - t.decay, step_size = a.step_size, rbc2 = a.rsqrt_bc2;
-  if (a.scalars) {
-    const float lr = a.scalars[0];
-    step_size = __fdiv_rn(lr, a.scalars[1]);
-    rbc2 = __fdiv_rn(1.0f, __fsqrt_rn(a.scalars[2]));
-    keep = 1.0f - lr * t.decay;
-  }
-  uint64_t seed = 0, roff = 0;
-  if constexpr (EIGHT) {
-    seed = a.rng[0];
-    roff = a.rng[1] + a.step;
-  }
-
   P* pp = reinterpret_cast<P*>(t.p);
   const G* pg = reinterpret_cast<const G*>(t.g);
   float p[kUnroll][kVec], g[kUnroll][kVec];
-  float m[kUnroll][kVec], v[kUnroll][kVec];
-  uint32_t mc[kUnroll], vc[kUnroll];
-  uint8_t msb[kUnroll], vsb[kUnroll];
+  float m[EIGHT ? 1 : kUnroll][kVec], v[EIGHT ? 1 : kUnroll][kVec];
+  uint32_t mc[kUnroll], vc[kUnroll], sb[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const uint64_t i = base + (uint64_t)u * (kThreads * kVec);
-    const bool full = vec && i + kVec <= n;
+    const bool full = FULL || (t.vec && i + kVec <= n);
     load4(pp, i, n, full, p[u]);
     load4(pg, i, n, full, g[u]);
     if constexpr (EIGHT) {
       mc[u] = load4_bytes(reinterpret_cast<const uint8_t*>(t.m), i, n, full);
       vc[u] = load4_bytes(reinterpret_cast<const uint8_t*>(t.v), i, n, full);
-      msb[u] = i < n ? t.ms[i / kStateBlock] : 0;
-      vsb[u] = i < n ? t.vs[i / kStateBlock] : 0;
+      sb[u] = FULL || i < n ? (uint32_t)t.ms[i / kStateBlock] |
+                                  ((uint32_t)t.vs[i / kStateBlock] << 8)
+                            : 0u;
     } else {
       load4(reinterpret_cast<const float*>(t.m), i, n, full, m[u]);
       load4(reinterpret_cast<const float*>(t.v), i, n, full, v[u]);
@@ -151,47 +156,58 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Args
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const uint64_t i = base + (uint64_t)u * (kThreads * kVec);
-    const bool full = vec && i + kVec <= n;
+    const bool full = FULL || (t.vec && i + kVec <= n);
+    constexpr int kKeep = EIGHT ? 0 : 1;
+    float(&mu)[kVec] = m[u * kKeep];
+    float(&vu)[kVec] = v[u * kKeep];
     if constexpr (EIGHT) {
-      const float ms = scale_value(msb[u]);
-      const float vs = scale_value(vsb[u]);
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const uint32_t cm = (mc[u] >> (8 * k)) & 0xFFu;
-        const float x = unpack8<20, 8u>(cm & 127u, ms);
-        m[u][k] = (cm & 128u) ? -x : x;
-        v[u][k] = unpack8<19, 16u>((vc[u] >> (8 * k)) & 0xFFu, vs);
-      }
+      unpack8x4<true>(mc[u], sb[u] & 0xFFu, mu);
+      unpack8x4<false>(vc[u], sb[u] >> 8, vu);
     }
-    // The roundings of each operation are kept apart (no contraction): the
-    // stochastic rounding below then depends on the formula alone, not on how
-    // a compiler fuses it.
+    // The roundings of each operation on the moments are kept apart (no
+    // contraction): the stochastic rounding below then depends on the formula
+    // alone, not on how a compiler fuses it.  The sums are scalar for that: a
+    // pair's product and sum were seen to be fused in spite of their .rn.
+    const uint64_t b1 = pair(a.beta1, a.beta1), b2 = pair(a.beta2, a.beta2);
+    const uint64_t o1 = pair(a.omb1, a.omb1), o2 = pair(a.omb2, a.omb2), gs = pair(r.gs, r.gs);
+#pragma unroll
+    for (int k = 0; k < kVec; k += 2) {
+      const uint64_t gk = mul2(pair(g[u][k], g[u][k + 1]), gs);
+      float x0, x1, y0, y1;
+      split(mul2(pair(mu[k], mu[k + 1]), b1), x0, x1);
+      split(mul2(gk, o1), y0, y1);
+      mu[k] = __fadd_rn(x0, y0);
+      mu[k + 1] = __fadd_rn(x1, y1);
+      split(mul2(pair(vu[k], vu[k + 1]), b2), x0, x1);
+      split(mul2(mul2(gk, gk), o2), y0, y1);
+      vu[k] = __fadd_rn(x0, y0);
+      vu[k + 1] = __fadd_rn(x1, y1);
+    }
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      const float gk = __fmul_rn(g[u][k], gs);
-      m[u][k] = __fadd_rn(__fmul_rn(m[u][k], a.beta1), __fmul_rn(gk, a.omb1));
-      v[u][k] = __fadd_rn(__fmul_rn(v[u][k], a.beta2), __fmul_rn(__fmul_rn(gk, gk), a.omb2));
-      const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[u][k]), rbc2), a.eps);
-      p[u][k] = __fadd_rn(__fmul_rn(p[u][k], keep),
-                          -__fmul_rn(__fdiv_rn(m[u][k], den), step_size));
+      const float update = __fdividef(mu[k], fmaf(fast_sqrt(vu[k]), r.rbc2, a.eps));
+      p[u][k] = fmaf(-update, r.step_size, p[u][k] * r.keep);
     }
     store4(pp, i, n, full, p[u]);
     if (t.copy != nullptr) store4(t.copy, i, n, full, p[u]);
     if (a.amax != nullptr) {
+      // the amax of what the cast will read: p rounded to bf16
+      if (FULL || i + kVec <= n) {
+        top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][0], p[u][1]) & 0x7FFF7FFFu);
+        top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][2], p[u][3]) & 0x7FFF7FFFu);
+      } else {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        // the amax of what the cast will read: p rounded to bf16
-        const float b = __bfloat162float(__float2bfloat16_rn(p[u][k]));
-        if (i + k < n) top = max(top, __float_as_uint(b) & 0x7FFFFFFFu);
+        for (int k = 0; k < kVec; ++k)
+          if (i + k < n) top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][k], 0.0f) & 0x7FFFu);
       }
     }
     if constexpr (EIGHT) {
       uint32_t am = 0, av = 0;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
-        if (i + k >= n) m[u][k] = v[u][k] = 0.0f;
-        am = max(am, __float_as_uint(m[u][k]) & 0x7FFFFFFFu);
-        av = max(av, __float_as_uint(v[u][k]) & 0x7FFFFFFFu);
+        if (!FULL && i + k >= n) mu[k] = vu[k] = 0.0f;
+        am = max(am, __float_as_uint(mu[k]) & 0x7FFFFFFFu);
+        av = max(av, __float_as_uint(vu[k]) & 0x7FFFFFFFu);
       }
       // NaN patterns are above infinity's, so the unsigned maximum keeps them.
       am = __reduce_max_sync(0xFFFFFFFFu, am) >> 23;
@@ -201,57 +217,128 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Args
       const float im = __uint_as_float((254u - min(sm, 254u)) << 23);
       const float iv = __uint_as_float((254u - min(sv, 254u)) << 23);
       Philox ph;
-      ph.init(seed, (t.offset + i) / kVec, roff, 0);
+      ph.init(r.seed, (t.offset + i) / kVec, r.offset, 0);
       const uint4 r4 = ph.generate4();
-      const uint32_t r[kVec] = {r4.x, r4.y, r4.z, r4.w};
+      const uint32_t w[kVec] = {r4.x, r4.y, r4.z, r4.w};
       uint32_t om = 0, ov = 0;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
-        uint32_t cm = sm == 255u ? 0u : pack8<20>(fabsf(m[u][k]), im, r[k] & 0xFFFFu);
-        cm |= m[u][k] < 0.0f ? 128u : 0u;
-        uint32_t cv = sv == 255u ? 0u : pack8<19>(v[u][k], iv, r[k] >> 16);
-        if (sv != 255u && v[u][k] > 0.0f) cv = max(cv, 1u);
-        om |= cm << (8 * k);
-        ov |= cv << (8 * k);
+        const uint32_t cm = pack8<20>(fabsf(mu[k]), im, w[k] & 0xFFFFu);
+        const uint32_t cv = pack8<19>(vu[k], iv, w[k] >> 16);
+        om |= ((sm == 255u ? 0u : cm) | (mu[k] < 0.0f ? 128u : 0u)) << (8 * k);
+        ov |= (sv == 255u ? 0u : max(cv, vu[k] > 0.0f ? 1u : 0u)) << (8 * k);
       }
       store4_bytes(reinterpret_cast<uint8_t*>(t.m), i, n, full, om);
       store4_bytes(reinterpret_cast<uint8_t*>(t.v), i, n, full, ov);
-      if ((threadIdx.x & 31) == 0 && i < n) {
+      if ((threadIdx.x & 31) == 0 && (FULL || i < n)) {
         t.ms[i / kStateBlock] = (uint8_t)sm;
         t.vs[i / kStateBlock] = (uint8_t)sv;
       }
     } else {
-      store4(reinterpret_cast<float*>(t.m), i, n, full, m[u]);
-      store4(reinterpret_cast<float*>(t.v), i, n, full, v[u]);
+      store4(reinterpret_cast<float*>(t.m), i, n, full, mu);
+      store4(reinterpret_cast<float*>(t.v), i, n, full, vu);
     }
   }
+  return top;
+}
+
+template <typename P, typename G, bool EIGHT, int CAP>
+__global__ void __launch_bounds__(kThreads, 3) k_adamw(const __grid_constant__ Args<CAP> a) {
+  // The tensor of this block's chunk: the last one whose first chunk is not
+  // behind it.
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.first_chunk[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  const Tensor& t = a.t[lo];
+  const uint64_t chunk = (uint64_t)(blockIdx.x - a.first_chunk[lo]) * kChunk;
+  Rates r;
+  r.gs = a.grad_scale ? *a.grad_scale : 1.0f;
+  r.keep = 1.0f - t.decay;
+  r.step_size = a.step_size;
+  r.rbc2 = a.rsqrt_bc2;
+  if (a.scalars) {
+    const float lr = a.scalars[0];
+    r.step_size = __fdiv_rn(lr, a.scalars[1]);
+    r.rbc2 = __fdiv_rn(1.0f, __fsqrt_rn(a.scalars[2]));
+    r.keep = 1.0f - lr * t.decay;
+  }
+  if constexpr (EIGHT) {
+    // Through a warp reduction, whose result the compiler knows to be the same
+    // in all lanes: the key schedule then costs the lanes nothing.
+    const uint64_t seed = a.rng[0];
+    r.seed = (uint64_t)__reduce_or_sync(0xFFFFFFFFu, (uint32_t)(seed >> 32)) << 32 |
+             __reduce_or_sync(0xFFFFFFFFu, (uint32_t)seed);
+    r.offset = a.rng[1] + a.step;
+  }
+  const uint64_t base = chunk + threadIdx.x * kVec;
+  uint32_t top = t.vec && chunk + kChunk <= t.n
+                     ? adamw_chunk<P, G, EIGHT, true, CAP>(a, t, r, base)
+                     : adamw_chunk<P, G, EIGHT, false, CAP>(a, t, r, base);
   if (a.amax != nullptr) {
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    top = __reduce_max_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16)) << 16;
     // The word only grows: a stale read costs an atomic, never a result.
     if ((threadIdx.x & 31) == 0 && top > *(volatile uint32_t*)(a.amax + lo))
       atomicMax(a.amax + lo, top);
   }
 }
 
-template <typename OUT, int DROP, uint32_t LOW, bool SIGNED>
+// N values a thread, which leave as one 16-byte vector (FULL), four times over;
+// else four values element by element.
+template <typename OUT, bool SIGNED, bool FULL>
 __global__ void __launch_bounds__(kThreads) k_unpack_state(const uint8_t* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales,
-                                                           size_t n, bool vec,
-                                                           OUT* __restrict__ out) {
-  const size_t stride = (size_t)gridDim.x * kThreads * kVec;
-  for (size_t i = ((size_t)blockIdx.x * kThreads + threadIdx.x) * kVec; i < n; i += stride) {
-    const bool full = vec && i + kVec <= n;
-    const uint32_t c = load4_bytes(codes, i, n, full);
-    const float s = scale_value(scales[i / kStateBlock]);
-    float x[kVec];
+                                                           size_t n, OUT* __restrict__ out) {
+  constexpr int N = FULL ? 16 / (int)sizeof(OUT) : 4, U = 4;
+  const size_t base = (size_t)blockIdx.x * (kThreads * N * U) + threadIdx.x * N;
+  uint32_t c[U][N / 4], s[U];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const uint32_t b = (c >> (8 * k)) & 0xFFu;
-      const float y = unpack8<DROP, LOW>(SIGNED ? b & 127u : b, s);
-      x[k] = SIGNED && (b & 128u) ? -y : y;
+  for (int u = 0; u < U; ++u) {
+    const size_t i = base + (size_t)u * (kThreads * N);
+    const bool in = FULL && i + N <= n;
+    if (in && N == 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(codes + i);
+      c[u][0] = q.x;
+      c[u][N / 4 - 1] = q.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) c[u][j] = load4_bytes(codes, i + 4 * j, n, in);
     }
-    store4(out, i, n, full, x);
+    s[u] = i < n ? scales[i / kStateBlock] : 0u;
   }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t i = base + (size_t)u * (kThreads * N);
+    float x[N / 4][4];
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) unpack8x4<SIGNED>(c[u][j], s[u], x[j]);
+    if (FULL && i + N <= n && N == 8) {
+      *reinterpret_cast<uint4*>(out + i) =
+          make_uint4(pack2<__nv_bfloat16>(x[0][0], x[0][1]), pack2<__nv_bfloat16>(x[0][2], x[0][3]),
+                     pack2<__nv_bfloat16>(x[N / 4 - 1][0], x[N / 4 - 1][1]),
+                     pack2<__nv_bfloat16>(x[N / 4 - 1][2], x[N / 4 - 1][3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j)
+        store4(out, i + 4 * j, n, FULL && i + N <= n, x[j]);
+    }
+  }
+}
+
+template <typename OUT, bool SIGNED>
+int launch_unpack(const void* codes, const uint8_t* scales, size_t n, void* out, cudaStream_t st) {
+  const uint8_t* c = reinterpret_cast<const uint8_t*>(codes);
+  OUT* o = reinterpret_cast<OUT*>(out);
+  constexpr size_t kFull = 16 / sizeof(OUT);
+  const bool full = (uintptr_t)c % kFull == 0 && (uintptr_t)o % 16 == 0;
+  const size_t per = (full ? kFull : 4) * 4 * kThreads, blocks = (n + per - 1) / per;
+  if (blocks > 0x7FFFFFFF) return NVFP4_ERR_INVALID_SHAPE;
+  if (full)
+    k_unpack_state<OUT, SIGNED, true><<<(unsigned)blocks, kThreads, 0, st>>>(c, scales, n, o);
+  else
+    k_unpack_state<OUT, SIGNED, false><<<(unsigned)blocks, kThreads, 0, st>>>(c, scales, n, o);
+  return cuda_status(cudaGetLastError());
 }
 
 template <typename P, typename G, bool EIGHT, int CAP>
@@ -261,7 +348,6 @@ int launch_group(const nvfp4_adamw_tensor* tensors, int count, double lr, Args<C
   for (int at = 0; at < count;) {
     uint64_t chunks = 0;
     int k = 0;
-    for (uint32_t& w : a.vec) w = 0;
     const int begin = at;
     for (; at < count && k < CAP; ++at) {
       const nvfp4_adamw_tensor& t = tensors[at];
@@ -274,12 +360,11 @@ int launch_group(const nvfp4_adamw_tensor* tensors, int count, double lr, Args<C
       d.n = t.n;
       d.offset = t.offset;
       d.decay = a.scalars ? (float)t.weight_decay : (float)(lr * t.weight_decay);
-      d.first_chunk = (uint32_t)chunks;
+      a.first_chunk[k] = (uint32_t)chunks;
       const uintptr_t state = EIGHT ? (uintptr_t)t.exp_avg % 4 | (uintptr_t)t.exp_avg_sq % 4
                                     : (uintptr_t)t.exp_avg % 16 | (uintptr_t)t.exp_avg_sq % 16;
-      if (((uintptr_t)t.param % (4 * sizeof(P)) | (uintptr_t)t.grad % (4 * sizeof(G)) | state |
-           (uintptr_t)t.copy % 8) == 0)
-        a.vec[k >> 5] |= 1u << (k & 31);
+      d.vec = ((uintptr_t)t.param % (4 * sizeof(P)) | (uintptr_t)t.grad % (4 * sizeof(G)) | state |
+               (uintptr_t)t.copy % 8) == 0;
       chunks += need;
       ++k;
     }
@@ -319,7 +404,11 @@ int launch_all(const nvfp4_adamw_tensor* tensors, int count, double lr, double b
     Args<32> a;
     return go(a);
   }
-  Args<384> a;
+  if (count <= 112) {
+    Args<112> a;
+    return go(a);
+  }
+  Args<368> a;
   return go(a);
 }
 
@@ -407,27 +496,14 @@ NVFP4_API int nvfp4_adamw_unpack_state(const void* codes, const uint8_t* scales,
   if ((uintptr_t)out % osize) return NVFP4_ERR_MISALIGNED;
   int sms = 0;
   if (int e = device_sm_count(&sms)) return e;
-  size_t blocks = (n + kThreads * kVec - 1) / (kThreads * kVec);
-  if (blocks > (size_t)sms * 32) blocks = (size_t)sms * 32;
-  const bool vec = (uintptr_t)codes % 4 == 0 && (uintptr_t)out % (4 * osize) == 0;
-  const uint8_t* c = reinterpret_cast<const uint8_t*>(codes);
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)blocks;
-  if (out_dtype == NVFP4_DTYPE_F32) {
-    float* o = reinterpret_cast<float*>(out);
-    if (moment == NVFP4_EXP_AVG)
-      k_unpack_state<float, 20, 8u, true><<<grid, kThreads, 0, st>>>(c, scales, n, vec, o);
-    else
-      k_unpack_state<float, 19, 16u, false><<<grid, kThreads, 0, st>>>(c, scales, n, vec, o);
-  } else {
-    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(out);
-    if (moment == NVFP4_EXP_AVG)
-      k_unpack_state<__nv_bfloat16, 20, 8u, true><<<grid, kThreads, 0, st>>>(c, scales, n, vec, o);
-    else
-      k_unpack_state<__nv_bfloat16, 19, 16u, false><<<grid, kThreads, 0, st>>>(c, scales, n, vec,
-                                                                               o);
-  }
-  return cuda_status(cudaGetLastError());
+  if (out_dtype == NVFP4_DTYPE_F32)
+    return moment == NVFP4_EXP_AVG
+               ? launch_unpack<float, true>(codes, scales, n, out, st)
+               : launch_unpack<float, false>(codes, scales, n, out, st);
+  return moment == NVFP4_EXP_AVG
+             ? launch_unpack<__nv_bfloat16, true>(codes, scales, n, out, st)
+             : launch_unpack<__nv_bfloat16, false>(codes, scales, n, out, st);
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
 // Element types of the element-wise kernels (fp32, bf16, fp16): conversion to
 // and from fp32, and groups of four moved as one vector where the tensor's
-// alignment allows (`full`), else element by element below the end `n`.
+// alignment allows (`full`), else element by element below the end `n`; pairs
+// of fp32.
 #pragma once
 
 #include <cstdint>
@@ -56,6 +57,30 @@ __device__ __forceinline__ void unpack2<__half>(uint32_t w, float& a, float& b) 
   b = f.y;
 }
 
+// Pairs of fp32 in one instruction (add / mul / fma.rn.f32x2).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, uint64_t i, uint64_t n, bool full,
                                       float (&x)[4]) {
