@@ -102,14 +102,47 @@ __device__ __forceinline__ void unpack8x4(uint32_t codes, uint32_t scale, float 
     for (int k = 0; k < 4; ++k) x[k] *= __uint_as_float((scale - 246u + 127u) << 23);
   }
 }
-// |x| scaled into [0, 256), rounded by 16 random bits at the top of the DROP
-// bits that are cut.
+// Moments of four elements as the step reads them: exp_avg through E4M3's own
+// conversion.  (A block that is not finite holds zero codes, and 0 times the
+// scale's infinity is NaN.)
+__device__ __forceinline__ void read_avg(uint32_t codes, uint32_t scale, float (&x)[4]) {
+  uint32_t lo, hi;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+  unpack2<__half>(lo, x[0], x[1]);
+  unpack2<__half>(hi, x[2], x[3]);
+  const float f = __uint_as_float(scale << 23);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] *= f;
+}
+__device__ __forceinline__ void read_avg_sq(uint32_t codes, uint32_t scale, float (&x)[4]) {
+  unpack2<__half>(__byte_perm(codes, 0u, 0x4140) << 6, x[0], x[1]);
+  unpack2<__half>(__byte_perm(codes, 0u, 0x4342) << 6, x[2], x[3]);
+  const float f = __uint_as_float(scale << 23);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = x[k] * f * 256.0f;
+}
+
+// Stochastic rounding of x, scaled below 256 in magnitude by `inv`: times 2^-120
+// the 8-bit formats' lowest binade (from 2^-6 down, equal steps) is fp32's own
+// subnormal range, so that the fp32 bits of every value count steps of 2^-DROP
+// of a code; 16 random bits below the code's last place carry into it.
 template <int DROP>
-__device__ __forceinline__ uint32_t pack8(float mag, float inv_scale, uint32_t r16) {
-  const float y = __fmul_rn(mag, inv_scale);
-  const bool low = y < 0.015625f;
-  const uint32_t t = __float_as_uint(low ? __fadd_rn(y, 0.015625f) : y) + (r16 << (DROP - 16));
-  return (t >> DROP) - ((low ? 121u : 120u) << (23 - DROP));
+__device__ __forceinline__ uint32_t rounded_bits(float x, float inv, uint32_t r16) {
+  return __float_as_uint(x * inv * 7.52316384526264e-37f) + (r16 << (DROP - 16));
+}
+// Byte 3 of four words in one.
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+__device__ __forceinline__ float max4_nan(float a, float b, float c, float d) {
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2, %3;\n\tmax.NaN.f32 %0, t, %4;\n\t}"
+      : "=f"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
 
 // x / y and sqrt(x) to a few 2^-23: p's update is rounded to p's precision
@@ -161,8 +194,8 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
     float(&mu)[kVec] = m[u * kKeep];
     float(&vu)[kVec] = v[u * kKeep];
     if constexpr (EIGHT) {
-      unpack8x4<true>(mc[u], sb[u] & 0xFFu, mu);
-      unpack8x4<false>(vc[u], sb[u] >> 8, vu);
+      read_avg(mc[u], sb[u] & 0xFFu, mu);
+      read_avg_sq(vc[u], sb[u] >> 8, vu);
     }
     // The roundings of each operation on the moments are kept apart (no
     // contraction): the stochastic rounding below then depends on the formula
@@ -202,16 +235,17 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
       }
     }
     if constexpr (EIGHT) {
-      uint32_t am = 0, av = 0;
+      if (!FULL) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        if (!FULL && i + k >= n) mu[k] = vu[k] = 0.0f;
-        am = max(am, __float_as_uint(mu[k]) & 0x7FFFFFFFu);
-        av = max(av, __float_as_uint(vu[k]) & 0x7FFFFFFFu);
+        for (int k = 0; k < kVec; ++k)
+          if (i + k >= n) mu[k] = vu[k] = 0.0f;
       }
       // NaN patterns are above infinity's, so the unsigned maximum keeps them.
-      am = __reduce_max_sync(0xFFFFFFFFu, am) >> 23;
-      av = __reduce_max_sync(0xFFFFFFFFu, av) >> 23;
+      const uint32_t am =
+          __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(max4_nan(fabsf(mu[0]), fabsf(mu[1]),
+                                                                  fabsf(mu[2]), fabsf(mu[3])))) >> 23;
+      const uint32_t av =
+          __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(max4_nan(vu[0], vu[1], vu[2], vu[3]))) >> 23;
       const uint32_t sm = am == 255u ? 255u : max((int)am - 7, 1);
       const uint32_t sv = av == 255u ? 255u : max((int)av - 7, 1);
       const float im = __uint_as_float((254u - min(sm, 254u)) << 23);
@@ -220,14 +254,25 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
       ph.init(r.seed, (t.offset + i) / kVec, r.offset, 0);
       const uint4 r4 = ph.generate4();
       const uint32_t w[kVec] = {r4.x, r4.y, r4.z, r4.w};
-      uint32_t om = 0, ov = 0;
+      uint32_t bm[kVec], bv[kVec];
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
-        const uint32_t cm = pack8<20>(fabsf(mu[k]), im, w[k] & 0xFFFFu);
-        const uint32_t cv = pack8<19>(vu[k], iv, w[k] >> 16);
-        om |= ((sm == 255u ? 0u : cm) | (mu[k] < 0.0f ? 128u : 0u)) << (8 * k);
-        ov |= (sv == 255u ? 0u : max(cv, vu[k] > 0.0f ? 1u : 0u)) << (8 * k);
+        // The code to the top byte; a sign only below zero (-0 + 0 is +0).
+        const uint32_t tm = rounded_bits<20>(mu[k] + 0.0f, im, w[k] & 0xFFFFu);
+        bm[k] = (tm << 4) | (tm & 0x80000000u);
+        uint32_t tv = rounded_bits<19>(vu[k], iv, w[k] >> 16);
+        if (vu[k] > 0.0f) tv = max(tv, 1u << 19);
+        bv[k] = tv << 5;
       }
+      uint32_t om = top_bytes(bm[0], bm[1], bm[2], bm[3]);
+      uint32_t ov = top_bytes(bv[0], bv[1], bv[2], bv[3]);
+      if (sm == 255u) {
+        // No code has a value here; the signs stay.
+        om = 0u;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) om |= mu[k] < 0.0f ? 0x80u << (8 * k) : 0u;
+      }
+      if (sv == 255u) ov = 0u;
       store4_bytes(reinterpret_cast<uint8_t*>(t.m), i, n, full, om);
       store4_bytes(reinterpret_cast<uint8_t*>(t.v), i, n, full, ov);
       if ((threadIdx.x & 31) == 0 && (FULL || i < n)) {
