@@ -18,13 +18,14 @@
 // thread, a warp's stores cover 32 consecutive elements of a row of D, and a
 // column sum of D (the bias gradient) never leaves a thread.
 //
-// Work: output tiles of 128 (n) x TN (m), persistent grid, warp-specialised:
+// m > 128 takes the kernel in gemm_nvfp4_wide_sm100.cu.  Here: output tiles of
+// 128 (n) x TN (m <= TN), warp-specialised:
 //   warps 0-7   epilogue: two groups of four warps, each half of the columns
 //   warp  8     TMA producer: 128-byte k-slices (256 codes) of both operands
 //               into a ring of 128-byte-swizzled stages
 //   warp  9     MMA issuer: copies a stage's scales to TMEM (tcgen05.cp),
 //               issues four K = 64 MMAs; owns the TMEM columns
-//   warps 10-   scale loaders: the casts' row-major scales into the 32 x 16
+//   warps 10-11 scale loaders: the casts' row-major scales into the 32 x 16
 //               byte atoms that tcgen05.cp spreads over the lanes.  A lane
 //               takes 16 bytes (one k-slice) of rows l, l + 32, l + 64, l + 96,
 //               so the transpose is a choice of registers.
@@ -49,30 +50,24 @@ constexpr int kMaxSplit = 8;
 // Tile widths and what follows from them.
 template <int TN>
 struct Tile {
-  static constexpr int kAtomsT = (TN + 127) / 128;           // scale atoms per step, m side
   static constexpr uint32_t kBytesF = kTileF * 128;
   static constexpr uint32_t kBytesT = TN * 128;
-  static constexpr uint32_t kBytesSf = kSteps * (1 + kAtomsT) * kAtomBytes;
+  static constexpr uint32_t kBytesSf = kSteps * 2 * kAtomBytes;
   static constexpr uint32_t kStageBytes = kBytesF + kBytesT + kBytesSf;
-  // TN >= 128: one CTA per SM with all of its shared memory.  Narrow tiles
-  // (short m) leave room for two, so that a split that does not divide the
-  // SMs evenly still runs in one wave.
+  static constexpr uint32_t kPlaceBytes = 2 * 128 * 16;      // scales in flight, a stage
+  // TN = 128: one CTA per SM with all of its shared memory.  Narrower tiles
+  // leave room for two, so that a split that does not divide the SMs evenly
+  // still runs in one wave.
   static constexpr int kCtasPerSm = TN >= 128 ? 1 : 2;
   static constexpr uint32_t kBudget = kSmemMax / kCtasPerSm - 2048;
-  static constexpr int kStagesRaw = (int)(kBudget / kStageBytes);
+  static constexpr int kStagesRaw = (int)(kBudget / (kStageBytes + kPlaceBytes));
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
-  static constexpr int kAccStages = TN <= 128 ? 2 : 1;
-  static constexpr uint32_t kSfCols = kSteps * 4 * (1 + kAtomsT);   // TMEM columns of a slice's scales
+  static constexpr int kAccStages = 2;
+  static constexpr uint32_t kSfCols = kSteps * 4 * 2;      // TMEM columns of a slice's scales
   static constexpr uint32_t kColsUsed = kAccStages * TN + 2 * kSfCols;
   static constexpr uint32_t kTmemCols = kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
-  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024;   // + alignment
-  // Scale loaders.  A whole SM's registers pay for two warps a part and turns
-  // of two slices (32 bytes of a row: one sector, not half of one twice).
-  static constexpr int kSfParts = 1 + kAtomsT;
-  static constexpr int kSfPerPart = kCtasPerSm == 1 ? 2 : 1;
-  static constexpr int kSfGroup = kCtasPerSm == 1 ? 2 : 1;
-  static constexpr int kSfAhead = kCtasPerSm == 1 ? 1 : 2;
-  static constexpr int kThreads = 32 * (kWarpScales + kSfParts * kSfPerPart);
+  static constexpr uint32_t kSmemBytes = kStages * (kStageBytes + kPlaceBytes) + 1024;
+  static constexpr int kThreads = 32 * (kWarpScales + 2);
   static_assert(kStages >= 3, "the scale columns of slice g - 2 are checked through its stage");
   static_assert(kColsUsed <= 512, "TMEM");
   static_assert(kTmemCols * kCtasPerSm <= 512, "TMEM of all CTAs of an SM");
@@ -81,6 +76,38 @@ struct Tile {
   static constexpr uint32_t kIdesc =
       (1u << 7) | (1u << 10) | ((uint32_t)(TN / 8) << 17) | ((uint32_t)(kTileF / 16) << 24);
 };
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+// 16 scale bytes (one k-slice) of a row (null: zeros) on their way to shared
+// memory; bytes behind the row's end become zero.
+__device__ __forceinline__ void fetch_scales(uint32_t dst, const uint8_t* row,
+                                             const uint8_t* any, int pitch, int width, int slice) {
+  const uint8_t* p = row ? row + slice * 16 : any;
+  const int left = row ? pitch - slice * 16 : 0;
+  if (width == 16) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p),
+                 "r"(left > 0 ? 16 : 0)
+                 : "memory");
+  } else if (width == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = 4 * i < left;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i),
+                   "l"(in ? p + 4 * i : any), "r"(in ? 4 : 0)
+                   : "memory");
+    }
+  } else {
+    const uint4 v = load_scales(row, pitch, width, slice);
+    sts128(dst, v.x, v.y, v.z, v.w);
+  }
+}
 
 // A thread's share of a tile: one feature (lane) and COLS columns from
 // column c0 on, the accumulator's values in v.
@@ -153,7 +180,7 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 1 + C::kSfParts);
+      mbar_init(full(s), 1 + 2);
       mbar_init(empty(s), 1);
     }
     for (int a = 0; a < C::kAccStages; ++a) {
@@ -254,16 +281,13 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
 #pragma unroll
           for (int q = 0; q < kSteps; ++q) {
             cp_scales(sf_f + 4 * q, desc_s + q * (kAtomBytes / 16));
-#pragma unroll
-            for (int b = 0; b < C::kAtomsT; ++b)
-              cp_scales(sf_t + 4 * (q * C::kAtomsT + b),
-                        desc_s + (kSteps * (1 + b) + q) * (kAtomBytes / 16));
+            cp_scales(sf_t + 4 * q, desc_s + (kSteps + q) * (kAtomBytes / 16));
           }
 #pragma unroll
           for (int q = 0; q < kSteps; ++q)
             if (q < steps)
               mma_nvfp4(d, desc_f + 2 * q, desc_t + 2 * q, C::kIdesc, sf_f + 4 * q,
-                        sf_t + 4 * q * C::kAtomsT, s > s_begin || q > 0);
+                        sf_t + 4 * q, s > s_begin || q > 0);
           tc_commit(empty(stage));
         }
         __syncwarp();
@@ -281,102 +305,73 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     volatile uint32_t never = 0u;
     wait_warp(drain, 0, &never, kErrTimeoutDrain);
   } else if (warp >= kWarpScales) {
-    // kSfPerPart warps share a part (0: n side; 1, 2: 128 rows each of the m
-    // side) by taking turns; a turn is kSfGroup k-slices of one tile, whose
-    // scales lie side by side in memory.  Each warp keeps kSfAhead turns in
-    // flight ahead of the one it stores.
-    constexpr int G = C::kSfGroup, W = C::kSfPerPart, D = C::kSfAhead;
-    const int part = (warp - kWarpScales) / W, turn0 = (warp - kWarpScales) % W;
+    // One warp a part (0: n side, 1: m side).  A lane looks after the rows
+    // l, l + 32, l + 64, l + 96: it fetches their 16 bytes of a k-slice
+    // asynchronously into a place of its own, as many slices ahead as the ring
+    // has stages, and later reads them back in the order of the atoms.  Nobody
+    // else touches that place, so its own wait is all the synchronization.
+    const int part = warp - kWarpScales;
     const bool f_side = part == 0;
     const uint8_t* sf = f_side ? p.sf_f : p.sf_t;
     const int width = f_side ? p.sf_width_f : p.sf_width_t;
     const int rows = f_side ? p.n : p.m;
-    const int tile_rows = f_side ? kTileF : min(TN - (part - 1) * 128, 128);
-    const int per_tile = s_end - s_begin;           // slices
-    const int turns = (per_tile + G - 1) / G;       // a tile's
-    // A cursor over this warp's turns.
+    const int tile_rows = f_side ? kTileF : TN;
+    const uint32_t place = ring + C::kStages * C::kStageBytes +
+                           (uint32_t)(part * C::kStages * 4 * 32 + lane) * 16;
     struct Cursor {
-      int tile, turn;
+      int tile, slice;
     };
-    auto advance = [&](Cursor& c) {
-      for (c.turn += W; c.turn >= turns && c.tile < tiles; c.turn -= turns) c.tile += stride;
+    auto next = [&](Cursor& c) {
+      if (++c.slice == s_end) { c.slice = s_begin; c.tile += stride; }
     };
-    uint4 buf[D + 1][G][4];
     const uint8_t* row[4];                          // this lane's rows, null behind the end
     int row_tile = -1;
-    auto load = [&](Cursor& c, uint4 (&b)[G][4]) {
-      if (c.tile >= tiles) return;
-      if (c.tile != row_tile) {
-        row_tile = c.tile;
-        int tf, tt;
-        tile_at(p, c.tile, tf, tt);
-        const int row0 = f_side ? tf * kTileF : tt * TN + (part - 1) * 128;
+    auto fetch = [&](const Cursor& c, uint32_t slot) {
+      if (c.tile < tiles) {
+        if (c.tile != row_tile) {
+          row_tile = c.tile;
+          int tf, tt;
+          tile_at(p, c.tile, tf, tt);
+          const int row0 = f_side ? tf * kTileF : tt * TN;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = q * 32 + lane;
-          row[q] = r < tile_rows && row0 + r < rows ? sf + (int64_t)(row0 + r) * p.sf_pitch
-                                                    : nullptr;
+          for (int q = 0; q < 4; ++q) {
+            const int r = q * 32 + lane;
+            row[q] = r < tile_rows && row0 + r < rows ? sf + (int64_t)(row0 + r) * p.sf_pitch
+                                                      : nullptr;
+          }
         }
-      }
-      const int s = s_begin + c.turn * G;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-          if (s + j < s_end) b[j][q] = load_scales(row[q], p.sf_pitch, width, s + j);
+        for (int q = 0; q < 4; ++q)
+          fetch_scales(place + (slot * 4 + q) * 512, row[q], sf, p.sf_pitch, width, c.slice);
       }
-      advance(c);
+      asm volatile("cp.async.commit_group;" ::: "memory");   // empty behind the last tile
     };
     uint32_t stage = 0, phase = 0;
+    Cursor in = {first, s_begin}, out = in;
+    for (int j = 0; j < C::kStages; ++j, next(in)) fetch(in, j);
     bool ok = true;
-    auto skip = [&](int n) {                        // n stages on
-      stage += n;
-      while (stage >= (uint32_t)C::kStages) { stage -= C::kStages; phase ^= 1u; }
-    };
-    Cursor out = {first, 0};                        // the turn whose stage `stage` is
-    auto store = [&](const Cursor& c, const uint4 (&b)[G][4]) {
-      // Stages of the turns in between belong to the other warps.
-      while (out.tile != c.tile || out.turn != c.turn) {
-        skip(min(G, per_tile - out.turn * G));
-        if (++out.turn == turns) { out.turn = 0; out.tile += stride; }
-      }
-      const int n = min(G, per_tile - c.turn * G);
-      uint32_t st = stage, ph = phase;
+    while (out.tile < tiles) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+      uint4 b[4];
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        if (j < n) {
-          if (!wait_warp(empty(st), ph ^ 1u, abort_flag, kErrTimeoutProducer)) {
-            ok = false;
-            return;
-          }
-          const uint32_t dst = ring + st * C::kStageBytes + C::kBytesF + C::kBytesT +
-                               part * kSteps * kAtomBytes + lane * 16;
-          sts128(dst, b[j][0].x, b[j][1].x, b[j][2].x, b[j][3].x);
-          sts128(dst + kAtomBytes, b[j][0].y, b[j][1].y, b[j][2].y, b[j][3].y);
-          sts128(dst + 2 * kAtomBytes, b[j][0].z, b[j][1].z, b[j][2].z, b[j][3].z);
-          sts128(dst + 3 * kAtomBytes, b[j][0].w, b[j][1].w, b[j][2].w, b[j][3].w);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full(st));
-          if (++st == (uint32_t)C::kStages) { st = 0; ph ^= 1u; }
-        }
-      }
-    };
-    Cursor in = {first, turn0 - W};                 // the next turn to load
-    advance(in);
-    Cursor done = in;                               // the next turn to store
-#pragma unroll
-    for (int j = 0; j < D; ++j) load(in, buf[j]);
-    while (done.tile < tiles && ok) {
-#pragma unroll
-      for (int u = 0; u <= D; ++u) {
-        if (done.tile < tiles && ok) {
-          load(in, buf[(u + D) % (D + 1)]);
-          store(done, buf[u]);
-          advance(done);
-        }
-      }
+      for (int q = 0; q < 4; ++q) b[q] = lds128(place + (stage * 4 + q) * 512);
+      fetch(in, stage);
+      next(in);
+      ok = wait_warp(empty(stage), phase ^ 1u, abort_flag, kErrTimeoutProducer);
+      if (!ok) break;
+      const uint32_t dst = ring + stage * C::kStageBytes + C::kBytesF + C::kBytesT +
+                           part * kSteps * kAtomBytes + lane * 16;
+      sts128(dst, b[0].x, b[1].x, b[2].x, b[3].x);
+      sts128(dst + kAtomBytes, b[0].y, b[1].y, b[2].y, b[3].y);
+      sts128(dst + 2 * kAtomBytes, b[0].z, b[1].z, b[2].z, b[3].z);
+      sts128(dst + 3 * kAtomBytes, b[0].w, b[1].w, b[2].w, b[3].w);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(stage));
+      next(out);
+      if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
   } else {
     // ------------------------------- epilogue -------------------------------
@@ -460,12 +455,24 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
         const int step = 2 * (int)split;
         const int have = min(TN, p.m - tt * TN);
         for (int c = c0; c < have; c += 4 * step) {
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (uint32_t r = 0; r < split; ++r) {
-            const uint32_t src = map_rank(ring + (uint32_t)(c * kTileF + l) * 4, r);
+          // All loads first: a remote one takes as long as several hundred adds.
+          float w[kMaxSplit][4], v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxSplit; ++r) {
+            if (r < split) {
+              const uint32_t src = map_rank(ring + (uint32_t)(c * kTileF + l) * 4, r);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[r][j] = c + j * step < have
+                              ? ld_cluster_f32(src + (uint32_t)(j * step * kTileF) * 4)
+                              : 0.0f;
+            }
+          }
+#pragma unroll
+          for (uint32_t r = 0; r < kMaxSplit; ++r) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (c + j * step < have) v[j] += ld_cluster_f32(src + (uint32_t)(j * step * kTileF) * 4);
+              if (r < split) v[j] += w[r][j];
           }
           finish<T, DACT, 4>(p, o, v, f, tt * TN + c, step, (have - c + step - 1) / step);
         }
@@ -576,12 +583,14 @@ Plan make_plan(int64_t m, int64_t n, int64_t k) {
   p.tiles_f = (n + kTileF - 1) / kTileF;
   p.tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   p.tiles_t = 1;
-  // Split k while the tiles leave CTA slots empty and every part keeps at
-  // least two slices.
-  const int64_t slots = (p.tn < 128 ? 2 : 1) * kSms;
-  int64_t s = slots / p.tiles_f;
-  if (s > slices / 2) s = slices / 2;
-  p.split = (int)(s < 1 ? 1 : s > kMaxSplit ? kMaxSplit : s);
+  // Split k while all clusters run at once and every part keeps at least two
+  // slices.  A cluster lives within one GPC: 148 SMs are counted as nine of 16.
+  // (5120 x 5120, one token: 10.9 us whole, 8.9 in four parts, 8.5 in six; in
+  // seven, whose clusters take two waves, 13.4.)
+  const int ctas = p.tn < 128 ? 2 : 1;
+  p.split = 1;
+  for (int s = 2; s <= kMaxSplit && 2 * s <= slices; ++s)
+    if (p.tiles_f <= 9 * (16 * ctas / s)) p.split = s;
   return p;
 }
 
@@ -609,22 +618,19 @@ int launch_tile(const Plan& plan, const Params& p, const CUtensorMap& f, const C
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)plan.split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  auto go = [&](auto kernel) {
-    if (cudaError_t e = cudaFuncSetAttribute(
-            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes))
-      return cuda_status(e);
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, f, t, p)) return cuda_status(e);
-    return cuda_status(cudaGetLastError());
-  };
   if (plan.split > 1) {
+    constexpr auto kernel = k_gemm<TN, T, DACT, true>;
+    if (int e = allow_smem<kernel>((int)C::kSmemBytes)) return e;
     cfg.gridDim = dim3((unsigned)(tiles * plan.split));
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return go(k_gemm<TN, T, DACT, true>);
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, f, t, p));
   }
+  constexpr auto kernel = k_gemm<TN, T, DACT, false>;
+  if (int e = allow_smem<kernel>((int)C::kSmemBytes)) return e;
   const int64_t slots = (int64_t)sms * C::kCtasPerSm;
   cfg.gridDim = dim3((unsigned)(tiles < slots ? tiles : slots));
-  return go(k_gemm<TN, T, DACT, false>);
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, f, t, p));
 }
 
 template <typename T, bool DACT>

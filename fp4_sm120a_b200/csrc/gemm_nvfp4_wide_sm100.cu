@@ -567,10 +567,8 @@ __global__ void __launch_bounds__(256) k_order_scales(const OrderArgs a) {
 template <int TN, typename T, bool DACT>
 int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
   using C = Wide<TN>;
-  auto kernel = k_gemm_pair<TN, T, DACT>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)C::kSmemBytes))
-    return cuda_status(e);
+  constexpr auto kernel = k_gemm_pair<TN, T, DACT>;
+  if (int e = allow_smem<kernel>((int)C::kSmemBytes)) return e;
   const int64_t tiles = (int64_t)p.tiles_f * p.tiles_t;
   const int64_t pairs = sms / 2 > 0 ? sms / 2 : 1;
   cudaLaunchConfig_t cfg = {};

@@ -2,6 +2,7 @@
 // properties.
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -21,5 +22,21 @@ int device_sm_count(int* sms);
 // source files, for nvfp4_device_error.  The device is already synchronized.
 int gemm_device_error(uint32_t* code, int clear);
 int layernorm_device_error(uint32_t* code, int clear);
+
+// Allows KERNEL `bytes` of dynamic shared memory, once a device (asking again
+// for every launch costs about as much as the launch).
+template <auto KERNEL>
+int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done;
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return cuda_status(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return NVFP4_OK;
+  if (cudaError_t e =
+          cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+    return cuda_status(e);
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return NVFP4_OK;
+}
 
 }  // namespace nvfp4

@@ -712,21 +712,11 @@ __global__ void __launch_bounds__(32 * kReduceWarps) k_bwd_reduce(const float* p
 int row_threads(int64_t n, int items) { return (int)(((n + items - 1) / items + 31) / 32 * 32); }
 
 // Blocks of `kernel` that an SM's registers and threads take, before shared
-// memory (kept: the query costs more than a launch).  Also allows the kernel
-// all of an SM's shared memory, once a device.
+// memory (kept: the query costs more than a launch).
 template <auto KERNEL>
 int blocks_of(int threads, int* blocks) {
   static std::atomic<int> kept[33];
-  static std::atomic<uint64_t> allowed;
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return cuda_status(e);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev > 63 || !(allowed.load(std::memory_order_acquire) & bit)) {
-    if (cudaError_t e = cudaFuncSetAttribute(
-            KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingMost))
-      return cuda_status(e);
-    allowed.fetch_or(bit, std::memory_order_release);
-  }
+  if (int e = allow_smem<KERNEL>((int)kRingMost)) return e;
   int n = kept[threads / 32].load(std::memory_order_relaxed);
   if (n == 0) {
     if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0))

@@ -8,83 +8,91 @@ ValueError here or NVFP4Error from the library.  The pointer-level forms, with
 explicit streams and workspaces, are in ops."""
 from __future__ import annotations
 
-import ctypes
-import functools
 from typing import Optional, Sequence
 
 import torch
 
 from . import ops
-from ._native import AdamWTensor
+from ._native import AdamWTensor, check, load
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32 = torch.float32
 STATE_BLOCK = 128   # elements that share one scale byte of an 8-bit state
 
-
-def _on_device_of_first(fn):
-    """Runs fn with the device of its first argument current (its streams and
-    allocations follow)."""
-    @functools.wraps(fn)
-    def run(x, *args, **kw):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            raise ValueError("expected a CUDA tensor")
-        if x.device.index == torch.cuda.current_device():
-            return fn(x, *args, **kw)
-        with torch.cuda.device(x.device):
-            return fn(x, *args, **kw)
-    return run
+# A small product or norm takes a few microseconds on the device, so these
+# wrappers look at each tensor once and call the library without the layers of
+# the pointer-level forms; the stream is asked for as an address (a Stream
+# object costs more than a launch).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _same_device(x: torch.Tensor, *others) -> None:
-    for t in others:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors on {x.device} and {t.device}")
+def _device(x) -> int:
+    """Index of a CUDA tensor's device."""
+    d = x.get_device() if isinstance(x, torch.Tensor) else -1
+    if d < 0:
+        raise ValueError("expected a CUDA tensor")
+    return d
 
 
-def _rows(t: torch.Tensor, shape, dtype, name: str) -> int:
-    """Row stride of a 2-D tensor with unit inner stride."""
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{name}: expected {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+def _call(device: int, name: str, *args) -> None:
+    """A library call on the device's current stream (the last argument of every
+    entry point)."""
+    fn = getattr(load(), name)
+    if device == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(device))
+    if status:
+        check(name, status)
+
+
+def _rows(t: torch.Tensor, m: int, n: int, dtype, device: int, name: str) -> int:
+    """Row stride of an m x n tensor with unit inner stride."""
+    if t.dtype != dtype or t.dim() != 2 or tuple(t.shape) != (m, n):
+        raise ValueError(f"{name}: expected {(m, n)} {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: not on cuda:{device}")
+    if t.is_contiguous():
+        return n
+    if n > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the inner stride must be 1")
     # A single row has no row stride to speak of.
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if m > 1 else max(t.stride(0), n)
 
 
-def _vector(t: torch.Tensor, n: int, name: str, dtypes=None) -> None:
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {n} contiguous values, got {tuple(t.shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise ValueError(f"{name}: unexpected type {t.dtype}")
+def _vector(t: torch.Tensor, n: int, device: int, name: str) -> int:
+    """Address of n contiguous values."""
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name}: expected {n} contiguous values on cuda:{device}, got "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _word(t: Optional[torch.Tensor], name: str, n: int = 1) -> None:
-    if t is not None and (t.numel() != n or t.dtype != torch.float32 or not t.is_contiguous()):
-        raise ValueError(f"{name}: expected {n} float32")
+def _words(t: Optional[torch.Tensor], n: int, device: int, name: str) -> Optional[int]:
+    """Address of n float32 on the device, or None."""
+    if t is None:
+        return None
+    if t.numel() != n or t.dtype != _F32 or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name}: expected {n} float32 on cuda:{device}")
+    return t.data_ptr()
 
 
-def _operand(codes: torch.Tensor, scales: torch.Tensor, amax: torch.Tensor, name: str):
-    if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
-        raise ValueError(f"{name}: codes are a contiguous 2-D uint8 tensor")
+def _operand(codes: torch.Tensor, scales: torch.Tensor, amax: torch.Tensor, device: int,
+             name: str):
+    if (codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous()
+            or codes.get_device() != device):
+        raise ValueError(f"{name}: codes are a contiguous 2-D uint8 tensor on cuda:{device}")
     rows, half = codes.shape
     if half % 16:
         raise ValueError(f"{name}: k must be a multiple of 32, got {2 * half}")
-    if scales.shape != (rows, half // 8) or scales.element_size() != 1 or not scales.is_contiguous():
-        raise ValueError(f"{name}: scales are contiguous bytes of shape {(rows, half // 8)}")
-    _word(amax, f"{name}: amax")
-    return rows, 2 * half
+    if (scales.element_size() != 1 or tuple(scales.shape) != (rows, half // 8)
+            or not scales.is_contiguous() or scales.get_device() != device):
+        raise ValueError(f"{name}: scales are contiguous bytes of shape {(rows, half // 8)} "
+                         f"on cuda:{device}")
+    return rows, 2 * half, _words(amax, 1, device, f"{name}: amax")
 
 
-def _operands(a, a_scales, a_amax, b, b_scales, b_amax):
-    _same_device(a, a_scales, a_amax, b, b_scales, b_amax)
-    m, k = _operand(a, a_scales, a_amax, "a")
-    n, kb = _operand(b, b_scales, b_amax, "b")
-    if k != kb:
-        raise ValueError(f"a and b differ in k: {k} and {kb}")
-    return m, n, k
-
-
-@_on_device_of_first
 def matmul_nvfp4(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Tensor, b: torch.Tensor,
                  b_scales: torch.Tensor, b_amax: torch.Tensor, *,
                  bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -96,103 +104,128 @@ def matmul_nvfp4(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Tensor, 
     aux or None); aux is the activation's argument, for matmul_nvfp4_dact.
     `out` (may be `residual`) receives D in place of a new tensor; `amax_out`
     (one float32) receives max |D|."""
-    m, n, k = _operands(a, a_scales, a_amax, b, b_scales, b_amax)
-    _same_device(a, bias, residual, out, amax_out)
+    device = _device(a)
+    m, k, pa = _operand(a, a_scales, a_amax, device, "a")
+    n, kb, pb = _operand(b, b_scales, b_amax, device, "b")
+    if k != kb:
+        raise ValueError(f"a and b differ in k: {k} and {kb}")
+    act = ops._activation(activation)
     if out is None:
-        if out_dtype not in _DTYPES:
+        code = _DTYPES.get(out_dtype)
+        if code is None:
             raise ValueError(f"unexpected out_dtype {out_dtype}")
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        out = a.new_empty((m, n), dtype=out_dtype)
         ldd = n
     else:
-        if out.dtype not in _DTYPES:
-            raise ValueError(f"out: unexpected type {out.dtype}")
-        ldd = _rows(out, (m, n), out.dtype, "out")
+        out_dtype = out.dtype
+        code = _DTYPES.get(out_dtype)
+        if code is None:
+            raise ValueError(f"out: unexpected type {out_dtype}")
+        ldd = _rows(out, m, n, out_dtype, device, "out")
+    bias_ptr, bias_code = None, 0
     if bias is not None:
-        _vector(bias, n, "bias", _DTYPES)
-    ldr = n if residual is None else _rows(residual, (m, n), out.dtype, "residual")
-    _word(amax_out, "amax_out")
-    aux = torch.empty((m, n), dtype=out.dtype, device=a.device) if with_aux else None
-    nbytes = ops.gemm_nvfp4_workspace_bytes(m, n, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    ops.gemm_nvfp4(m, n, k, a, a_scales, a_amax, b, b_scales, b_amax, out, ldd, out.dtype, bias,
-                   torch.float32 if bias is None else bias.dtype, residual, ldr, activation, aux,
-                   n, amax_out, ws, nbytes)
+        bias_code = _DTYPES.get(bias.dtype)
+        if bias_code is None:
+            raise ValueError(f"bias: unexpected type {bias.dtype}")
+        bias_ptr = _vector(bias, n, device, "bias")
+    res_ptr, ldr = None, n
+    if residual is not None:
+        ldr = _rows(residual, m, n, out_dtype, device, "residual")
+        res_ptr = residual.data_ptr()
+    amax_ptr = _words(amax_out, 1, device, "amax_out")
+    aux = a.new_empty((m, n), dtype=out_dtype) if with_aux else None
+    nbytes = load().nvfp4_gemm_workspace_bytes(m, n, k)
+    ws = a.new_empty(nbytes) if nbytes else None
+    _call(device, "nvfp4_gemm", m, n, k, a.data_ptr(), a_scales.data_ptr(), pa, b.data_ptr(),
+          b_scales.data_ptr(), pb, out.data_ptr(), ldd, code, bias_ptr, bias_code, res_ptr, ldr,
+          act, aux.data_ptr() if with_aux else None, n, amax_ptr,
+          ws.data_ptr() if nbytes else None, nbytes, 0)
     return out, aux
 
 
-@_on_device_of_first
 def matmul_nvfp4_dact(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Tensor,
                       b: torch.Tensor, b_scales: torch.Tensor, b_amax: torch.Tensor,
                       aux: torch.Tensor, *, activation: str, with_dbias: bool = False,
                       amax_out: Optional[torch.Tensor] = None):
     """(A B^T) act'(aux), of aux's type, and its column sums in fp32 (the bias
     gradient) or None."""
-    m, n, k = _operands(a, a_scales, a_amax, b, b_scales, b_amax)
-    _same_device(a, aux, amax_out)
-    if aux.dtype not in _DTYPES:
-        raise ValueError(f"aux: unexpected type {aux.dtype}")
-    ldaux = _rows(aux, (m, n), aux.dtype, "aux")
-    _word(amax_out, "amax_out")
-    d = torch.empty((m, n), dtype=aux.dtype, device=a.device)
-    dbias = None
-    if with_dbias:
-        dbias = torch.empty(n, dtype=torch.float32, device=a.device)
-        nbytes = ops.gemm_nvfp4_dact_workspace_bytes(m, n, k)
-    else:
-        nbytes = ops.gemm_nvfp4_workspace_bytes(m, n, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    ops.gemm_nvfp4_dact(m, n, k, a, a_scales, a_amax, b, b_scales, b_amax, aux, ldaux, activation,
-                        d, n, d.dtype, dbias, amax_out, ws, nbytes)
+    device = _device(a)
+    m, k, pa = _operand(a, a_scales, a_amax, device, "a")
+    n, kb, pb = _operand(b, b_scales, b_amax, device, "b")
+    if k != kb:
+        raise ValueError(f"a and b differ in k: {k} and {kb}")
+    act = ops._activation(activation)
+    dtype = aux.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"aux: unexpected type {dtype}")
+    ldaux = _rows(aux, m, n, dtype, device, "aux")
+    amax_ptr = _words(amax_out, 1, device, "amax_out")
+    d = a.new_empty((m, n), dtype=dtype)
+    dbias = a.new_empty(n, dtype=_F32) if with_dbias else None
+    lib = load()
+    nbytes = (lib.nvfp4_gemm_dact_workspace_bytes if with_dbias
+              else lib.nvfp4_gemm_workspace_bytes)(m, n, k)
+    ws = a.new_empty(nbytes) if nbytes else None
+    _call(device, "nvfp4_gemm_dact", m, n, k, a.data_ptr(), a_scales.data_ptr(), pa, b.data_ptr(),
+          b_scales.data_ptr(), pb, aux.data_ptr(), ldaux, act, d.data_ptr(), n, code,
+          dbias.data_ptr() if with_dbias else None, amax_ptr, ws.data_ptr() if nbytes else None,
+          nbytes, 0)
     return d, dbias
 
 
-def _norm_shapes(x: torch.Tensor, gamma: torch.Tensor):
-    if x.dim() != 2 or x.dtype not in _DTYPES:
+def _norm(x: torch.Tensor, gamma: torch.Tensor, device: int):
+    """(rows, cols, codes of both types, row stride, address of gamma)."""
+    dtype = x.dtype
+    code, weight = _DTYPES.get(dtype), _DTYPES.get(gamma.dtype)
+    if x.dim() != 2 or code is None:
         raise ValueError("x: expected a 2-D float32, bfloat16 or float16 tensor")
+    if weight is None or weight not in (0, code):
+        raise ValueError(f"gamma: expected {dtype} or float32, got {gamma.dtype}")
     rows, cols = x.shape
-    _vector(gamma, cols, "gamma", (x.dtype, torch.float32))
-    return rows, cols
+    return rows, cols, code, weight, _rows(x, rows, cols, dtype, device, "x"), _vector(
+        gamma, cols, device, "gamma")
 
 
-@_on_device_of_first
 def layernorm(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Tensor] = None,
               eps: float = 1e-5, *, amax_out: Optional[torch.Tensor] = None):
     """Layer norm over the last dimension of a 2-D tensor.  Returns (y, mean,
     rstd); `amax_out` (one float32) receives max |y| for the cast of y."""
-    rows, cols = _norm_shapes(x, gamma)
-    _same_device(x, gamma, beta, amax_out)
-    ldx = _rows(x, x.shape, x.dtype, "x")
+    device = _device(x)
+    rows, cols, code, weight, ldx, gamma_ptr = _norm(x, gamma, device)
+    beta_ptr = None
     if beta is not None:
-        _vector(beta, cols, "beta", (gamma.dtype,))
-    _word(amax_out, "amax_out")
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    ops.layernorm_fwd(rows, cols, x, ldx, gamma, beta, x.dtype, gamma.dtype, eps, y, cols, mean,
-                      rstd, amax_out)
+        if beta.dtype != gamma.dtype:
+            raise ValueError(f"beta: expected {gamma.dtype}, got {beta.dtype}")
+        beta_ptr = _vector(beta, cols, device, "beta")
+    amax_ptr = _words(amax_out, 1, device, "amax_out")
+    y = x.new_empty((rows, cols))
+    mean, rstd = x.new_empty(rows, dtype=_F32), x.new_empty(rows, dtype=_F32)
+    _call(device, "nvfp4_layernorm_fwd", rows, cols, x.data_ptr(), ldx, gamma_ptr, beta_ptr, code,
+          weight, eps, y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr(), amax_ptr)
     return y, mean, rstd
 
 
-@_on_device_of_first
 def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
                        gamma: torch.Tensor, *, residual: Optional[torch.Tensor] = None):
     """Gradients (dx, dgamma, dbeta) of layernorm; `residual` is added to dx
     (the gradient that reaches x past the norm).  dgamma and dbeta have
     gamma's type."""
-    rows, cols = _norm_shapes(x, gamma)
-    _same_device(x, dy, mean, rstd, gamma, residual)
-    ldx = _rows(x, x.shape, x.dtype, "x")
-    lddy = _rows(dy, x.shape, x.dtype, "dy")
-    ldr = cols if residual is None else _rows(residual, x.shape, x.dtype, "residual")
-    _vector(mean, rows, "mean", (torch.float32,))
-    _vector(rstd, rows, "rstd", (torch.float32,))
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    grads = torch.empty((2, cols), dtype=gamma.dtype, device=x.device)
-    dgamma, dbeta = grads[0], grads[1]
-    nbytes = ops.layernorm_bwd_workspace_bytes(rows, cols)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    ops.layernorm_bwd(rows, cols, dy, lddy, x, ldx, mean, rstd, gamma, residual, ldr, x.dtype,
-                      gamma.dtype, dx, cols, dgamma, dbeta, ws, nbytes)
+    device = _device(x)
+    rows, cols, code, weight, ldx, gamma_ptr = _norm(x, gamma, device)
+    lddy = _rows(dy, rows, cols, x.dtype, device, "dy")
+    res_ptr, ldr = None, cols
+    if residual is not None:
+        ldr = _rows(residual, rows, cols, x.dtype, device, "residual")
+        res_ptr = residual.data_ptr()
+    mean_ptr, rstd_ptr = _words(mean, rows, device, "mean"), _words(rstd, rows, device, "rstd")
+    dx = x.new_empty((rows, cols))
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    nbytes = load().nvfp4_layernorm_bwd_workspace_bytes(rows, cols)
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _call(device, "nvfp4_layernorm_bwd", rows, cols, dy.data_ptr(), lddy, x.data_ptr(), ldx,
+          mean_ptr, rstd_ptr, gamma_ptr, res_ptr, ldr, code, weight, dx.data_ptr(), cols,
+          dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), nbytes)
     return dx, dgamma, dbeta
 
 
@@ -241,9 +274,8 @@ class AdamW:
         if rng_state is not None and (rng_state.numel() != 2 or rng_state.dtype != torch.int64
                                       or rng_state.device != self.device):
             raise ValueError("rng_state: expected int64 {seed, offset} on the parameters' device")
-        _word(amax_out, "amax_out", count)
-        if amax_out is not None and amax_out.device != self.device:
-            raise ValueError("amax_out: not on the parameters' device")
+        self._device = _device(params[0])
+        amax_ptr = _words(amax_out, count, self._device, "amax_out")
         state = torch.uint8 if self.eight else torch.float32
 
         def take(seq, i, n, dtype, name):
@@ -276,7 +308,10 @@ class AdamW:
             d.offset = at if offsets is None else int(offsets[i])
             at += -(-n // STATE_BLOCK) * STATE_BLOCK
             d.weight_decay = 0.0 if weight_decays is None else float(weight_decays[i])
-        self.count, self.amax_out, self.rng_state = count, amax_out, rng_state
+        self.count = count
+        self._fixed = (self._table, count, _DTYPES[self.param_dtype], _DTYPES[self.grad_dtype],
+                       int(self.eight))
+        self._words = (amax_ptr, None if rng_state is None else rng_state.data_ptr())
 
     def step(self, step: int, *, lr: float, beta1: float = 0.9, beta2: float = 0.95,
              eps: float = 1e-8, grad_scale: Optional[torch.Tensor] = None,
@@ -285,30 +320,29 @@ class AdamW:
         (one float32 on the device) multiplies the gradients; scalars (three
         float32 on the device: lr, 1 - beta1^step, 1 - beta2^step) take the
         place of lr and step in a captured step."""
-        for name, t, n in (("grad_scale", grad_scale, 1), ("scalars", scalars, 3)):
-            _word(t, name, n)
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{name}: not on {self.device}")
-        with torch.cuda.device(self.device):
-            ops.adamw_step(self._table, self.count, self.param_dtype, self.grad_dtype,
-                           int(self.eight), lr, beta1, beta2, eps, step, grad_scale, scalars,
-                           self.amax_out, self.rng_state)
+        d = self._device
+        _call(d, "nvfp4_adamw_step", *self._fixed, lr, beta1, beta2, eps, step,
+              _words(grad_scale, 1, d, "grad_scale"), _words(scalars, 3, d, "scalars"),
+              *self._words)
 
 
-@_on_device_of_first
 def adamw_unpack_state(codes: torch.Tensor, scales: torch.Tensor, moment: str,
                        out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of an 8-bit moment ("exp_avg" or "exp_avg_sq"), for a
     checkpoint in floating point or for inspection."""
+    device = _device(codes)
     n = codes.numel()
-    _same_device(codes, scales)
     if codes.dtype != torch.uint8 or not codes.is_contiguous():
         raise ValueError("codes: expected contiguous uint8")
     if (scales.dtype != torch.uint8 or not scales.is_contiguous()
-            or scales.numel() != -(-n // STATE_BLOCK)):
-        raise ValueError(f"scales: expected {-(-n // STATE_BLOCK)} contiguous uint8")
-    if out_dtype not in (torch.float32, torch.bfloat16):
+            or scales.numel() != -(-n // STATE_BLOCK) or scales.get_device() != device):
+        raise ValueError(f"scales: expected {-(-n // STATE_BLOCK)} contiguous uint8 on "
+                         f"cuda:{device}")
+    if out_dtype not in (_F32, torch.bfloat16):
         raise ValueError(f"unexpected out_dtype {out_dtype}")
-    out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
-    ops.adamw_unpack_state(codes, scales, n, moment, out, out_dtype)
+    if moment not in ops.MOMENTS:
+        raise ValueError(f"unknown moment {moment!r}: one of {', '.join(ops.MOMENTS)}")
+    out = codes.new_empty(codes.shape, dtype=out_dtype)
+    _call(device, "nvfp4_adamw_unpack_state", codes.data_ptr(), scales.data_ptr(), n,
+          ops.MOMENTS[moment], out.data_ptr(), _DTYPES[out_dtype])
     return out
