@@ -286,6 +286,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_st,
                 const Params p) {
   using C = Wide<TN>;
+  // k_dbias may be scheduled; it waits for this kernel to complete.
+  asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_holder;
@@ -343,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t stage = 0, phase = 0;
     bool ok = true;
     const uint32_t first_full = map_rank(full(0), 0);     // the first CTA's barriers
-    grid_dependency_wait();     // the scales in their order
+    grid_dependency_wait();     // the scales in their order, the amax cleared
     for (int i = first; i < tiles && ok; i += stride) {
       int tf, tt;
       tile_at(p, i, tf, tt);
@@ -530,10 +532,12 @@ struct OrderArgs {
   int rows[2], width[2];
   int blocks0;          // row blocks of operand 0
   int pitch, slices;
+  uint32_t* amax;       // cleared for the product's epilogue, may be null
 };
 
 __global__ void __launch_bounds__(256) k_order_scales(const OrderArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
+  if (a.amax && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.amax = 0u;
   __shared__ uint32_t tile[128][33];                     // 8 slices x 4 words, padded
   const int which = (int)blockIdx.y >= a.blocks0;
   const int block = (int)blockIdx.y - (which ? a.blocks0 : 0);
@@ -628,6 +632,7 @@ int launch_wide(int dtype, bool dact, int tn, const Params& p, const void* a, co
   o.width[0] = p.sf_width_f;
   o.width[1] = p.sf_width_t;
   o.blocks0 = (int)row_blocks(p.n);
+  o.amax = p.amax;
   const int64_t blocks = row_blocks(p.n) + row_blocks(p.m);
   const dim3 grid((unsigned)((p.slices + 7) / 8), (unsigned)blocks);
   k_order_scales<<<grid, 256, 0, st>>>(o);

@@ -51,6 +51,13 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
   return x;
 }
+// The sum over 16 lanes (a half warp each), for the joint of at most 16 warps.
+template <int WARPS>
+__device__ __forceinline__ float join_sum(float x) {
+#pragma unroll
+  for (int o = WARPS > 16 ? 16 : 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  return x;
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
@@ -335,12 +342,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
     fetch_weights<T, W, ALIGNED, ITEMS>(wb, a.cols, beta);
   }
   __syncthreads();
-  // Elements that warp `lane` holds of a row (0 for lanes without a warp).
+  // The warp whose sums this lane joins, and the elements it holds of a row
+  // (0 for lanes without a warp).
+  const int share = THREADS > 512 ? lane : lane & 15;
   float nw = 0.0f;
-  if (lane < nwarps) {
+  if (share < nwarps) {
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it)
-      nw += (float)(min(max(nvec - lane * 32 - it * nthr, 0), 32) * VEC);
+      nw += (float)(min(max(nvec - share * 32 - it * nthr, 0), 32) * VEC);
   }
   const float own = __shfl_sync(0xFFFFFFFFu, nw, warp);
   const float inv_own = own > 0.0f ? 1.0f / own : 0.0f;
@@ -360,12 +369,25 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
       const float mw = warp_sum(sum2(s)) * inv_own;
       const uint64_t minus = pair(-mw, -mw);
       s = pair(0.0f, 0.0f);
+      if constexpr (ALIGNED) {
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        // What lies behind the row's end counts as the mean.
-        const float u = my.has(e / VEC) ? f[e] : mw, v = my.has((e + 1) / VEC) ? f[e + 1] : mw;
-        const uint64_t d = add2(pair(u, v), minus);
-        s = fma2(d, d, s);
+        for (int it = 0; it < ITEMS; ++it) {
+          if (my.has(it)) {
+#pragma unroll
+            for (int e = it * VEC; e < (it + 1) * VEC; e += 2) {
+              const uint64_t d = add2(pair(f[e], f[e + 1]), minus);
+              s = fma2(d, d, s);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          // What lies behind the row's end counts as the mean.
+          const float u = my.has(e) ? f[e] : mw, v = my.has(e + 1) ? f[e + 1] : mw;
+          const uint64_t d = add2(pair(u, v), minus);
+          s = fma2(d, d, s);
+        }
       }
       const float q = warp_sum(sum2(s));
       if (lane == 0) sh.red[k & 1][warp] = make_float2(mw, q);
@@ -376,11 +398,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
     __syncthreads();
     if (*(volatile uint32_t*)&sh.abort_flag) break;
     if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
-    // Lane w joins warp w's share; every warp does so by itself.
-    const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
-    const float mean = warp_sum(part.x * (nw * inv_n));
+    // A lane joins one warp's share; every warp does so by itself.
+    const float2 part = share < nwarps ? sh.red[k & 1][share] : make_float2(0.0f, 0.0f);
+    const float mean = join_sum<THREADS / 32>(part.x * (nw * inv_n));
     const float d = part.x - mean;
-    const float rstd = rsqrtf(warp_sum(part.y + nw * d * d) * inv_n + a.eps);
+    const float rstd = rsqrtf(join_sum<THREADS / 32>(part.y + nw * d * d) * inv_n + a.eps);
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -582,8 +604,10 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
     __syncthreads();
     if (*(volatile uint32_t*)&sh.abort_flag) break;
     if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
-    const float2 part = lane < nwarps ? sh.red[k & 1][lane] : make_float2(0.0f, 0.0f);
-    const float c1 = warp_sum(part.x) * inv_n * rstd, c2 = warp_sum(part.y) * inv_n * rstd;
+    const int share = THREADS > 512 ? lane : lane & 15;
+    const float2 part = share < nwarps ? sh.red[k & 1][share] : make_float2(0.0f, 0.0f);
+    const float c1 = join_sum<THREADS / 32>(part.x) * inv_n * rstd;
+    const float c2 = join_sum<THREADS / 32>(part.y) * inv_n * rstd;
     const uint64_t scale = pair(rstd, rstd), n1 = pair(-c1, -c1), n2 = pair(-c2, -c2);
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
