@@ -95,8 +95,11 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// Tells another CTA that TMEM reads are done (they are: tcgen05.wait::ld).  No
+// memory is handed over, so nothing has to wait for this thread's stores, as a
+// release would.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
 }
 __device__ __forceinline__ void grid_dependency_wait() {
@@ -166,11 +169,12 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
 struct Acc {
   float alpha;
   float bias[8], dbias[8];
-  uint32_t top;
+  uint32_t top, some;   // maximum over whole vectors (packed) and the others (fp32 bits)
   int f;
 };
 
-// One token's eight features: x holds the accumulators.
+// One token's eight features, all of them in D and in whole vectors: x holds
+// the accumulators.
 template <typename T, bool DACT, int ACT>
 __device__ __forceinline__ void finish8(const Params& p, Acc& o, float (&x)[8], const Raw8<T>& r,
                                         int64_t t) {
@@ -188,14 +192,7 @@ __device__ __forceinline__ void finish8(const Params& p, Acc& o, float (&x)[8], 
     for (int j = 0; j < 8; ++j) x[j] = x[j] * o.alpha + o.bias[j];
     if (p.aux) {
       w.set(x);
-      T* a = reinterpret_cast<T*>(p.aux) + t * p.ldaux + o.f;
-      if (p.vec && o.f + 8 <= p.n) {
-        w.store(a);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (o.f + j < p.n) a[j] = from_f32<T>(x[j]);
-      }
+      w.store(reinterpret_cast<T*>(p.aux) + t * p.ldaux + o.f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = activate<ACT>(x[j]);
@@ -204,21 +201,48 @@ __device__ __forceinline__ void finish8(const Params& p, Acc& o, float (&x)[8], 
       for (int j = 0; j < 8; ++j) x[j] += e[j];
     }
   }
-  T* d = reinterpret_cast<T*>(p.d) + t * p.ldd + o.f;
-  if (o.f + 8 > p.n) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (o.f + j >= p.n) x[j] = 0.0f;
-  }
   w.set(x);
-  o.top = w.top(o.top);
-  if (p.vec && o.f + 8 <= p.n) {
-    w.store(d);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (o.f + j < p.n) d[j] = from_f32<T>(x[j]);
+  if (p.amax) o.top = w.top(o.top);
+  w.store(reinterpret_cast<T*>(p.d) + t * p.ldd + o.f);
+}
+
+// The same element by element, for the features that exist: ragged borders and
+// unaligned rows.  A function of its own, since the instruction cache holds
+// little more than the loop that calls it.  In: accumulators in x, the scaled
+// bias beside them; out: what D holds (0 outside), for the bias gradient.
+template <typename T, bool DACT>
+__device__ __noinline__ uint32_t finish_some(const Params& p, float alpha, const float* bias,
+                                             float* x, int f, int64_t t) {
+  uint32_t top = 0;
+#pragma unroll 1
+  for (int j = 0; j < 8; ++j) {
+    if (f + j >= p.n) {
+      x[j] = 0.0f;
+      continue;
+    }
+    const float e = DACT || p.res
+                        ? to_f32(reinterpret_cast<const T*>(p.res)[t * p.ldr + f + j])
+                        : 0.0f;
+    float z = x[j] * alpha;
+    if constexpr (DACT) {
+      z *= p.act == kRelu   ? slope<kRelu>(e)
+           : p.act == kGelu ? slope<kGelu>(e)
+           : p.act == kSilu ? slope<kSilu>(e)
+                            : 1.0f;
+    } else {
+      z += bias[j];
+      if (p.aux) reinterpret_cast<T*>(p.aux)[t * p.ldaux + f + j] = from_f32<T>(z);
+      z = (p.act == kRelu   ? activate<kRelu>(z)
+           : p.act == kGelu ? activate<kGelu>(z)
+           : p.act == kSilu ? activate<kSilu>(z)
+                            : z) + e;
+    }
+    const T s = from_f32<T>(z);
+    reinterpret_cast<T*>(p.d)[t * p.ldd + f + j] = s;
+    x[j] = z;
+    top = max(top, __float_as_uint(to_f32(s)) & 0x7FFFFFFFu);
   }
+  return top;
 }
 
 // A warp's chunk: lane l holds feature l's accumulators of the tokens t0 ..
@@ -229,6 +253,7 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
                                              float* turn, int lane, int t0) {
   constexpr int kRows = kTurnRows / 8;         // tokens of a thread at a time
   const T* res = reinterpret_cast<const T*>(p.res);
+  const bool whole = p.vec && o.f + 8 <= p.n;
 #pragma unroll
   for (int h = 0; h < 32; h += kTurnRows) {
     Raw8<T> r[kRows];
@@ -237,17 +262,7 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const int64_t t = t0 + h + row0 + 8 * i;
-        if (t < p.m) {
-          if (p.vec && o.f + 8 <= p.n) {
-            r[i].load(res + t * p.ldr + o.f);
-          } else {
-            float e[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              e[j] = o.f + j < p.n ? to_f32(res[t * p.ldr + o.f + j]) : 0.0f;
-            r[i].set(e);
-          }
-        }
+        if (t < p.m && whole) r[i].load(res + t * p.ldr + o.f);
       }
     }
     __syncwarp();
@@ -268,9 +283,27 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
     auto all = [&](auto act) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
-        if (t0 + h + row0 + 8 * i < p.m && o.f < p.n)
+        if (t0 + h + row0 + 8 * i < p.m)
           finish8<T, DACT, decltype(act)::value>(p, o, x[i], r[i], t0 + h + row0 + 8 * i);
     };
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int64_t t = t0 + h + row0 + 8 * i;
+        if (t < p.m && o.f < p.n) {
+          float y[8], b[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            y[j] = x[i][j];
+            b[j] = o.bias[j];
+          }
+          o.some = max(o.some, finish_some<T, DACT>(p, o.alpha, b, y, o.f, t));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o.dbias[j] += y[j];
+        }
+      }
+      continue;
+    }
     switch (p.act) {
       case kRelu: all(Const<kRelu>()); break;
       case kGelu: all(Const<kGelu>()); break;
@@ -453,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     float* turn = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) +
                                            C::kStages * C::kStageBytes + warp * kTurnWarp);
     Acc o;
-    o.top = 0u;
+    o.top = o.some = 0u;
     {
       const float ea = global_encode_scale(*p.amax_f), eb = global_encode_scale(*p.amax_t);
       o.alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
@@ -506,7 +539,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     if (p.amax) {
-      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, top_bits<T>(o.top));
+      const uint32_t top =
+          __reduce_max_sync(0xFFFFFFFFu, max(top_bits<T>(o.top), o.some));
       if (lane == 0 && top) atomicMax(p.amax, top);
     }
     tc_fence_before();
