@@ -564,7 +564,7 @@ struct Plan {
   bool wide;
   int tn, split;
   int64_t tiles_f, tiles_t;
-  int64_t partial_rows() const { return tiles_t * (wide ? 4 : 2 * split); }
+  int64_t partial_rows() const { return tiles_t * (wide ? 3 : 2 * split); }
 };
 constexpr int kSms = 148;
 

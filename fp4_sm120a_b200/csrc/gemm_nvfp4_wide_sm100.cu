@@ -19,7 +19,7 @@
 // epilogue of a tile takes the shared columns first, and the next tile's
 // products start when these (not the whole accumulator) have been read.
 //
-// Warps: 0-15 epilogue, 16 TMA producer, 17 MMA issuer (of the pair's first
+// Warps: 0-11 epilogue, 12 TMA producer, 13 MMA issuer (of the pair's first
 // CTA).  Epilogue: a warp's 32 lanes (features) x 32 columns (tokens) are turned
 // around through 2 KB of shared memory, after which a thread holds eight
 // consecutive features of a token: bias, activation, residual and the stores
@@ -30,8 +30,9 @@ namespace nvfp4 {
 namespace gemm {
 namespace {
 
-// Sixteen epilogue warps: four column groups of four warps (TMEM lane quarters).
-constexpr int kPairEpiWarps = 16, kGroups = kPairEpiWarps / 4;
+// Twelve epilogue warps: three column groups of four warps (TMEM lane quarters),
+// as many as 128 registers a thread allow.
+constexpr int kPairEpiWarps = 12, kGroups = kPairEpiWarps / 4;
 constexpr int kWarpTma = kPairEpiWarps, kWarpMma = kPairEpiWarps + 1;
 constexpr int kThreads = 32 * (kPairEpiWarps + 2);
 constexpr int kTurnRows = 16;                                // tokens turned around at once
@@ -53,13 +54,13 @@ struct Wide {
   static constexpr int kOverlap = 2 * TN > kFree ? 2 * TN - kFree : 0;
   static constexpr int kAcc1 = TN - kOverlap;                // second accumulator's first column
   static constexpr int kChunks = TN / 32;
-  static constexpr int kTurns = kChunks / kGroups;           // per column group
+  static constexpr int kTurns = (kChunks + kGroups - 1) / kGroups;   // per column group
   // Turns whose columns the next tile's products overwrite.
   static constexpr int kEarly = (kOverlap + 32 * kGroups - 1) / (32 * kGroups);
   static constexpr uint32_t kIdesc =
       (1u << 7) | (1u << 10) | ((uint32_t)(TN / 8) << 17) | ((uint32_t)(256 / 16) << 24);
   static_assert(kStages >= 3, "the scale columns of slice g - 2 are checked through its stage");
-  static_assert(kEarly <= 1 && kTurns >= 1, "columns held in registers");
+  static_assert(kEarly <= 1, "columns held in registers");
 };
 
 // TMA load by a CTA of a pair into its own shared memory, completing on the
@@ -516,14 +517,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       constexpr int kLast = C::kEarly > 0 ? C::kEarly - 1 : C::kTurns - 1;
 #pragma unroll 1
       for (int u = 0; u < C::kTurns; ++u) {
+        const bool have = kGroups * u + group < C::kChunks;
         float v[32];
-        tmem_ld_32cols(src + 32 * chunk(u), v);
-        tc_wait_ld();
+        if (have) {
+          tmem_ld_32cols(src + 32 * chunk(u), v);
+          tc_wait_ld();
+        }
         if (u == kLast) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_cluster(map_rank(acc_free(a), 0));
         }
+        if (!have) break;
         finish_chunk<T, DACT>(p, o, v, turn, lane, tt * TN + 32 * chunk(u));
       }
       if (DACT && p.dbias_partial) {
