@@ -80,7 +80,7 @@ def check_backward(nvlib, x, gamma, dy, res, mean, rstd, dev=None):
     close(db, wdb, (rows + 64) * 2.0 ** -24 * t + hw * wdb.abs() + sub, "dbeta")
 
 
-SHAPES = [(1, 1), (1, 8), (3, 7), (2, 16), (5, 64), (17, 129), (4, 256), (33, 1000), (7, 1024),
+SHAPES = [(1200, 8192), (1190, 1024), (3000, 4096), (2000, 40), (1, 1), (1, 8), (3, 7), (2, 16), (5, 64), (17, 129), (4, 256), (33, 1000), (7, 1024),
           (300, 520), (9, 4099), (2, 5120), (400, 2048), (3, 8192), (2, 8200), (2, 12288),
           (2, 16384), (3, 16392), (1, 16411), (2, 40000), (1200, 24)]
 
