@@ -18,8 +18,8 @@
 // thread, a warp's stores cover 32 consecutive elements of a row of D, and a
 // column sum of D (the bias gradient) never leaves a thread.
 //
-// m > 128 takes the kernel in gemm_nvfp4_wide_sm100.cu.  Here: output tiles of
-// 128 (n) x TN (m <= TN), warp-specialised:
+// Products of many tiles take the kernel in gemm_nvfp4_wide_sm100.cu.  Here:
+// output tiles of 128 (n) x TN (m), warp-specialised:
 //   warps 0-7   epilogue: two groups of four warps, each half of the columns
 //   warp  8     TMA producer: 128-byte k-slices (256 codes) of both operands
 //               into a ring of 128-byte-swizzled stages
@@ -55,10 +55,9 @@ struct Tile {
   static constexpr uint32_t kBytesSf = kSteps * 2 * kAtomBytes;
   static constexpr uint32_t kStageBytes = kBytesF + kBytesT + kBytesSf;
   static constexpr uint32_t kPlaceBytes = 2 * 128 * 16;      // scales in flight, a stage
-  // TN = 128: one CTA per SM with all of its shared memory.  Narrower tiles
-  // leave room for two, so that a split that does not divide the SMs evenly
-  // still runs in one wave.
-  static constexpr int kCtasPerSm = TN >= 128 ? 1 : 2;
+  // Two CTAs an SM: a split that does not divide the SMs evenly still runs in
+  // one wave, and one CTA's epilogue meets the other's products.
+  static constexpr int kCtasPerSm = 2;
   static constexpr uint32_t kBudget = kSmemMax / kCtasPerSm - 2048;
   static constexpr int kStagesRaw = (int)(kBudget / (kStageBytes + kPlaceBytes));
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
@@ -377,8 +376,7 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     // ------------------------------- epilogue -------------------------------
     const int group = warp >> 2, quad = warp & 3;
     constexpr int kHalf = TN / 2;
-    constexpr int kMost = C::kCtasPerSm == 1 ? 32 : 16;   // what the registers hold
-    constexpr int kChunk = kHalf < kMost ? kHalf : kMost;
+    constexpr int kChunk = kHalf < 16 ? kHalf : 16;   // what the registers hold
     Out o;
     o.top = 0u;
     {
@@ -571,26 +569,33 @@ constexpr int kSms = 148;
 Plan make_plan(int64_t m, int64_t n, int64_t k) {
   Plan p;
   const int64_t slices = (k + kSliceK - 1) / kSliceK;
-  p.wide = m > 128;
+  // Few tiles: one launch, k split over clusters.  Many: pairs of CTAs behind the
+  // kernel that orders the scales.  (m n k = 512 512 512, 32 tiles: 7.2 us
+  // against 8.4; 200 5120 1280, 160 tiles: 10.4 against 9.4.)
+  p.wide = m > 64 && ((m + 63) / 64) * ((n + 127) / 128) > 96;
   if (p.wide) {
-    // Pairs of CTAs; the narrower tile while the wider leaves pairs without one.
+    // The narrower tile where it takes no more waves of pairs: it is done
+    // sooner, but not twice as soon.  (200 5120 5120: 14.4 us against 15.4; 512
+    // 5120 5120, two waves against one: 19.7 against 16.5.)
     p.tiles_f = (n + 255) / 256;
-    p.tn = p.tiles_f * ((m + 255) / 256) < kSms / 2 ? 128 : 256;
+    auto waves = [&](int64_t tn) {
+      return (p.tiles_f * ((m + tn - 1) / tn) + kSms / 2 - 1) / (kSms / 2);
+    };
+    p.tn = waves(128) <= waves(256) ? 128 : 256;
     p.tiles_t = (m + p.tn - 1) / p.tn;
     p.split = 1;
     return p;
   }
   p.tiles_f = (n + kTileF - 1) / kTileF;
-  p.tn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  p.tiles_t = 1;
-  // Split k while all clusters run at once and every part keeps at least two
-  // slices.  A cluster lives within one GPC: 148 SMs are counted as nine of 16.
-  // (5120 x 5120, one token: 10.9 us whole, 8.9 in four parts, 8.5 in six; in
-  // seven, whose clusters take two waves, 13.4.)
-  const int ctas = p.tn < 128 ? 2 : 1;
+  p.tn = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+  p.tiles_t = (m + p.tn - 1) / p.tn;
+  // Split k while all clusters run at once and every part keeps at least four
+  // slices.  A cluster lives within one GPC: 148 SMs are counted as nine of 16,
+  // each SM with room for two CTAs.  (5120 x 5120, one token: 10.9 us whole, 8.9
+  // in four parts, 8.5 in six; in seven, whose clusters take two waves, 13.4.)
   p.split = 1;
-  for (int s = 2; s <= kMaxSplit && 2 * s <= slices; ++s)
-    if (p.tiles_f <= 9 * (16 * ctas / s)) p.split = s;
+  for (int s = 2; s <= kMaxSplit && 4 * s <= slices; ++s)
+    if (p.tiles_f * p.tiles_t <= 9 * (32 / s)) p.split = s;
   return p;
 }
 
@@ -639,8 +644,7 @@ int launch_type(const Plan& plan, const Params& p, const CUtensorMap& f, const C
   switch (plan.tn) {
     case 16: return launch_tile<16, T, DACT>(plan, p, f, t, sms, st);
     case 32: return launch_tile<32, T, DACT>(plan, p, f, t, sms, st);
-    case 64: return launch_tile<64, T, DACT>(plan, p, f, t, sms, st);
-    default: return launch_tile<128, T, DACT>(plan, p, f, t, sms, st);
+    default: return launch_tile<64, T, DACT>(plan, p, f, t, sms, st);
   }
 }
 

@@ -207,9 +207,9 @@ __device__ __forceinline__ void finish8(const Params& p, Acc& o, float (&x)[8], 
   w.store(reinterpret_cast<T*>(p.d) + t * p.ldd + o.f);
 }
 
-// The same element by element, for the features that exist: ragged borders and
-// unaligned rows.  A function of its own, since the instruction cache holds
-// little more than the loop that calls it.  In: accumulators in x, the scaled
+// The same element by element, for the features that exist: ragged borders.  A
+// function of its own, since the instruction cache holds little more than the
+// loop that calls it.  In: accumulators in x, the scaled
 // bias beside them; out: what D holds (0 outside), for the bias gradient.
 template <typename T, bool DACT>
 __device__ __noinline__ uint32_t finish_some(const Params& p, float alpha, const float* bias,
@@ -254,7 +254,7 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
                                              float* turn, int lane, int t0) {
   constexpr int kRows = kTurnRows / 8;         // tokens of a thread at a time
   const T* res = reinterpret_cast<const T*>(p.res);
-  const bool whole = p.vec && o.f + 8 <= p.n;
+  const bool whole = o.f + 8 <= p.n;
 #pragma unroll
   for (int h = 0; h < 32; h += kTurnRows) {
     Raw8<T> r[kRows];
@@ -314,7 +314,57 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
   }
 }
 
-template <int TN, typename T, bool DACT>
+// Rows that take no vectors (an odd stride or address): a lane keeps its feature
+// f, and a warp's access of one token covers 32 neighbours.  The chunk's tokens
+// are t0 .. t0 + 31.
+template <typename T, bool DACT>
+__device__ __forceinline__ void finish_lanes(const Params& p, Acc& o, const float (&v)[32], int f,
+                                             int t0, float bias, float& sum) {
+  const int count = f < p.n ? p.m - t0 : 0;
+  const T* res = reinterpret_cast<const T*>(p.res) + (int64_t)t0 * p.ldr + f;
+  T* d = reinterpret_cast<T*>(p.d) + (int64_t)t0 * p.ldd + f;
+  T* aux = reinterpret_cast<T*>(p.aux) + (int64_t)t0 * p.ldaux + f;
+  auto all = [&](auto act) {
+#pragma unroll
+    for (int h = 0; h < 32; h += 8) {
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = (DACT || p.res) && h + j < count ? to_f32(*res) : 0.0f;
+        res += p.ldr;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (h + j < count) {
+          float z = v[h + j] * o.alpha;
+          if constexpr (DACT) {
+            z *= slope<decltype(act)::value>(e[j]);
+            sum += z;
+          } else {
+            z += bias;
+            if (p.aux) *aux = from_f32<T>(z);
+            z = activate<decltype(act)::value>(z) + e[j];
+          }
+          const T s = from_f32<T>(z);
+          *d = s;
+          o.some = max(o.some, __float_as_uint(to_f32(s)) & 0x7FFFFFFFu);
+        }
+        d += p.ldd;
+        aux += p.ldaux;
+      }
+    }
+  };
+  switch (p.act) {
+    case kRelu: all(Const<kRelu>()); break;
+    case kGelu: all(Const<kGelu>()); break;
+    case kSilu: all(Const<kSilu>()); break;
+    default: all(Const<kNone>()); break;
+  }
+}
+
+// VEC: rows of D, residual / argument and aux take 16-byte vectors.  (Kernels of
+// their own: with both epilogues in one the vector form lost a fifth.)
+template <int TN, typename T, bool DACT, bool VEC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_gemm_pair(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUtensorMap tm_t,
                 const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_st,
@@ -499,9 +549,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       o.f = tf * 256 + (int)rank * 128 + quad * 32 + (lane & 3) * 8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        o.bias[j] = !DACT && o.f + j < p.n ? load_bias(p, o.f + j) : 0.0f;
+        o.bias[j] = VEC && !DACT && o.f + j < p.n ? load_bias(p, o.f + j) : 0.0f;
         o.dbias[j] = 0.0f;
       }
+      // Without vectors a lane keeps one feature instead.
+      const int lane_f = tf * 256 + (int)rank * 128 + quad * 32 + lane;
+      const float lane_bias = !DACT && !VEC && lane_f < p.n ? load_bias(p, lane_f) : 0.0f;
+      float lane_sum = 0.0f;
       const uint32_t a = n & 1u;
       if (!wait_warp(acc_full(a), (n >> 1) & 1u, abort_flag, kErrTimeoutEpilogue)) break;
       tc_fence_after();
@@ -529,9 +583,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) arrive_cluster(map_rank(acc_free(a), 0));
         }
         if (!have) break;
-        finish_chunk<T, DACT>(p, o, v, turn, lane, tt * TN + 32 * chunk(u));
+        const int t0 = tt * TN + 32 * chunk(u);
+        if constexpr (VEC)
+          finish_chunk<T, DACT>(p, o, v, turn, lane, t0);
+        else
+          finish_lanes<T, DACT>(p, o, v, lane_f, t0, lane_bias, lane_sum);
       }
-      if (DACT && p.dbias_partial) {
+      if (!VEC && DACT && p.dbias_partial) {
+        if (lane_f < p.n) p.dbias_partial[(int64_t)(tt * kGroups + group) * p.n + lane_f] = lane_sum;
+      } else if (DACT && p.dbias_partial) {
         // A feature's tokens are spread over the eight lanes l, l + 4, ...
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -607,10 +667,10 @@ __global__ void __launch_bounds__(256) k_order_scales(const OrderArgs a) {
   }
 }
 
-template <int TN, typename T, bool DACT>
+template <int TN, typename T, bool DACT, bool VEC>
 int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
   using C = Wide<TN>;
-  constexpr auto kernel = k_gemm_pair<TN, T, DACT>;
+  constexpr auto kernel = k_gemm_pair<TN, T, DACT, VEC>;
   if (int e = allow_smem<kernel>((int)C::kSmemBytes)) return e;
   const int64_t tiles = (int64_t)p.tiles_f * p.tiles_t;
   const int64_t pairs = sms / 2 > 0 ? sms / 2 : 1;
@@ -630,12 +690,19 @@ int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t 
   return cuda_status(cudaGetLastError());
 }
 
+template <typename T, bool DACT>
+int launch_tile(int tn, const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
+  if (tn == 128)
+    return p.vec ? launch<128, T, DACT, true>(p, maps, sms, st)
+                 : launch<128, T, DACT, false>(p, maps, sms, st);
+  return p.vec ? launch<256, T, DACT, true>(p, maps, sms, st)
+               : launch<256, T, DACT, false>(p, maps, sms, st);
+}
 template <typename T>
 int launch_type(bool dact, int tn, const Params& p, const CUtensorMap (&maps)[4], int sms,
                 cudaStream_t st) {
-  if (tn == 128)
-    return dact ? launch<128, T, true>(p, maps, sms, st) : launch<128, T, false>(p, maps, sms, st);
-  return dact ? launch<256, T, true>(p, maps, sms, st) : launch<256, T, false>(p, maps, sms, st);
+  return dact ? launch_tile<T, true>(tn, p, maps, sms, st)
+              : launch_tile<T, false>(tn, p, maps, sms, st);
 }
 
 int64_t row_blocks(int64_t rows) { return (rows + 127) / 128; }

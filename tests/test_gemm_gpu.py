@@ -64,7 +64,8 @@ SHAPES = [
     (1, 1, 32), (1, 128, 64), (1, 256, 256), (1, 130, 4096), (2, 5120, 1024), (16, 384, 512),
     (17, 129, 288), (31, 257, 2048), (33, 1000, 96), (64, 128, 512), (65, 200, 1056),
     (100, 3000, 320), (128, 128, 256), (129, 255, 544), (200, 640, 1280), (257, 4096, 512),
-    (511, 2050, 768), (300, 19200, 256), (2100, 2200, 288),
+    (511, 2050, 768), (300, 19200, 256), (2100, 2200, 288), (700, 2047, 224), (130, 9000, 64),
+    (90, 300, 4096), (128, 2000, 1024), (300, 310, 8192),
 ]
 
 
@@ -81,7 +82,7 @@ def test_product(nvlib, m, n, k):
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
 @pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("m,n,k", [(3, 200, 1024), (50, 129, 96), (140, 333, 512),
-                                   (2304, 2200, 64)])
+                                   (2304, 2200, 64), (900, 1501, 96), (80, 400, 2048)])
 def test_epilogue(nvlib, m, n, k, out, act):
     dtype, hs = TYPES[out], orc.half_step(TYPES[out])
     a, b, z, tol = problem(m, n, k, m + n)
@@ -105,7 +106,7 @@ def test_epilogue(nvlib, m, n, k, out, act):
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
 @pytest.mark.parametrize("out", ["bf16", "f32"])
 @pytest.mark.parametrize("m,n,k", [(1, 130, 512), (40, 300, 2048), (333, 514, 256),
-                                   (2500, 2177, 96)])
+                                   (2500, 2177, 96), (1030, 1800, 64), (130, 200, 4096)])
 def test_backward_epilogue(nvlib, m, n, k, out, act):
     dtype, hs = TYPES[out], orc.half_step(TYPES[out])
     a, b, z, tol = problem(m, n, k, m + 2 * n)

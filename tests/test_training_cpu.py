@@ -28,8 +28,8 @@ def gemm(lib, m=4, n=8, k=64, A=P, SFA=P, aa=P, B=P, SFB=P, ab=P, D=P, ldd=None,
     (dict(A=P + 8), ALIGN), (dict(B=P + 8), ALIGN), (dict(D=P + 1), ALIGN),
     (dict(D=P + 2, out=0), ALIGN), (dict(res=P + 1), ALIGN), (dict(aux=P + 1), ALIGN),
     (dict(bias=P + 2), ALIGN), (dict(aa=P + 2), ALIGN), (dict(amax=P + 2), ALIGN),
-    (dict(m=500, n=512), ARG), (dict(m=500, n=512, ws=P, nb=1024), ARG),
-    (dict(m=500, n=512, ws=P + 16, nb=1 << 20), ALIGN),
+    (dict(m=5000, n=512), ARG), (dict(m=5000, n=512, ws=P, nb=1024), ARG),
+    (dict(m=5000, n=512, ws=P + 16, nb=1 << 20), ALIGN),
     (dict(m=0), OK), (dict(n=0), OK), (dict(m=0, A=None, D=None), OK),
 ])
 def test_gemm_refuses(nvlib, kw, want):
@@ -162,7 +162,7 @@ def test_workspaces_follow_the_sizes(nvlib):
                 # whole blocks of 128 rows x 256 codes
                 assert b - a >= 2 * 4 * n
                 assert a in (0, (-(-m // 128) + -(-n // 128)) * -(-k // 256) * 2048)
-    assert plain(128, 5120, 4096) == 0
+    assert plain(64, 5120, 4096) == 0 and plain(128, 512, 4096) == 0
     assert plain(0, 8, 64) == dact(4, 0, 64) == 0
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10, 7) == 10 * 2 * 7 * 4
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 4 * 296 * 2 * 7 * 4
