@@ -249,7 +249,7 @@ __device__ __noinline__ uint32_t finish_some(const Params& p, float alpha, const
 // A warp's chunk: lane l holds feature l's accumulators of the tokens t0 ..
 // t0 + 31 in v.  `turn` is the warp's 2 KB: row = token, 16-byte units of a
 // row swapped by the token's parity so that neither side meets a bank twice.
-template <typename T, bool DACT>
+template <typename T, bool DACT, int ACT>
 __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const float (&v)[32],
                                              float* turn, int lane, int t0) {
   constexpr int kRows = kTurnRows / 8;         // tokens of a thread at a time
@@ -281,12 +281,6 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
       x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
       x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
     }
-    auto all = [&](auto act) {
-#pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        if (t0 + h + row0 + 8 * i < p.m)
-          finish8<T, DACT, decltype(act)::value>(p, o, x[i], r[i], t0 + h + row0 + 8 * i);
-    };
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
@@ -305,66 +299,56 @@ __device__ __forceinline__ void finish_chunk(const Params& p, Acc& o, const floa
       }
       continue;
     }
-    switch (p.act) {
-      case kRelu: all(Const<kRelu>()); break;
-      case kGelu: all(Const<kGelu>()); break;
-      case kSilu: all(Const<kSilu>()); break;
-      default: all(Const<kNone>()); break;
-    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (t0 + h + row0 + 8 * i < p.m)
+        finish8<T, DACT, ACT>(p, o, x[i], r[i], t0 + h + row0 + 8 * i);
   }
 }
 
 // Rows that take no vectors (an odd stride or address): a lane keeps its feature
 // f, and a warp's access of one token covers 32 neighbours.  The chunk's tokens
 // are t0 .. t0 + 31.
-template <typename T, bool DACT>
+template <typename T, bool DACT, int ACT>
 __device__ __forceinline__ void finish_lanes(const Params& p, Acc& o, const float (&v)[32], int f,
                                              int t0, float bias, float& sum) {
   const int count = f < p.n ? p.m - t0 : 0;
   const T* res = reinterpret_cast<const T*>(p.res) + (int64_t)t0 * p.ldr + f;
   T* d = reinterpret_cast<T*>(p.d) + (int64_t)t0 * p.ldd + f;
   T* aux = reinterpret_cast<T*>(p.aux) + (int64_t)t0 * p.ldaux + f;
-  auto all = [&](auto act) {
 #pragma unroll
-    for (int h = 0; h < 32; h += 8) {
-      float e[8];
+  for (int h = 0; h < 32; h += 8) {
+    float e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = (DACT || p.res) && h + j < count ? to_f32(*res) : 0.0f;
-        res += p.ldr;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (h + j < count) {
-          float z = v[h + j] * o.alpha;
-          if constexpr (DACT) {
-            z *= slope<decltype(act)::value>(e[j]);
-            sum += z;
-          } else {
-            z += bias;
-            if (p.aux) *aux = from_f32<T>(z);
-            z = activate<decltype(act)::value>(z) + e[j];
-          }
-          const T s = from_f32<T>(z);
-          *d = s;
-          o.some = max(o.some, __float_as_uint(to_f32(s)) & 0x7FFFFFFFu);
-        }
-        d += p.ldd;
-        aux += p.ldaux;
-      }
+    for (int j = 0; j < 8; ++j) {
+      e[j] = (DACT || p.res) && h + j < count ? to_f32(*res) : 0.0f;
+      res += p.ldr;
     }
-  };
-  switch (p.act) {
-    case kRelu: all(Const<kRelu>()); break;
-    case kGelu: all(Const<kGelu>()); break;
-    case kSilu: all(Const<kSilu>()); break;
-    default: all(Const<kNone>()); break;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (h + j < count) {
+        float z = v[h + j] * o.alpha;
+        if constexpr (DACT) {
+          z *= slope<ACT>(e[j]);
+          sum += z;
+        } else {
+          z += bias;
+          if (p.aux) *aux = from_f32<T>(z);
+          z = activate<ACT>(z) + e[j];
+        }
+        const T s = from_f32<T>(z);
+        *d = s;
+        o.some = max(o.some, __float_as_uint(to_f32(s)) & 0x7FFFFFFFu);
+      }
+      d += p.ldd;
+      aux += p.ldaux;
+    }
   }
 }
 
 // VEC: rows of D, residual / argument and aux take 16-byte vectors.  (Kernels of
 // their own: with both epilogues in one the vector form lost a fifth.)
-template <int TN, typename T, bool DACT, bool VEC>
+template <int TN, typename T, bool DACT, bool VEC, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_gemm_pair(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUtensorMap tm_t,
                 const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_st,
@@ -585,9 +569,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!have) break;
         const int t0 = tt * TN + 32 * chunk(u);
         if constexpr (VEC)
-          finish_chunk<T, DACT>(p, o, v, turn, lane, t0);
+          finish_chunk<T, DACT, ACT>(p, o, v, turn, lane, t0);
         else
-          finish_lanes<T, DACT>(p, o, v, lane_f, t0, lane_bias, lane_sum);
+          finish_lanes<T, DACT, ACT>(p, o, v, lane_f, t0, lane_bias, lane_sum);
       }
       if (!VEC && DACT && p.dbias_partial) {
         if (lane_f < p.n) p.dbias_partial[(int64_t)(tt * kGroups + group) * p.n + lane_f] = lane_sum;
@@ -667,10 +651,10 @@ __global__ void __launch_bounds__(256) k_order_scales(const OrderArgs a) {
   }
 }
 
-template <int TN, typename T, bool DACT, bool VEC>
-int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
+template <int TN, typename T, bool DACT, bool VEC, int ACT>
+int launch_act(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
   using C = Wide<TN>;
-  constexpr auto kernel = k_gemm_pair<TN, T, DACT, VEC>;
+  constexpr auto kernel = k_gemm_pair<TN, T, DACT, VEC, ACT>;
   if (int e = allow_smem<kernel>((int)C::kSmemBytes)) return e;
   const int64_t tiles = (int64_t)p.tiles_f * p.tiles_t;
   const int64_t pairs = sms / 2 > 0 ? sms / 2 : 1;
@@ -690,6 +674,15 @@ int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t 
   return cuda_status(cudaGetLastError());
 }
 
+template <int TN, typename T, bool DACT, bool VEC>
+int launch(const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
+  switch (p.act) {
+    case kRelu: return launch_act<TN, T, DACT, VEC, kRelu>(p, maps, sms, st);
+    case kGelu: return launch_act<TN, T, DACT, VEC, kGelu>(p, maps, sms, st);
+    case kSilu: return launch_act<TN, T, DACT, VEC, kSilu>(p, maps, sms, st);
+    default: return launch_act<TN, T, DACT, VEC, kNone>(p, maps, sms, st);
+  }
+}
 template <typename T, bool DACT>
 int launch_tile(int tn, const Params& p, const CUtensorMap (&maps)[4], int sms, cudaStream_t st) {
   if (tn == 128)
