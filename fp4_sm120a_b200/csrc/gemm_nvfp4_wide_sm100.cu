@@ -354,8 +354,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_st,
                 const Params p) {
   using C = Wide<TN>;
-  // k_dbias may be scheduled; it waits for this kernel to complete.
-  asm volatile("griddepcontrol.launch_dependents;");
+  // k_dbias may be scheduled; it waits for this kernel to complete.  (Only when it
+  // follows: a caller's own programmatic dependent must not start this early.)
+  if (DACT && p.dbias_partial) asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_holder;

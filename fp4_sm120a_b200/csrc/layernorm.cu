@@ -494,12 +494,15 @@ struct BwdArgs {
   int64_t rows, lddy, ldx, ldr, lddx;
   int cols, stages, partials;
   uint32_t slot_bytes;
+  int reduce;           // k_bwd_reduce follows
 };
 
 template <typename T, typename W, bool ALIGNED, int ITEMS, int THREADS, bool RES>
 __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
-  // k_bwd_reduce may be scheduled; it waits for this kernel to complete.
-  asm volatile("griddepcontrol.launch_dependents;");
+  // k_bwd_reduce may be scheduled; it waits for this kernel to complete.  (Only
+  // when it follows: a caller's own programmatic dependent must not start this
+  // early.)
+  if (a.reduce) asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared sh;
   constexpr int VEC = Layout<T, ALIGNED>::kVec, E = ITEMS * VEC;
@@ -979,7 +982,7 @@ NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, in
     return NVFP4_OK;
   }
   BwdArgs a = {dy, x, mean, rstd, gamma, residual, dx, reinterpret_cast<float*>(workspace),
-               rows, lddy, ldx, ldr, lddx, (int)cols, 1, 0, 0u};
+               rows, lddy, ldx, ldr, lddx, (int)cols, 1, 0, 0u, dgamma || dbeta};
   auto rows_of = [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
