@@ -230,16 +230,27 @@ __device__ __forceinline__ uint32_t put(const Mine<T, ALIGNED, ITEMS>& my, T* ro
   }
   return top;
 }
-// This thread's weights, zero behind the row's end.
+// This thread's weights, zero behind the row's end: as 16-byte vectors where
+// they are aligned (a launch of few rows waits for them).
 template <typename T, typename W, bool ALIGNED, int ITEMS>
 __device__ __forceinline__ void fetch_weights(const W* w, int cols, float* f) {
   constexpr int VEC = Layout<T, ALIGNED>::kVec;
+  const bool vectors = ALIGNED && (uintptr_t)w % 16 == 0;
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it) {
+    const int c = ((int)threadIdx.x + it * (int)blockDim.x) * VEC;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const int c = ((int)threadIdx.x + it * (int)blockDim.x) * VEC + k;
-      f[it * VEC + k] = w != nullptr && c < cols ? to_f32(w[c]) : 0.0f;
+    for (int k = 0; k < VEC; ++k) f[it * VEC + k] = 0.0f;
+    if (w != nullptr && c < cols) {
+      if (vectors) {
+        constexpr int N = 16 / (int)sizeof(W);       // VEC or half of it
+#pragma unroll
+        for (int k = 0; k + N <= VEC; k += N)
+          unpack16<W>(*reinterpret_cast<const uint4*>(w + c + k), f + it * VEC + k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[it * VEC + k] = to_f32(w[c + k]);
+      }
     }
   }
 }
