@@ -621,11 +621,12 @@ struct OrderArgs {
 
 __global__ void __launch_bounds__(256) k_order_scales(const OrderArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
-  if (a.amax && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.amax = 0u;
+  if (a.amax && blockIdx.x == 0 && threadIdx.x == 0) *a.amax = 0u;
   __shared__ uint32_t tile[128][33];                     // 8 slices x 4 words, padded
-  const int which = (int)blockIdx.y >= a.blocks0;
-  const int block = (int)blockIdx.y - (which ? a.blocks0 : 0);
-  const int s0 = (int)blockIdx.x * 8;
+  const int groups = (a.slices + 7) / 8;
+  const int at = (int)blockIdx.x / groups, which = at >= a.blocks0;
+  const int block = at - (which ? a.blocks0 : 0);
+  const int s0 = ((int)blockIdx.x - at * groups) * 8;
   const int rows = which ? a.rows[1] : a.rows[0], width = which ? a.width[1] : a.width[0];
   const uint8_t* sf = which ? a.sf[1] : a.sf[0];
   uint32_t* out = which ? a.out[1] : a.out[0];
@@ -733,9 +734,10 @@ int launch_wide(int dtype, bool dact, int tn, const Params& p, const void* a, co
   o.width[1] = p.sf_width_t;
   o.blocks0 = (int)row_blocks(p.n);
   o.amax = p.amax;
-  const int64_t blocks = row_blocks(p.n) + row_blocks(p.m);
-  const dim3 grid((unsigned)((p.slices + 7) / 8), (unsigned)blocks);
-  k_order_scales<<<grid, 256, 0, st>>>(o);
+  // One-dimensional: more than 65535 blocks of rows are a long m, no error.
+  const int64_t blocks = (row_blocks(p.n) + row_blocks(p.m)) * ((p.slices + 7) / 8);
+  if (blocks > INT32_MAX) return NVFP4_ERR_INVALID_SHAPE;
+  k_order_scales<<<(unsigned)blocks, 256, 0, st>>>(o);
   if (cudaError_t e = cudaGetLastError()) return cuda_status(e);
   if (dtype == NVFP4_DTYPE_F32) return launch_type<float>(dact, tn, p, maps, sms, st);
   if (dtype == NVFP4_DTYPE_BF16) return launch_type<__nv_bfloat16>(dact, tn, p, maps, sms, st);

@@ -201,6 +201,17 @@ def test_scale_alignment(nvlib, k, shift):
     close(d, z, tol + 2.0 ** -24 * z.abs(), "d")
 
 
+def test_long_m(nvlib):
+    """More blocks of 128 rows than a grid's second dimension holds (65535)."""
+    base, times, n, k = 1000, 8389, 8, 32
+    a, b, z, tol = problem(base, n, k, 17)
+    rows = [t.cuda().repeat(times, 1) for t in a[:2]]
+    d, _ = nvlib.matmul_nvfp4(*rows, a[2].cuda(), *cuda(b), out_dtype=torch.float32)
+    d = d.view(times, base, n)
+    for edge in (d.amin(0), d.amax(0)):
+        close(edge, z, tol + 2.0 ** -24 * z.abs(), "d")
+
+
 def test_special_values(nvlib):
     """Zero operands, a zero amax, NaN scales and infinite residuals end where
     they belong."""
