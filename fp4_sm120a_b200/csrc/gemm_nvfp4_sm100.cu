@@ -694,6 +694,9 @@ int run(const Call& c) {
   if (!empty) {
     if (!c.a || !c.sfa || !c.b || !c.sfb || !c.amax_a || !c.amax_b || !c.d || (c.dact && !c.res))
       return NVFP4_ERR_INVALID_ARGUMENT;
+    // amax_out is cleared before the operands' amax are read.
+    if (c.amax_out && (c.amax_out == c.amax_a || c.amax_out == c.amax_b))
+      return NVFP4_ERR_INVALID_ARGUMENT;
     const Plan plan = make_plan(c.m, c.n, c.k);
     if (plan.tiles_f * plan.tiles_t > (1ll << 28)) return NVFP4_ERR_INVALID_SHAPE;
     const size_t need = workspace_bytes(c.m, c.n, c.k, c.dbias != nullptr);

@@ -288,7 +288,7 @@ enum { NVFP4_ACT_NONE = 0, NVFP4_ACT_RELU = 1, NVFP4_ACT_GELU = 2, NVFP4_ACT_SIL
  *   residual    m x n, or NULL; may be D itself (accumulation in place)
  *   aux         receives z (what the backward pass needs), or NULL
  *   amax_out    receives max |D| as stored, NaN-propagating (what the cast of
- *               D needs), or NULL
+ *               D needs), or NULL; not amax_a or amax_b
  *   workspace   scratch of nvfp4_gemm_workspace_bytes(m, n, k) bytes, 256-byte
  *               aligned (0 bytes: may be NULL); it needs no initial state and
  *               keeps none, but no two calls may use it at the same time

@@ -36,6 +36,12 @@ def test_gemm_refuses(nvlib, kw, want):
     assert gemm(nvlib.load(), **kw) == want
 
 
+def test_gemm_refuses_its_operands_amax_as_output(nvlib):
+    """amax_out is cleared before the operands' amax are read."""
+    assert gemm(nvlib.load(), amax=P, ab=P + 4) == ARG
+    assert gemm(nvlib.load(), amax=P, aa=P + 4) == ARG
+
+
 def test_gemm_dact_refuses(nvlib):
     lib = nvlib.load()
 
