@@ -8,6 +8,7 @@ ValueError here or NVFP4Error from the library.  The pointer-level forms, with
 explicit streams and workspaces, are in ops."""
 from __future__ import annotations
 
+from itertools import accumulate
 from typing import Optional, Sequence
 
 import torch
@@ -278,36 +279,39 @@ class AdamW:
         amax_ptr = _words(amax_out, count, self._device, "amax_out")
         state = torch.uint8 if self.eight else torch.float32
 
-        def take(seq, i, n, dtype, name):
-            if seq is None:
-                return 0
-            t = seq[i]
-            if (not t.is_cuda or t.device != self.device or t.dtype != dtype or t.numel() != n
-                    or not t.is_contiguous()):
-                raise ValueError(f"{name}[{i}]: expected {n} contiguous {dtype} on {self.device}")
-            self._keep.append(t)
-            return t.data_ptr()
-
         # The tensors are held as long as their addresses are.
         self._keep = [t for t in (amax_out, rng_state) if t is not None]
-        self._table = (AdamWTensor * count)()
-        at = 0
-        for i, d in enumerate(self._table):
-            n = params[i].numel()
-            d.param = take(params, i, n, self.param_dtype, "params")
-            d.grad = take(grads, i, n, self.grad_dtype, "grads")
-            d.exp_avg = take(exp_avgs, i, n, state, "exp_avgs")
-            d.exp_avg_sq = take(exp_avg_sqs, i, n, state, "exp_avg_sqs")
-            if self.eight:
-                blocks = -(-n // STATE_BLOCK)
-                d.exp_avg_scale = take(exp_avg_scales, i, blocks, torch.uint8, "exp_avg_scales")
-                d.exp_avg_sq_scale = take(exp_avg_sq_scales, i, blocks, torch.uint8,
-                                          "exp_avg_sq_scales")
-            d.copy = take(copies, i, n, torch.bfloat16, "copies")
-            d.n = n
-            d.offset = at if offsets is None else int(offsets[i])
-            at += -(-n // STATE_BLOCK) * STATE_BLOCK
-            d.weight_decay = 0.0 if weight_decays is None else float(weight_decays[i])
+        sizes = [p.numel() for p in params]
+        blocks = [-(-n // STATE_BLOCK) for n in sizes]
+
+        def take(seq, sizes, dtype, name):
+            """The addresses of contiguous tensors of these sizes."""
+            if seq is None:
+                return [0] * count
+            for i, (t, n) in enumerate(zip(seq, sizes)):
+                if (t.get_device() != self._device or t.dtype != dtype or t.numel() != n
+                        or not t.is_contiguous()):
+                    raise ValueError(f"{name}[{i}]: expected {n} contiguous {dtype} on "
+                                     f"{self.device}")
+            self._keep.extend(seq)
+            return [t.data_ptr() for t in seq]
+
+        if offsets is None:
+            offsets = [0, *accumulate(b * STATE_BLOCK for b in blocks)][:count]
+        fields = (take(params, sizes, self.param_dtype, "params"),
+                  take(grads, sizes, self.grad_dtype, "grads"),
+                  take(exp_avgs, sizes, state, "exp_avgs"),
+                  take(exp_avg_sqs, sizes, state, "exp_avg_sqs"),
+                  take(exp_avg_scales if self.eight else None, blocks, torch.uint8,
+                       "exp_avg_scales"),
+                  take(exp_avg_sq_scales if self.eight else None, blocks, torch.uint8,
+                       "exp_avg_sq_scales"),
+                  take(copies, sizes, torch.bfloat16, "copies"), sizes, map(int, offsets),
+                  map(float, weight_decays) if weight_decays is not None else [0.0] * count)
+        own = [p for p, n in zip(fields[0], sizes) if n]
+        if len(set(own)) != len(own):
+            raise ValueError("params: the same tensor twice")
+        self._table = (AdamWTensor * count)(*zip(*fields))
         self.count = count
         self._fixed = (self._table, count, _DTYPES[self.param_dtype], _DTYPES[self.grad_dtype],
                        int(self.eight))

@@ -326,3 +326,11 @@ def test_first_step_by_differences(nvlib):
     opt = nvlib.AdamW([p], [g], [torch.zeros(4, device="cuda")], [torch.zeros(4, device="cuda")])
     opt.step(1, lr=0.5, beta1=0.9, beta2=0.95, eps=1e-12)
     close(p, -0.5 * g.sign().double().cpu(), torch.full((4,), 0.5 * 2.0 ** -20), "p")
+
+
+def test_refuses_a_tensor_twice(nvlib):
+    """Tied weights are one parameter: two blocks would update it at once."""
+    p, g, m, v = ([torch.zeros(8, device="cuda") for _ in range(2)] for _ in range(4))
+    nvlib.AdamW(p, g, m, v)
+    with pytest.raises(ValueError):
+        nvlib.AdamW([p[0], p[0]], g, m, v)
