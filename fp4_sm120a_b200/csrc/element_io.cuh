@@ -26,10 +26,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
-// x as T holds it.
-template <typename T>
-__device__ __forceinline__ float round_to(float x) { return to_f32(from_f32<T>(x)); }
-
 // Two values in one 32-bit word (16-bit types), the first in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);

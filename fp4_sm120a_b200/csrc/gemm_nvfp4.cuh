@@ -26,12 +26,6 @@ constexpr uint32_t kAtomBytes = 512;         // scales of 128 rows x one MMA ste
 constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
-// A compile-time choice passed as a value.
-template <int V>
-struct Const {
-  static constexpr int value = V;
-};
-
 enum Activation : int { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
 
 struct Params {
@@ -55,7 +49,7 @@ struct Params {
   int act;
   float* dbias_partial;       // [partial rows][n]
   uint32_t* amax;
-  int vec;                    // D, residual / argument and aux take 16-byte accesses
+  int vec;                    // rows of D, residual / argument and aux are 16-byte aligned (wide kernel)
 };
 
 // Launch of the wide kernel (tiles of 256 (n) x tn (m) by pairs of CTAs); the
@@ -187,9 +181,7 @@ static inline int scale_width(const void* sf, int64_t pitch) {
 // COLS consecutive fp32 columns of this thread's TMEM lane.
 template <int COLS>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[COLS]) {
-  if constexpr (COLS == 32) {
-    tmem_ld_32cols(taddr, v);
-  } else if constexpr (COLS == 16) {
+  if constexpr (COLS == 16) {
     uint32_t r[16];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -202,7 +194,7 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[COLS]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
   } else {
-    static_assert(COLS == 8, "8, 16 or 32 columns");
+    static_assert(COLS == 8, "8 or 16 columns");
     uint32_t r[8];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
