@@ -226,12 +226,12 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
     if (a.amax != nullptr) {
       // the amax of what the cast will read: p rounded to bf16
       if (FULL || i + kVec <= n) {
-        top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][0], p[u][1]) & 0x7FFF7FFFu);
-        top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][2], p[u][3]) & 0x7FFF7FFFu);
+        top = max_abs2<__nv_bfloat16>(top, pack2<__nv_bfloat16>(p[u][0], p[u][1]));
+        top = max_abs2<__nv_bfloat16>(top, pack2<__nv_bfloat16>(p[u][2], p[u][3]));
       } else {
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
-          if (i + k < n) top = __vmaxu2(top, pack2<__nv_bfloat16>(p[u][k], 0.0f) & 0x7FFFu);
+          if (i + k < n) top = max_abs2<__nv_bfloat16>(top, pack2<__nv_bfloat16>(p[u][k], 0.0f));
       }
     }
     if constexpr (EIGHT) {
@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_adamw(const __grid_constant__ A
                      ? adamw_chunk<P, G, EIGHT, true, CAP>(a, t, r, base)
                      : adamw_chunk<P, G, EIGHT, false, CAP>(a, t, r, base);
   if (a.amax != nullptr) {
+    top &= 0x7FFF7FFFu;
     top = __reduce_max_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16)) << 16;
     // The word only grows: a stale read costs an atomic, never a result.
     if ((threadIdx.x & 31) == 0 && top > *(volatile uint32_t*)(a.amax + lo))

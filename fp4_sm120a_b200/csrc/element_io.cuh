@@ -5,6 +5,7 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -51,6 +52,18 @@ __device__ __forceinline__ void unpack2<__half>(uint32_t w, float& a, float& b) 
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
   a = f.x;
   b = f.y;
+}
+
+// Maximum of the magnitudes of two pairs of 16-bit values, NaN if one is; the
+// results' signs mean nothing.
+template <typename T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>)
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // Pairs of fp32 in one instruction (add / mul / fma.rn.f32x2).

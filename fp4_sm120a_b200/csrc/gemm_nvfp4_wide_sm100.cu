@@ -141,8 +141,9 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(p)[i] = q[i];
   }
-  // Unsigned maximum of the magnitudes' bit patterns (per 16-bit half or per
-  // word): above every finite value comes infinity, above that NaN.
+  // Maximum of the magnitudes, NaN if one is: of fp32 words as an unsigned
+  // maximum of their bits (above every finite value comes infinity, above that
+  // NaN), of 16-bit halves with signs that mean nothing.
   __device__ __forceinline__ uint32_t top(uint32_t m) const {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -150,8 +151,8 @@ struct Raw8 {
         m = max(max(m, q[i].x & 0x7FFFFFFFu), q[i].y & 0x7FFFFFFFu);
         m = max(max(m, q[i].z & 0x7FFFFFFFu), q[i].w & 0x7FFFFFFFu);
       } else {
-        m = __vmaxu2(__vmaxu2(m, q[i].x & 0x7FFF7FFFu), q[i].y & 0x7FFF7FFFu);
-        m = __vmaxu2(__vmaxu2(m, q[i].z & 0x7FFF7FFFu), q[i].w & 0x7FFF7FFFu);
+        m = max_abs2<T>(max_abs2<T>(m, q[i].x), q[i].y);
+        m = max_abs2<T>(max_abs2<T>(m, q[i].z), q[i].w);
       }
     }
     return m;
@@ -162,7 +163,7 @@ template <typename T>
 __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
   if constexpr (sizeof(T) == 4) return m;
   float lo, hi;
-  unpack2<T>(m, lo, hi);
+  unpack2<T>(m & 0x7FFF7FFFu, lo, hi);
   return max(__float_as_uint(lo), __float_as_uint(hi));
 }
 

@@ -100,11 +100,13 @@ __device__ __forceinline__ uint4 pack16(const float* x) {
     return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
                       pack2<T>(x[6], x[7]));
 }
-// Unsigned maximum of the magnitudes' bit patterns, per 16-bit half or per
-// word (NaN patterns are above infinity's), and its value as fp32 bits.
+// Maximum of the magnitudes, NaN if one is: of fp32 words as an unsigned maximum
+// of their bits (NaN patterns are above infinity's), of 16-bit halves with signs
+// that mean nothing.  And its value as fp32 bits.
 template <typename T>
 __device__ __forceinline__ uint32_t max_bits(uint32_t m, uint32_t w) {
-  return sizeof(T) == 4 ? max(m, w & 0x7FFFFFFFu) : __vmaxu2(m, w & 0x7FFF7FFFu);
+  if constexpr (sizeof(T) == 4) return max(m, w & 0x7FFFFFFFu);
+  else return max_abs2<T>(m, w);
 }
 template <typename T>
 __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
@@ -112,7 +114,7 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
     return m;
   } else {
     float lo, hi;
-    unpack2<T>(m, lo, hi);
+    unpack2<T>(m & 0x7FFF7FFFu, lo, hi);
     return max(__float_as_uint(lo), __float_as_uint(hi));
   }
 }

@@ -246,6 +246,23 @@ def test_special_values(nvlib):
     assert torch.equal(d, bias.expand(m, n))
 
 
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,n", [(5, 40), (900, 1600), (900, 1601)])
+def test_amax_of_odd_values(nvlib, m, n, out):
+    """The amax of a lone negative maximum, of an infinity and of a NaN, whatever
+    its sign and wherever it stands."""
+    a, b, z, tol = problem(m, n, 64, 3)
+    zero, amax = torch.zeros_like(a[0]).cuda(), torch.empty(1, device="cuda")
+    for at in (0, 3, m * n - 1):
+        for value in (-8.0, math.inf, -math.inf, math.nan, -math.nan):
+            res = torch.full((m, n), 0.5, dtype=TYPES[out], device="cuda")
+            res.view(-1)[at] = value
+            nvlib.matmul_nvfp4(zero, a[1].cuda(), a[2].cuda(), *cuda(b), residual=res,
+                               out_dtype=TYPES[out], amax_out=amax)
+            got = float(amax)
+            assert math.isnan(got) if math.isnan(value) else got == abs(value), (at, value, got)
+
+
 def test_huge_activation_arguments(nvlib):
     """Arguments whose powers overflow: slopes of 0 or 1, no NaN."""
     m, n, k = 4, 130, 64
