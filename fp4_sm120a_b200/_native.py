@@ -12,6 +12,7 @@ from ctypes import (c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_uin
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnvfp4_b200.so"
+BINDING_PATH = LIB_PATH.with_name("_torch_binding.so")
 
 
 class AdamWTensor(ctypes.Structure):
@@ -128,6 +129,22 @@ def load() -> ctypes.CDLL:
         fn.restype = restype
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def load_binding():
+    """The compiled tensor-level calls (csrc/torch_binding.cpp)."""
+    global _binding
+    if _binding is None:
+        load()
+        if not BINDING_PATH.exists():
+            raise ImportError(f"{BINDING_PATH.name} is not built; run "
+                              "`python -m fp4_sm120a_b200.build`")
+        from . import _torch_binding
+        _binding = _torch_binding
+    return _binding
 
 
 def check(fn: str, status: int) -> None:

@@ -1,6 +1,8 @@
-"""Build the in-tree CUDA library libnvfp4_b200.so for sm_100a with nvcc.
+"""Build the in-tree CUDA library libnvfp4_b200.so for sm_100a with nvcc, and the
+tensor-level binding _torch_binding.so against torch's headers with the host
+compiler.
 
-The library is built next to this file so that it travels with the source
+Both are built next to this file so that they travel with the source
 tree; nothing is installed into site-packages.
 """
 from __future__ import annotations
@@ -8,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -17,7 +20,13 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libnvfp4_b200.so"
 OBJDIR = PKG / "_build"
+BINDING = PKG / "_torch_binding.so"
+BINDING_SOURCE = CSRC / "torch_binding.cpp"
 
+# The system's compiler, whatever CXX says: the binding must share torch's
+# libstdc++ (exceptions and streams cross between the two), and another compiler may
+# link a copy of its own.
+CXX = "g++"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["rht_gemm_sm100.cu", "sr_kernels.cu", "fp8_kernels.cu", "fp8_kernels_loose.cu",
            "gemm_nvfp4_sm100.cu", "gemm_nvfp4_wide_sm100.cu", "layernorm.cu", "adamw.cu"]
@@ -39,8 +48,36 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return not target.exists() or any(d.stat().st_mtime > target.stat().st_mtime for d in deps)
 
 
+def _binding_deps() -> list[Path]:
+    return [BINDING_SOURCE, INCLUDE / "nvfp4_b200.h"]
+
+
 def needs_build() -> bool:
-    return _stale(LIB, _deps())
+    return _stale(LIB, _deps()) or _stale(BINDING, _binding_deps())
+
+
+def _run(cmd: list[str], what: str, verbose: bool = False) -> None:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed")
+
+
+def _build_binding(verbose: bool) -> None:
+    """Needs LIB: the binding links against it (found beside it at run time)."""
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
+          f"-I{Path(NVCC).resolve().parent.parent / 'include'}",
+          f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", str(BINDING_SOURCE),
+          "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+          "-ltorch", "-lc10_cuda", "-lc10", f"-L{PKG}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"],
+         "building the torch binding", verbose)
+    os.replace(tmp, BINDING)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -54,23 +91,18 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         obj = OBJDIR / (Path(src).stem + ".o")
         if not force and not _stale(obj, [CSRC / src, *headers]):
             return str(obj)
-        cmd = [NVCC, *FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if verbose or r.returncode != 0:
-            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed on {src}")
+        _run([NVCC, *FLAGS, "-c", str(CSRC / src), "-o", str(obj)], f"nvcc on {src}", verbose)
         return str(obj)
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
-        objs = list(pool.map(compile_one, SOURCES))
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", *objs, "-o", str(tmp)]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
-        raise RuntimeError("link failed")
-    os.replace(tmp, LIB)
+    if force or _stale(LIB, _deps()):
+        with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+            objs = list(pool.map(compile_one, SOURCES))
+        tmp = LIB.with_suffix(".so.tmp")
+        _run([NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", *objs, "-o",
+              str(tmp)], "link")
+        os.replace(tmp, LIB)
+    if force or _stale(BINDING, _binding_deps()):
+        _build_binding(verbose)
     return LIB
 
 

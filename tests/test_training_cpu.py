@@ -173,3 +173,15 @@ def test_workspaces_follow_the_sizes(nvlib):
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10, 7) == 10 * 2 * 7 * 4
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 7) == 4 * 296 * 2 * 7 * 4
     assert lib.nvfp4_layernorm_bwd_workspace_bytes(10**6, 5120) == 296 * 2 * 5120 * 4
+
+
+def test_binding_shares_the_process_libstdcxx(nvlib):
+    """A second copy of the C++ runtime would crash on the first error message."""
+    from fp4_sm120a_b200._native import load_binding
+    x = torch.zeros(2, 32)
+    with pytest.raises(TypeError, match="expected 5 arguments, got 1"):
+        load_binding().layernorm(x)
+    with pytest.raises(ValueError):
+        load_binding().layernorm(3, x, None, 1e-5, None)
+    with pytest.raises(ValueError):
+        load_binding().matmul(*[x] * 6, None, None, 0, 1, None, False, None)
