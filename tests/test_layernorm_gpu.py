@@ -112,6 +112,69 @@ def test_strides(nvlib, dtype, pad, shift):
     check_backward(nvlib, x, gamma, dy, res, mean, rstd, dev=(px, pdy, pres))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols,pad", [(1203, 33, 0), (1203, 33, 1), (1203, 262, 2),
+                                           (901, 1027, 0), (901, 1030, 4), (640, 4098, 8),
+                                           (310, 8191, 1), (5, 3, 5), (3000, 9, 2),
+                                           (1100, 8190, 3), (4100, 2050, 1), (8300, 1011, 0)])
+@pytest.mark.parametrize("places", [(0, 0, 0), (1, 1, 1), (6, 6, 6), (1, 2, 3)])
+def test_unaligned_rows(nvlib, rows, cols, pad, places, dtype):
+    """Rows of any phase of 16 bytes, the same in all arrays and not, many to a
+    block; what lies around the outputs' rows stays as it was."""
+    x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], torch.float32, rows + cols)
+
+    def place(t, at):
+        ld = cols + pad
+        flat = torch.full((rows * ld + 16,), 77.0, dtype=t.dtype, device="cuda")
+        v = flat[at:at + rows * ld].view(rows, ld)[:, :cols]
+        v.copy_(t)
+        return flat, v
+
+    def around(flat, at):
+        keep = flat.clone()
+        keep[at:at + rows * (cols + pad)].view(rows, cols + pad)[:, :cols] = 77.0
+        return bool((keep == 77.0).all())
+    (_, xd), (_, dyd), (_, rd) = (place(t, at) for t, at in zip((x, dy, res), places))
+    mean, rstd = check_forward(nvlib, x, gamma, beta, xd)
+    check_backward(nvlib, x, gamma, dy, res, mean, rstd, (xd, dyd, rd))
+    # the same through the addresses, in place: outputs at the inputs' phases
+    y, _, _ = nvlib.layernorm(xd, gamma.cuda(), beta.cuda())
+    dx, dg, db = nvlib.layernorm_backward(dyd, xd, mean, rstd, gamma.cuda(), residual=rd)
+    ld = cols + pad
+    flat, yd = place(x, places[0])
+    amax = torch.empty(1, device="cuda")
+    nvlib.layernorm_fwd(rows, cols, yd, ld, gamma.cuda(), beta.cuda(), x.dtype, torch.float32, EPS,
+                        yd, ld, None, None, amax)
+    flat2, dxd = place(dy, places[1])
+    ws = torch.empty(nvlib.layernorm_bwd_workspace_bytes(rows, cols), dtype=torch.uint8,
+                     device="cuda")
+    dg2, db2 = torch.empty_like(dg), torch.empty_like(db)
+    nvlib.layernorm_bwd(rows, cols, dxd, ld, xd, ld, mean, rstd, gamma.cuda(), rd, ld, x.dtype,
+                        torch.float32, dxd, ld, dg2, db2, ws, ws.numel())
+    torch.cuda.synchronize()
+    # Two results of the same formula: each within its check's tolerance.
+    L = max(32, cols // 256) + 16
+    m, r = mean.double().cpu()[:, None], rstd.double().cpu()[:, None]
+    h, g = (x.double() - m) * r, gamma.double().abs()
+    one = (r * g * L * 2.0 ** -24 * x.double().abs().amax(1, keepdim=True)
+           + L * 2.0 ** -22 * h.abs() * g + 2.0 ** -23 * beta.double().abs()
+           + (orc.half_step(x.dtype) + 2.0 ** -23) * y.double().cpu().abs() * (1 + 2.0 ** -6)
+           + orc.least_step(x.dtype))
+    close(yd, y.double().cpu(), 2 * one, "y in place")
+    u = (dy.double() * gamma.double()).abs()
+    part = r * (u + u.mean(1, keepdim=True) + h.abs() * (u * h.abs()).mean(1, keepdim=True))
+    one = (L * 2.0 ** -22 * part + 2.0 ** -23 * res.double().abs()
+           + orc.half_step(x.dtype) * dx.double().cpu().abs() * (1 + 2.0 ** -6)
+           + orc.least_step(x.dtype))
+    close(dxd, dx.double().cpu(), 2 * one, "dx in place")
+    t = 2 * (rows + 70) * 2.0 ** -24
+    close(dg2, dg.double().cpu(), t * (dy.double() * h).abs().sum(0), "dgamma in place")
+    close(db2, db.double().cpu(), t * dy.double().abs().sum(0), "dbeta in place")
+    assert float(amax) == float(yd.float().abs().max())
+    assert around(flat, places[0]) and around(flat2, places[1])
+    assert nvlib.device_error() == 0
+
+
 def test_offset_and_outliers(nvlib):
     """A common offset far above the spread, and a first element far off: the
     statistics keep their digits."""
