@@ -32,9 +32,9 @@
 // Few tiles (short m): the k range is split over a cluster of up to 8 CTAs,
 // whose partial tiles meet in distributed shared memory and are added in rank
 // order (no atomics: results repeat bit for bit).
-// Measured, on the device: 1 x 5120 x 5120 8.5 us (14.8 MB; a launch, the first
-// loads' latency and the cluster's join are most of it), 37 x 5000 x 8192 11.6 us
-// (24 MB), 64 x 5120 x 5120 12.6 us.  The bytes alone would take 2.3, 3.7 and
+// Measured, on the device: 1 x 5120 x 5120 7.7 us (14.8 MB; a launch, the first
+// loads' latency and the cluster's join are most of it), 37 x 5000 x 8192 11.2 us
+// (24 MB), 64 x 5120 x 5120 10.8 us.  The bytes alone would take 2.3, 3.7 and
 // 2.4 us.
 // Every wait is bounded; a kernel that gives up records an error word, waits
 // for its own copies and MMAs, frees TMEM and returns.
@@ -181,33 +181,6 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
   const uint32_t drain = bar0 + 8 * (2 * C::kStages + 2 * C::kAccStages);
   volatile uint32_t* abort_flag = &abort_word;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 1 + 2);
-      mbar_init(empty(s), 1);
-    }
-    for (int a = 0; a < C::kAccStages; ++a) {
-      mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), kEpiThreads);
-    }
-    mbar_init(drain, 1);
-    abort_word = 0u;
-    fence_barrier_init();
-  }
-  if (warp == kWarpTma && lane == 0) {
-    prefetch_tmap(&tm_f);
-    prefetch_tmap(&tm_t);
-  }
-  if (warp == kWarpMma) {
-    tmem_alloc(smem_addr(&tmem_holder), C::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_holder;
-  const uint32_t tmem_sf = tmem + C::kAccStages * TN;
-
   // This CTA's tiles and k-slices.
   const uint32_t split = SPLIT ? cluster_size() : 1u, rank = SPLIT ? cluster_rank() : 0u;
   const int first = SPLIT ? (int)(blockIdx.x / split) : (int)blockIdx.x;
@@ -216,26 +189,57 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
   const int s_begin = SPLIT ? (int)((int64_t)p.slices * rank / split) : 0;
   const int s_end = SPLIT ? (int)((int64_t)p.slices * (rank + 1) / split) : p.slices;
 
+  // The one barrier of all warps: behind it barriers and TMEM stand.  Each role
+  // comes to it after what it can do alone, so that the first loads are under way
+  // while TMEM is being allocated (one token, 5120 x 5120: 7.7 us against 8.4).
+  auto start = [&] {
+    __syncwarp();
+    tc_fence_before();
+    asm volatile("barrier.cta.sync.aligned 0, %0;" ::"n"(C::kThreads) : "memory");
+    tc_fence_after();
+  };
+  float alpha = 0.0f, bias = 0.0f;      // of the epilogue's threads; the bias with SPLIT
+
   if (warp == kWarpTma) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, issued = 0;
-      bool ok = true;
-      for (int i = first; i < tiles && ok; i += stride) {
+    uint32_t stage = 0, phase = 0, issued = 0;
+    int tile = first, slice = s_begin;
+    // Loads until `most` have been issued; false: given up.
+    auto produce = [&](uint32_t most) {
+      while (tile < tiles && issued < most) {
+        // (The first kStages find their stages empty.)
+        if (issued >= (uint32_t)C::kStages &&
+            !wait(empty(stage), phase ^ 1u, abort_flag, kErrTimeoutProducer))
+          return false;
         int tf, tt;
-        tile_at(p, i, tf, tt);
-        for (int s = s_begin; s < s_end; ++s) {
-          if (!wait(empty(stage), phase ^ 1u, abort_flag, kErrTimeoutProducer)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = ring + stage * C::kStageBytes;
-          mbar_arrive_expect_tx(full(stage), C::kBytesF + C::kBytesT);
-          tma_load_2d(dst, &tm_f, full(stage), s * 128, tf * kTileF);
-          tma_load_2d(dst + C::kBytesF, &tm_t, full(stage), s * 128, tt * TN);
-          ++issued;
-          if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
-        }
+        tile_at(p, tile, tf, tt);
+        const uint32_t dst = ring + stage * C::kStageBytes;
+        mbar_arrive_expect_tx(full(stage), C::kBytesF + C::kBytesT);
+        tma_load_2d(dst, &tm_f, full(stage), slice * 128, tf * kTileF);
+        tma_load_2d(dst + C::kBytesF, &tm_t, full(stage), slice * 128, tt * TN);
+        ++issued;
+        if (++stage == (uint32_t)C::kStages) { stage = 0; phase ^= 1u; }
+        if (++slice == s_end) { slice = s_begin; tile += stride; }
       }
+      return true;
+    };
+    if (lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(full(s), 1 + 2);
+        mbar_init(empty(s), 1);
+      }
+      for (int a = 0; a < C::kAccStages; ++a) {
+        mbar_init(acc_full(a), 1);
+        mbar_init(acc_empty(a), kEpiThreads);
+      }
+      mbar_init(drain, 1);
+      abort_word = 0u;
+      fence_barrier_init();
+      fence_proxy_async_smem();
+      produce(C::kStages);
+    }
+    start();
+    if (lane == 0) {
+      const bool ok = produce(0xFFFFFFFFu);
       if (!ok) {
         // Given up: the loads in flight land before the CTA ends.  (A stage
         // whose scale loader gave up too never completes: its wait runs to the
@@ -250,6 +254,10 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     }
     __syncwarp();
   } else if (warp == kWarpMma) {
+    tmem_alloc(smem_addr(&tmem_holder), C::kTmemCols);
+    tmem_relinquish();
+    start();
+    const uint32_t tmem = tmem_holder, tmem_sf = tmem + C::kAccStages * TN;
     // The whole warp walks the loop, so that addresses and descriptors stay
     // uniform; one elected lane issues.
     const bool leader = elect_one();
@@ -352,6 +360,7 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     uint32_t stage = 0, phase = 0;
     Cursor in = {first, s_begin}, out = in;
     for (int j = 0; j < C::kStages; ++j, next(in)) fetch(in, j);
+    start();
     bool ok = true;
     while (out.tile < tiles) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
@@ -384,10 +393,17 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
     Out o;
     o.top = 0u;
     {
-      // The two amax are on their way while the first tile is computed.
       const float ea = global_encode_scale(*p.amax_f), eb = global_encode_scale(*p.amax_t);
-      o.alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
+      o.alpha = alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
     }
+    if constexpr (SPLIT) {
+      int tf, tt;
+      tile_at(p, first, tf, tt);
+      const int f = tf * kTileF + quad * 32 + lane;
+      if (f < p.n) bias = load_bias(p, f);
+    }
+    start();
+    const uint32_t tmem = tmem_holder;
     uint32_t acc = 0, acc_phase = 0;
     for (int i = first; i < tiles; i += stride) {
       int tf, tt;
@@ -449,10 +465,9 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
       Out o;
       o.top = 0u;
       o.dbias = 0.0f;
-      const float ea = global_encode_scale(*p.amax_f), eb = global_encode_scale(*p.amax_t);
-      o.alpha = __fdiv_rn(1.0f, ea) * __fdiv_rn(1.0f, eb);
+      o.alpha = alpha;
+      o.bias = bias;
       if (f < p.n) {
-        o.bias = load_bias(p, f);
         const int c0 = (int)rank + group * (int)split;     // this group's first column
         const int step = 2 * (int)split;
         const int have = min(TN, p.m - tt * TN);
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__(Tile<TN>::kThreads, Tile<TN>::kCtasPerSm)
   __syncthreads();
   if (warp == kWarpMma) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
+    tmem_dealloc(tmem_holder, C::kTmemCols);
   }
 }
 
