@@ -221,7 +221,9 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
     }
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
-      const float update = __fdividef(mu[k], fmaf(fast_sqrt(vu[k]), r.rbc2, a.eps));
+      // (The root of a subnormal number is far above them; an eps below 2^-126
+      // counts as zero.)
+      const float update = mu[k] * fast_rcp(fmaf(fast_sqrt(vu[k]), r.rbc2, a.eps));
       p[u][k] = fmaf(-update, r.step_size, p[u][k] * r.keep);
     }
     store4(pp, i, n, full, p[u]);

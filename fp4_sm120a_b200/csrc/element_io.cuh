@@ -54,6 +54,19 @@ __device__ __forceinline__ void unpack2<__half>(uint32_t w, float& a, float& b) 
   b = f.y;
 }
 
+// 1 / x and 2^x to a few 2^-23, subnormal arguments and results taken as zero: the
+// full-range forms spend more instructions on those than on the result.
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Maximum of the magnitudes of two pairs of 16-bit values, NaN if one is; the
 // results' signs mean nothing.
 template <typename T>

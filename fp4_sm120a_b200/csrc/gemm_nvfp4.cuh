@@ -207,8 +207,10 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[COLS]) {
   }
 }
 
-// 1 / (1 + exp(-x)) from the hardware's exponential and reciprocal.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// 1 / (1 + exp(-x)).  Where 2^-126 is the difference, 1 + exp(-x) does not show it.
+__device__ __forceinline__ float sigmoid(float x) {
+  return fast_rcp(1.0f + fast_exp2(-1.4426950408889634f * x));
+}
 
 constexpr float kGeluC = 1.5957691216057308f;    // 2 sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
