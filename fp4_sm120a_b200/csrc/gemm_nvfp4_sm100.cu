@@ -589,9 +589,12 @@ Plan make_plan(int64_t m, int64_t n, int64_t k) {
   Plan p;
   const int64_t slices = (k + kSliceK - 1) / kSliceK;
   // Few tiles: one launch, k split over clusters.  Many: pairs of CTAs behind the
-  // kernel that orders the scales.  (m n k = 512 512 512, 32 tiles: 7.2 us
-  // against 8.4; 200 5120 1280, 160 tiles: 10.4 against 9.4.)
-  p.wide = m > 64 && ((m + 63) / 64) * ((n + 127) / 128) > 96;
+  // kernel that orders the scales, which a short k does not repay while every SM
+  // has one tile.  (m n k = 512 512 512, 32 tiles: 7.2 us against 8.4; 128 6400 512,
+  // 100 tiles: 7.0 against 8.2; 128 7000 1280, 110 tiles: 8.8 against 9.0; 400 2560
+  // 4096, 140 tiles: 13.5 against 12.1; 200 5120 1280, 160 tiles: 10.2 against 9.0.)
+  const int64_t few = slices <= 5 ? kSms : 96;
+  p.wide = m > 64 && ((m + 63) / 64) * ((n + 127) / 128) > few;
   if (p.wide) {
     // The narrower tile where it takes no more waves of pairs: it is done
     // sooner, but not twice as soon.  (200 5120 5120: 14.4 us against 15.4; 512

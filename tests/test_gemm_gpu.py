@@ -65,7 +65,8 @@ SHAPES = [
     (17, 129, 288), (31, 257, 2048), (33, 1000, 96), (64, 128, 512), (65, 200, 1056),
     (100, 3000, 320), (128, 128, 256), (129, 255, 544), (200, 640, 1280), (257, 4096, 512),
     (511, 2050, 768), (300, 19200, 256), (2100, 2200, 288), (700, 2047, 224), (130, 9000, 64),
-    (90, 300, 4096), (128, 2000, 1024), (300, 310, 8192),
+    (90, 300, 4096), (128, 2000, 1024), (300, 310, 8192), (127, 6401, 480), (65, 9400, 1280),
+    (66, 9500, 1280), (129, 6400, 1312),
 ]
 
 
