@@ -590,15 +590,15 @@ Plan make_plan(int64_t m, int64_t n, int64_t k) {
   const int64_t slices = (k + kSliceK - 1) / kSliceK;
   // Few tiles: one launch, k split over clusters.  Many: pairs of CTAs behind the
   // kernel that orders the scales, which a short k does not repay while every SM
-  // has one tile.  (m n k = 512 512 512, 32 tiles: 7.2 us against 8.4; 128 6400 512,
+  // has one tile.  (m n k = 512 512 512, 32 tiles: 7.0 us against 7.9; 128 6400 512,
   // 100 tiles: 7.0 against 8.2; 128 7000 1280, 110 tiles: 8.8 against 9.0; 400 2560
   // 4096, 140 tiles: 13.5 against 12.1; 200 5120 1280, 160 tiles: 10.2 against 9.0.)
   const int64_t few = slices <= 5 ? kSms : 96;
   p.wide = m > 64 && ((m + 63) / 64) * ((n + 127) / 128) > few;
   if (p.wide) {
     // The narrower tile where it takes no more waves of pairs: it is done
-    // sooner, but not twice as soon.  (200 5120 5120: 14.4 us against 15.4; 512
-    // 5120 5120, two waves against one: 19.7 against 16.5.)
+    // sooner, but not twice as soon.  (200 5120 5120: 14.0 us against 15.1; 512
+    // 5120 5120, two waves against one: 19.5 against 16.4.)
     p.tiles_f = (n + 255) / 256;
     auto waves = [&](int64_t tn) {
       return (p.tiles_f * ((m + tn - 1) / tn) + kSms / 2 - 1) / (kSms / 2);
@@ -613,8 +613,8 @@ Plan make_plan(int64_t m, int64_t n, int64_t k) {
   p.tiles_t = (m + p.tn - 1) / p.tn;
   // Split k while all clusters run at once and every part keeps at least four
   // slices.  A cluster lives within one GPC: 148 SMs are counted as nine of 16,
-  // each SM with room for two CTAs.  (5120 x 5120, one token: 10.9 us whole, 8.9
-  // in four parts, 8.5 in six; in seven, whose clusters take two waves, 13.4.)
+  // each SM with room for two CTAs.  (5120 x 5120, one token: 11.5 us whole, 8.5
+  // in four parts, 8.0 in five or six; in seven, whose clusters take two waves, 11.5.)
   p.split = 1;
   for (int s = 2; s <= kMaxSplit && 4 * s <= slices; ++s)
     if (p.tiles_f * p.tiles_t <= 9 * (32 / s)) p.split = s;
