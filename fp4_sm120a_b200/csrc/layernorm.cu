@@ -30,9 +30,8 @@
 // TB/s), 16384 x 8192 171 us (6.3 TB/s), fp32 16384 x 4096 159 us (6.8 TB/s).  The
 // forward pass is bound by the latency of a row's two reductions at the 32 warps an
 // SM that the registers allow (issue slots 61 % taken), the backward pass by memory.
-// Unaligned rows: bf16 forward 8192 x 5121 78 us, backward 139; fp32 10000 x 5001 88 us
-// (4.5 TB/s) and 157 us (5.1 TB/s), backward 1003 x 4099 20 us, bound by their
-// addressing.  Rows wider than the registers: bf16 forward 4096 x 16384 94 us (2.8
+// Unaligned rows: bf16 forward 8192 x 5121 66 us, backward 95; fp32 10000 x 5001 81 us
+// (5.0 TB/s) and 122 us (6.5 TB/s), backward 1003 x 4099 17 us.  Rows wider than the registers: bf16 forward 4096 x 16384 94 us (2.8
 // TB/s), backward 189.
 #include <atomic>
 #include <cstdint>
@@ -134,28 +133,22 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
   }
 }
 
-// The part of a row that bulk copies can take: whole 16-byte units.  The few
-// elements before and behind them (unaligned rows) are read directly, so
-// nothing outside the row is touched.
-struct Span {
-  uint32_t lead;     // bytes from the 16-byte boundary below the row to the row
-  uint32_t skip;     // ... to the first whole unit (0 or 16)
-  uint32_t bytes;    // of whole units
-};
+// A row's bytes in whole 16-byte units, which is what bulk copies move.  The first
+// and last unit of an unaligned row hold its neighbours' bytes too: they are read
+// (an aligned unit lies within one allocation) and left unused, whatever is being
+// written to them meanwhile.  Loading the row's share of them apart, a row ahead,
+// made the first warp late for every barrier (fp32 backward 10000 x 4097: 151 us
+// against 102).
 template <int MODE>
-__device__ __forceinline__ Span span_of(const void* row, uint32_t row_bytes) {
-  if constexpr (MODE == kWhole) return {0u, 0u, row_bytes};
-  const uint32_t lead = (uint32_t)((uintptr_t)row & 15u), skip = lead ? 16u : 0u;
-  const uint32_t end = (lead + row_bytes) & ~15u;
-  return {lead, skip, end > skip ? end - skip : 0u};
+__device__ __forceinline__ uint32_t span_bytes(const void* row, uint32_t row_bytes) {
+  if constexpr (MODE == kWhole) return row_bytes;
+  return (((uint32_t)(uintptr_t)row & 15u) + row_bytes + 15u) & ~15u;
 }
-// Starts a row's copy; returns the bytes to expect.
 template <int MODE>
-__device__ __forceinline__ void span_load(const Span& s, uint32_t slot, const void* row,
+__device__ __forceinline__ void span_load(uint32_t slot, const void* row, uint32_t row_bytes,
                                           uint32_t bar) {
-  if (MODE == kWhole || s.bytes)
-    bulk_load(slot + s.skip, reinterpret_cast<const unsigned char*>(row) - s.lead + s.skip, s.bytes,
-              bar);
+  bulk_load(slot, reinterpret_cast<const void*>((uintptr_t)row & ~(uintptr_t)15),
+            span_bytes<MODE>(row, row_bytes), bar);
 }
 // A thread's items (vectors or elements) within the row: the first `count`.
 template <typename T, int MODE, int ITEMS>
@@ -189,31 +182,6 @@ struct Mine {
   }
   __device__ __forceinline__ bool in(int it, int k) const {
     return k >= (it == 0 && threadIdx.x == 0 ? shift : 0) && k < (it == last ? hi : kVec);
-  }
-};
-// The elements of an unaligned row outside its whole 16-byte units lie among
-// its first and last eight.  Lanes 0-15 of the first warp look after one each:
-// they load it a row ahead of the row's copy and store it into the slot when
-// the copy starts, two barriers before the slot is read.
-template <typename T, int MODE>
-struct Edge {
-  int e;       // this lane's element, -1: none
-  T value;
-  __device__ __forceinline__ explicit Edge(int cols) : e(-1), value() {
-    if (MODE != kWhole && threadIdx.x < 16) {
-      const int lane = (int)threadIdx.x;
-      e = cols >= 16 && lane >= 8 ? cols - 16 + lane : lane;
-      if (e >= cols) e = -1;
-    }
-  }
-  __device__ __forceinline__ void load(const T* row) {
-    if (MODE != kWhole && e >= 0) value = row[e];
-  }
-  __device__ __forceinline__ void store(unsigned char* slot, const Span& s) const {
-    if (MODE != kWhole && e >= 0) {
-      const uint32_t off = s.lead + (uint32_t)e * (uint32_t)sizeof(T);
-      if (off - s.skip >= s.bytes) *reinterpret_cast<T*>(slot + off) = value;
-    }
   }
 };
 // This thread's elements of a row that has arrived in `slot`.
@@ -375,26 +343,15 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   ring.stages = a.stages;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
   auto row_at = [&](int64_t k) { return (int64_t)blockIdx.x + k * gridDim.x; };
-  Edge<T, MODE> edge(a.cols);
-  // By the first warp; row k's edge elements have been loaded.
   auto issue = [&](int64_t k, uint32_t stage) {
     const T* row = x + row_at(k) * a.ldx;
-    const Span s = span_of<MODE>(row, row_bytes);
-    edge.store(smem + stage * ring.stage_bytes, s);
-    if (tid == 0) {
-      mbar_arrive_expect_tx(ring.bar + 8 * stage, s.bytes);
-      span_load<MODE>(s, ring.base + stage * ring.stage_bytes, row, ring.bar + 8 * stage);
-    }
-    if (k + 1 < mine) edge.load(x + row_at(k + 1) * a.ldx);
+    mbar_arrive_expect_tx(ring.bar + 8 * stage, span_bytes<MODE>(row, row_bytes));
+    span_load<MODE>(ring.base + stage * ring.stage_bytes, row, row_bytes, ring.bar + 8 * stage);
   };
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
     fence_barrier_init();
-  }
-  if (warp == 0) {
-    __syncwarp();
-    edge.load(x + row_at(0) * a.ldx);
     for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
@@ -471,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
     // before this barrier.)
     __syncthreads();
     if (*(volatile uint32_t*)&sh.abort_flag) break;
-    if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
+    if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     // A lane joins one warp's share; every warp does so by itself.
     const float2 part = share < nwarps ? sh.red[k & 1][share] : make_float2(0.0f, 0.0f);
     const float mean = join_sum<THREADS / 32>(part.x * (nw * inv_n));
@@ -596,39 +553,21 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   ring.bar = smem_addr(sh.bar);
   ring.stages = a.stages;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
-  Edge<T, MODE> ex(a.cols), ed(a.cols), er(a.cols);
-  auto edges = [&](int64_t row) {
-    ex.load(x + row * a.ldx);
-    ed.load(dy + row * a.lddy);
-    if constexpr (RES) er.load(res + row * a.ldr);
-  };
-  // By the first warp; row k's edge elements have been loaded.
   auto issue = [&](int64_t k, uint32_t stage) {
     const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
     const int64_t row = blockIdx.x + k * gridDim.x;
-    const Span s0 = span_of<MODE>(x + row * a.ldx, row_bytes);
-    const Span s1 = span_of<MODE>(dy + row * a.lddy, row_bytes);
-    const Span s2 = RES ? span_of<MODE>(res + row * a.ldr, row_bytes) : Span{0u, 0u, 0u};
-    unsigned char* slot = smem + stage * ring.stage_bytes;
-    ex.store(slot, s0);
-    ed.store(slot + ring.slot_bytes, s1);
-    if constexpr (RES) er.store(slot + 2 * ring.slot_bytes, s2);
-    if (tid == 0) {
-      mbar_arrive_expect_tx(bar, s0.bytes + s1.bytes + s2.bytes);
-      span_load<MODE>(s0, dst, x + row * a.ldx, bar);
-      span_load<MODE>(s1, dst + ring.slot_bytes, dy + row * a.lddy, bar);
-      if constexpr (RES) span_load<MODE>(s2, dst + 2 * ring.slot_bytes, res + row * a.ldr, bar);
-    }
-    if (k + 1 < mine) edges(row + gridDim.x);
+    const T *rx = x + row * a.ldx, *rdy = dy + row * a.lddy;
+    const T* rr = RES ? res + row * a.ldr : nullptr;
+    mbar_arrive_expect_tx(bar, span_bytes<MODE>(rx, row_bytes) + span_bytes<MODE>(rdy, row_bytes) +
+                                   (RES ? span_bytes<MODE>(rr, row_bytes) : 0u));
+    span_load<MODE>(dst, rx, row_bytes, bar);
+    span_load<MODE>(dst + ring.slot_bytes, rdy, row_bytes, bar);
+    if constexpr (RES) span_load<MODE>(dst + 2 * ring.slot_bytes, rr, row_bytes, bar);
   };
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
     fence_barrier_init();
-  }
-  if (warp == 0) {
-    __syncwarp();
-    edges(blockIdx.x);
     for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
@@ -680,7 +619,7 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
     }
     __syncthreads();
     if (*(volatile uint32_t*)&sh.abort_flag) break;
-    if (warp == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
+    if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
     const int share = THREADS > 512 ? lane : lane & 15;
     const float2 part = share < nwarps ? sh.red[k & 1][share] : make_float2(0.0f, 0.0f);
     const float c1 = join_sum<THREADS / 32>(part.x) * inv_n * rstd;
