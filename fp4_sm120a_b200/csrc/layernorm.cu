@@ -806,11 +806,12 @@ bool in_phase(const void* x, int64_t ldx, const void* p, int64_t ld, int64_t es)
 }
 // Unaligned rows of at least so many columns, and in the backward pass of at
 // least so many elements, go by vectors with partial ends (kPhased); the others
-// element by element, which starts sooner.  Forward, bf16: 16000 x 1001 35 us against
-// 45, 4000 x 4099 33 against 53, but 4000 x 777 16.5 against 16.4 and 16000 x 201 22
-// against 21.  Backward, bf16: 4000 x 4099 68 us against 73, f16 9000 x 8001 168
-// against 227, but 1200 x 4099 25 against 24 and 4000 x 777 19 against 18.
-constexpr int64_t kPhasedCols = 1000, kPhasedSize = 1 << 23;
+// element by element, which starts sooner.  Forward, bf16: 16000 x 1001 31 us against
+// 41, 4000 x 4099 29 against 43, 16000 x 777 30 against 37, but fp32 16000 x 501 25
+// against 23 and 16000 x 201 23 against 19.  Backward, bf16: 4000 x 4099 49 us against
+// 53, 16000 x 1001 44 against 46, but 1200 x 4099 22 against 21 and 4000 x 777 18
+// against 16.
+constexpr int64_t kPhasedCols = 700, kPhasedSize = 1 << 23;
 uint32_t slot_of(size_t row_bytes, bool aligned) {
   return (uint32_t)(aligned ? row_bytes : (row_bytes + 15) / 16 * 16 + 16);
 }
