@@ -21,9 +21,13 @@
 // (k_fwd_wide, k_bwd_wide).
 //
 // The statistics come from two passes over registers: each warp's mean, then
-// its sum of squares about that mean, combined over warps by
-//   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
-// so a large common offset or an outlier costs no digits.
+// its sum of squares about that mean, and of what the first pass's rounding left
+// in the mean; combined over warps by
+//   mean = mean_0 + sum_w n_w (mean_w - mean_0) / n,  M2 = sum_w M2_w + n_w (mean_w - mean)^2.
+// Every sum but the first is of differences (or exact), so the mean is off by its own last
+// rounding and by little of the spread, however large a common offset is, and the
+// mean of a constant row is its value exactly: x - mean is zero there, which an
+// rstd of 1 / sqrt(eps) would otherwise blow up.
 //
 // Measured, bf16 with fp32 weights: forward with the amax 16384 x 8192 105 us (5.1
 // TB/s), 16384 x 5120 74 us; backward with a residual 16384 x 5120 122 us (5.5
@@ -66,6 +70,30 @@ __device__ __forceinline__ float join_sum(float x) {
 #pragma unroll
   for (int o = WARPS > 16 ? 16 : 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
   return x;
+}
+
+// Mean and sum of squares about it (times `scale`), of n values whose sums about a
+// rounded mean `m` are q (of squares) and `left`; fix = left / n.  Values that are
+// not finite leave m as it is and the squares not finite.
+__device__ __forceinline__ float2 centred(float m, float q, float left, float fix, float scale) {
+  const float m2 = (q - left * fix) * scale;
+  return make_float2(fix == fix ? m + fix : m, m2 < 0.0f ? 0.0f : m2);
+}
+// Two sums over 16 lanes, for the joint of at most 16 warps: the lower half warp
+// joins a, the upper one b, of the same warps.  And over 32 lanes.  In all lanes.
+__device__ __forceinline__ float2 halves_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  const float other = __shfl_xor_sync(0xFFFFFFFFu, v, 16);
+  return threadIdx.x & 16 ? make_float2(other, v) : make_float2(v, other);
+}
+__device__ __forceinline__ float2 warp_sum2(float a, float b) {
+  const bool upper = threadIdx.x & 16;
+  const float give = upper ? a : b, keep = upper ? b : a;
+  return halves_sum(keep + __shfl_xor_sync(0xFFFFFFFFu, give, 16));
+}
+__device__ __forceinline__ float finite_or_zero(float x) {
+  return fabsf(x) <= 3.402823466e38f ? x : 0.0f;
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
@@ -329,9 +357,13 @@ template <typename T, typename W, int MODE, int ITEMS, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared sh;
+  // Of each warp: the elements n it holds of a row, 1 / n (0 for none), n / cols and
+  // 1 / cols.  In shared memory, since registers that do not change over the rows
+  // are the ones that get spilled, and a spilled one costs more than these reads
+  // (16384 x 8192 bf16: 108 us with four words spilled, 104 with none).
+  __shared__ float4 counts[16];
   constexpr int VEC = Layout<T, MODE>::kVec, E = ITEMS * VEC;
   const int tid = threadIdx.x, nthr = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int nwarps = nthr >> 5;
   const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
   const T* x = reinterpret_cast<const T*>(a.x);
   const Mine<T, MODE, ITEMS> my(a.cols, x + blockIdx.x * a.ldx);
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   ring.base = smem_addr(smem);
   ring.bar = smem_addr(sh.bar);
   ring.stages = a.stages;
-  const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
   auto row_at = [&](int64_t k) { return (int64_t)blockIdx.x + k * gridDim.x; };
   auto issue = [&](int64_t k, uint32_t stage) {
     const T* row = x + row_at(k) * a.ldx;
@@ -358,30 +390,33 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   const W* wb = reinterpret_cast<const W*>(a.beta);
   // Weights stay in registers while there is room for them.
   constexpr bool kKeep = E <= 16;
+  constexpr bool kSumLeft = sizeof(T) == 4;
   float gamma[E], beta[E];
   if constexpr (kKeep) {
     fetch_weights<T, W, MODE, ITEMS>(my, wg, a.cols, gamma);
     fetch_weights<T, W, MODE, ITEMS>(my, wb, a.cols, beta);
   }
-  __syncthreads();
-  // The warp whose sums this lane joins, and the elements it holds of a row
-  // (0 for lanes without a warp).
-  const int share = THREADS > 512 ? lane : lane & 15;
-  float nw = 0.0f;
-  if (share < nwarps) {
+  static_assert(THREADS <= 512, "a half warp joins all warps");
+  const int share = lane & 15;        // the warp whose sums this lane joins
+  if (warp == 0 && lane < 16) {
+    float n = 0.0f;
+    if (lane >= nthr >> 5) {
+      sh.red[0][lane] = sh.red[1][lane] = make_float2(0.0f, 0.0f);
+    } else {
 #pragma unroll
-    for (int it = 0; it < ITEMS; ++it)
-      nw += (float)(min(max(my.total - share * 32 - it * nthr, 0), 32) * VEC);
-    if constexpr (MODE == kPhased) {
-      if (share == 0) nw -= (float)my.shift;
-      if ((my.total - 1) % nthr >> 5 == share) nw -= (float)(VEC - my.hi);
+      for (int it = 0; it < ITEMS; ++it)
+        n += (float)(min(max(my.total - lane * 32 - it * nthr, 0), 32) * VEC);
+      if constexpr (MODE == kPhased) {
+        if (lane == 0) n -= (float)my.shift;
+        if ((my.total - 1) % nthr >> 5 == lane) n -= (float)(VEC - my.hi);
+      }
     }
+    const float inv_n = 1.0f / (float)a.cols;
+    counts[lane] = make_float4(n, n > 0.0f ? 1.0f / n : 0.0f, n * inv_n, inv_n);
   }
-  const float own = __shfl_sync(0xFFFFFFFFu, nw, warp);
-  const float inv_own = own > 0.0f ? 1.0f / own : 0.0f;
-  const float inv_n = 1.0f / (float)a.cols;
+  __syncthreads();
   uint32_t top = 0;
-  int64_t k = 0;
+  int k = 0;
   RingAt at;
   for (; k < mine; ++k, at.next(ring)) {
     const int64_t row = row_at(k);
@@ -391,8 +426,16 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
       uint64_t s = pair(0.0f, 0.0f);
 #pragma unroll
       for (int e = 0; e < E; e += 2) s = add2(s, pair(f[e], f[e + 1]));
-      const float mw = warp_sum(sum2(s)) * inv_own;
+      const float4 own = counts[warp];
+      const float sum = warp_sum(sum2(s));
+      float mw = sum * own.y;
+      // What the rounding of mw leaves.  In 16 bits the difference of the sums: a
+      // warp's 1024 values of similar size at most (8 or 11 digits and 10 more) add up
+      // without rounding.  In 32 bits sum (f - mw), taken along with the squares.
+      // (16384 x 8192 bf16: 104 us, with the second sum 118.)
+      if constexpr (!kSumLeft) mw += finite_or_zero(fmaf(-own.x, mw, sum) * own.y);
       const uint64_t minus = pair(-mw, -mw);
+      uint64_t r = pair(0.0f, 0.0f);
       s = pair(0.0f, 0.0f);
       if constexpr (MODE != kOdd) {
 #pragma unroll
@@ -408,6 +451,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
             for (int e = it * VEC; e < (it + 1) * VEC; e += 2) {
               const uint64_t d = add2(pair(f[e], f[e + 1]), minus);
               s = fma2(d, d, s);
+              if constexpr (kSumLeft) r = add2(r, d);
             }
           }
         }
@@ -418,10 +462,16 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
           const float u = my.has(e) ? f[e] : mw, v = my.has(e + 1) ? f[e + 1] : mw;
           const uint64_t d = add2(pair(u, v), minus);
           s = fma2(d, d, s);
+          if constexpr (kSumLeft) r = add2(r, d);
         }
       }
-      const float q = warp_sum(sum2(s));
-      if (lane == 0) sh.red[k & 1][warp] = make_float2(mw, q);
+      if constexpr (kSumLeft) {
+        const float2 t = warp_sum2(sum2(s), sum2(r));
+        if (lane == 0) sh.red[k & 1][warp] = centred(mw, t.x, t.y, t.y * own.y, own.w);
+      } else {
+        const float q = warp_sum(sum2(s)) * own.w;
+        if (lane == 0) sh.red[k & 1][warp] = make_float2(mw, q);
+      }
     }
     // Everybody has taken its part of the stage and written its sums.  (The
     // sums alternate between two copies: those written next were last read
@@ -429,11 +479,18 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
     __syncthreads();
     if (*(volatile uint32_t*)&sh.abort_flag) break;
     if (tid == 0 && k + ring.stages < mine) issue(k + ring.stages, at.stage);
-    // A lane joins one warp's share; every warp does so by itself.
-    const float2 part = share < nwarps ? sh.red[k & 1][share] : make_float2(0.0f, 0.0f);
-    const float mean = join_sum<THREADS / 32>(part.x * (nw * inv_n));
-    const float d = part.x - mean;
-    const float rstd = rsqrtf(join_sum<THREADS / 32>(part.y + nw * d * d) * inv_n + a.eps);
+    // A lane joins one warp's share; every warp does so by itself.  Both sums are
+    // taken about the first warp's mean, so that neither waits for the other: with
+    // v = mean - about, M2 = sum (M2_w + n_w (mean_w - about)^2) - n v^2.  The first
+    // warp's own deviation is in M2, so the difference loses four digits of 24 at
+    // the most.
+    const float2 part = sh.red[k & 1][share];       // zeros where there is no such warp
+    const float about = finite_or_zero(sh.red[k & 1][0].x);
+    const float d = part.x - about, v = d * counts[share].z;
+    const float2 joint = halves_sum(lane < 16 ? v : fmaf(v, d, part.y));
+    const float mean = about + joint.x;
+    const float var = joint.y - joint.x * joint.x;
+    const float rstd = rsqrtf((var < 0.0f ? 0.0f : var) + a.eps);
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -442,8 +499,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
       fetch_weights<T, W, MODE, ITEMS>(my, wg, a.cols, gamma);
       fetch_weights<T, W, MODE, ITEMS>(my, wb, a.cols, beta);
     }
-    // (x - mean) first: a constant row's difference is zero exactly, whatever
-    // rstd makes of a rounding error.
+    // (x - mean) first: a constant row's difference is zero exactly, and stays so
+    // whatever rstd is.
     const uint64_t scale = pair(rstd, rstd), minus = pair(-mean, -mean);
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
@@ -462,38 +519,57 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   }
 }
 
+// Sums of f(c, a, b) over a thread's columns, in runs of 32 that are added
+// afterwards: the error of a sum of a long row does not grow with its length.
+template <typename F>
+__device__ __forceinline__ float2 wide_sums(int cols, const F& f) {
+  constexpr int kRun = 32;
+  float a = 0.0f, b = 0.0f;
+  int c = threadIdx.x;
+  while (c < cols) {
+    float ra = 0.0f, rb = 0.0f;
+    const int end = min(c + kRun * kWideThreads, cols);
+#pragma unroll 8
+    for (; c < end; c += kWideThreads) f(c, ra, rb);
+    a += ra;
+    b += rb;
+  }
+  return make_float2(warp_sum(a), warp_sum(b));
+}
 // Rows wider than the registers hold: three passes over a row, the second and
 // third mostly from cache.
 template <typename T, typename W>
 __global__ void __launch_bounds__(kWideThreads) k_fwd_wide(const FwdArgs a) {
-  __shared__ float red[2][kWideThreads / 32];
+  __shared__ float first[kWideThreads / 32];
+  __shared__ float2 second[kWideThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float inv_n = 1.0f / (float)a.cols;
   uint32_t top = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
     T* y = reinterpret_cast<T*>(a.y) + row * a.ldy;
-    float s = 0.0f;
-    for (int c = tid; c < a.cols; c += kWideThreads) s += to_f32(x[c]);
-    s = warp_sum(s);
-    if (lane == 0) red[0][warp] = s;
+    const float2 s = wide_sums(a.cols, [&](int c, float& sum, float&) { sum += to_f32(x[c]); });
+    if (lane == 0) first[warp] = s.x;
     __syncthreads();
-    float mean = 0.0f;
+    float m = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWideThreads / 32; ++w) mean += red[0][w];
-    mean *= inv_n;
-    float q = 0.0f;
-    for (int c = tid; c < a.cols; c += kWideThreads) {
-      const float d = to_f32(x[c]) - mean;
-      q += d * d;
+    for (int w = 0; w < kWideThreads / 32; ++w) m += first[w];
+    m *= inv_n;
+    const float2 t = wide_sums(a.cols, [&](int c, float& squares, float& left) {
+      const float d = to_f32(x[c]) - m;
+      squares += d * d;
+      left += d;
+    });
+    if (lane == 0) second[warp] = t;
+    __syncthreads();
+    float q = 0.0f, left = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWideThreads / 32; ++w) {
+      q += second[w].x;
+      left += second[w].y;
     }
-    q = warp_sum(q);
-    if (lane == 0) red[1][warp] = q;
-    __syncthreads();
-    float m2 = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWideThreads / 32; ++w) m2 += red[1][w];
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(m2 * inv_n + a.eps));
+    const float2 stat = centred(m, q, left, left * inv_n, inv_n);
+    const float mean = stat.x, rstd = __fdiv_rn(1.0f, __fsqrt_rn(stat.y + a.eps));
     if (tid == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;

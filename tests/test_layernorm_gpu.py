@@ -285,3 +285,36 @@ def test_streams_and_capture(nvlib, rows, cols):
         torch.cuda.synchronize()
         assert torch.equal(gy, y) and all(torch.equal(p, q) for p, q in zip(gg, want))
         assert float(amax) == float(y.float().abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("cols", [40, 100, 501, 777, 1000, 4097, 5000, 5120, 12288, 16411, 70001])
+def test_constant_rows_give_beta(nvlib, cols, dtype):
+    """A row of one value, whatever its digits: the mean is that value, and y is
+    beta, however small eps is."""
+    g = torch.Generator().manual_seed(cols)
+    values = torch.cat([torch.tensor([935.1373, 0.1, -1.0 / 3.0, 1000.1]),
+                        torch.rand(60, generator=g) * 1000.0]).to(TYPES[dtype])
+    x = values[:, None].expand(values.numel(), cols).contiguous()
+    gamma, beta = torch.randn(2, cols, generator=g)
+    for eps in (1e-5, 1e-12):
+        y, mean, rstd = nvlib.layernorm(x.cuda(), gamma.cuda(), beta.cuda(), eps)
+        assert torch.equal(mean.cpu(), values.float())
+        assert torch.equal(y.cpu(), beta.to(TYPES[dtype]).expand_as(x))
+
+
+@pytest.mark.parametrize("cols", [100, 777, 1000, 5000, 5120, 12288, 20001])
+@pytest.mark.parametrize("offset", [1000.0, -935.1373, 60000.0])
+def test_mean_of_rows_with_an_offset(nvlib, cols, offset):
+    """The mean is off by two roundings (a warp's and the row's, 2^-24 of it each)
+    and by its sums of differences: chains of at most 64 additions, 2^-18 of the
+    mean difference."""
+    x, gamma, beta, _, _ = make(24, cols, torch.float32, torch.float32, cols, offset=offset)
+    y, mean, rstd = nvlib.layernorm(x.cuda(), gamma.cuda(), beta.cuda(), EPS)
+    wy, wm, wr = orc.layernorm(x, gamma, beta, EPS)
+    spread = (x.double() - wm[:, None]).abs()
+    em = 2.0 ** -23 * wm.abs() + 2.0 ** -18 * spread.mean(1)
+    close(mean, wm, em, "mean")
+    g, h = gamma.double().abs(), spread * wr[:, None]
+    close(y, wy, g * ((wr * em)[:, None] + 64 * 2.0 ** -22 * h) + 2.0 ** -22 * beta.double().abs()
+          + 2.0 ** -23 * wy.abs(), "y")
