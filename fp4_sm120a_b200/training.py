@@ -140,8 +140,10 @@ class AdamW:
                            or rng_state is None):
             raise ValueError("8-bit moments need their scales and rng_state")
         if rng_state is not None and (rng_state.numel() != 2 or rng_state.dtype != torch.int64
+                                      or not rng_state.is_contiguous()
                                       or rng_state.device != self.device):
-            raise ValueError("rng_state: expected int64 {seed, offset} on the parameters' device")
+            raise ValueError("rng_state: expected contiguous int64 {seed, offset} on the "
+                             "parameters' device")
         self._device = _device(params[0])
         amax_ptr = _words(amax_out, count, self._device, "amax_out")
         state = torch.uint8 if self.eight else torch.float32

@@ -185,3 +185,13 @@ def test_binding_shares_the_process_libstdcxx(nvlib):
         load_binding().layernorm(3, x, None, 1e-5, None)
     with pytest.raises(ValueError):
         load_binding().matmul(*[x] * 6, None, None, 0, 1, None, False, None)
+
+
+@pytest.mark.parametrize("rng", [torch.zeros(4, dtype=torch.int64)[::2],
+                                 torch.zeros(1, dtype=torch.int64).expand(2)])
+def test_adamw_refuses_a_strided_rng_state(nvlib, rng):
+    """The kernel reads {seed, offset} as adjacent words."""
+    w, u = torch.ones(32), torch.zeros(32, dtype=torch.uint8)
+    s = torch.zeros(1, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="rng_state"):
+        nvlib.AdamW([w], [w], [u], [u], exp_avg_scales=[s], exp_avg_sq_scales=[s], rng_state=rng)
