@@ -6,13 +6,16 @@
 // a layer norm of 16 x 5120 takes 6.3 us there, 7 us of host time here, and took 14
 // through ctypes, of which the library's own launch is 4.
 //
-// Each function takes its arguments by position and returns a tuple of tensors,
-// or the library's status as an int when that is not 0.  Bad tensors raise
-// ValueError.
+// Each function takes its arguments by position and returns a tuple of tensors (or
+// the table of an optimizer's tensors), or the library's status as an int when that
+// is not 0.  Bad tensors raise ValueError.
 #include <Python.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <memory>
+#include <utility>
+#include <vector>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -20,6 +23,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include "nvfp4_b200.h"
 
@@ -320,24 +324,204 @@ PyObject* layernorm_backward(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// device, table, count, parameter type, gradient type, state format, amax_out, rng_state
-// (addresses), lr, beta1, beta2, eps, step, grad_scale, scalars -> ()
+// The lists of tensors of an AdamW step.
+enum List { kParams, kGrads, kAvgs, kAvgSqs, kAvgScales, kAvgSqScales, kCopies, kLists };
+constexpr const char* kListName[kLists] = {"params",         "grads",
+                                           "exp_avgs",       "exp_avg_sqs",
+                                           "exp_avg_scales", "exp_avg_sq_scales",
+                                           "copies"};
+
+// A tensor whose address a table holds.  Holding the tensor does not hold its memory:
+// `p.data = ...`, set_ and resize_ give a tensor other memory and free the old, so
+// that every step looks whether the tensor is still what it was.
+struct Held {
+  Tensor tensor;
+  const void* data;
+  int64_t n;
+  ScalarType type;
+  explicit Held(const Tensor& t)
+      : tensor(t), data(t.data_ptr()), n(t.numel()), type(t.scalar_type()) {}
+  bool same() const {
+    return tensor.const_data_ptr() == data && tensor.numel() == n &&
+           tensor.scalar_type() == type && tensor.is_contiguous();
+  }
+};
+
+struct AdamWTable {
+  int device = 0, param = 0, grad = 0, state = 0;
+  std::vector<nvfp4_adamw_tensor> rows;
+  std::vector<Held> lists[kLists];
+  std::vector<Held> words;             // amax_out, rng_state
+  std::vector<char> follows;           // grads[i] is params[i].grad
+  float* amax = nullptr;
+  const size_t* rng = nullptr;
+};
+constexpr const char* kTableName = "fp4_sm120a_b200.AdamWTable";
+constexpr int64_t kStateBlock = 128;
+
+AdamWTable& table_of(PyObject* o) {
+  void* p = PyCapsule_GetPointer(o, kTableName);
+  if (!p) throw python_error();
+  return *static_cast<AdamWTable*>(p);
+}
+
+// A list's tensors: contiguous, of one type, n(i) elements each.
+template <typename N>
+std::vector<Held> held(PyObject* seq, size_t count, ScalarType type, List list, const N& n) {
+  THPObjectPtr fast(PySequence_Fast(seq, kListName[list]));
+  if (!fast) throw python_error();
+  TORCH_CHECK_VALUE((size_t)PySequence_Fast_GET_SIZE(fast.get()) == count, kListName[list], ": ",
+                    PySequence_Fast_GET_SIZE(fast.get()), " entries for ", count, " parameters");
+  std::vector<Held> r;
+  r.reserve(count);
+  for (size_t i = 0; i < count; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(fast.get(), i);
+    TORCH_CHECK_VALUE(THPVariable_Check(o), kListName[list], "[", i, "]: expected a tensor");
+    const Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK_VALUE(t.scalar_type() == type && t.numel() == n(i) && t.is_contiguous(),
+                      kListName[list], "[", i, "]: expected ", n(i), " contiguous ", type,
+                      ", got ", t.sizes(), " ", t.scalar_type());
+    r.emplace_back(t);
+  }
+  return r;
+}
+void on_device(const std::vector<Held>& list, int device, const char* name) {
+  for (size_t i = 0; i < list.size(); ++i)
+    TORCH_CHECK_VALUE(list[i].tensor.is_cuda() && list[i].tensor.get_device() == device, name, "[",
+                      i, "]: not on the parameters' device");
+}
+// Which gradients are their parameters' own .grad.
+void see_whose(AdamWTable& t) {
+  t.follows.resize(t.rows.size());
+  for (size_t i = 0; i < t.rows.size(); ++i) {
+    const Tensor& g = t.lists[kParams][i].tensor.unsafeGetTensorImpl()->grad();
+    t.follows[i] = g.defined() && g.is_same(t.lists[kGrads][i].tensor);
+  }
+}
+void put_grads(AdamWTable& t, std::vector<Held>&& grads) {
+  on_device(grads, t.device, kListName[kGrads]);
+  t.lists[kGrads] = std::move(grads);
+  for (size_t i = 0; i < t.rows.size(); ++i) t.rows[i].grad = t.lists[kGrads][i].data;
+  see_whose(t);
+}
+
+// params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, copies,
+// weight_decays, offsets, amax_out, rng_state (None where there is none; the types of
+// the first tensors, and what belongs together, have been looked at) -> table
+PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count(n_args, 11);
+  auto t = std::make_unique<AdamWTable>();
+  const Py_ssize_t tensors = PySequence_Size(o[kParams]);
+  if (tensors < 0) throw python_error();
+  TORCH_CHECK_VALUE(tensors > 0, "no parameters");
+  TORCH_CHECK_VALUE(tensors <= INT32_MAX, "params: too many");
+  auto type_of_first = [&](List list) {
+    THPObjectPtr first(PySequence_GetItem(o[list], 0));
+    if (!first) throw python_error();
+    return tensor(first.get(), kListName[list]).scalar_type();
+  };
+  const ScalarType param = type_of_first(kParams), grad = type_of_first(kGrads),
+                   state = type_of_first(kAvgs) == kU8 ? kU8 : kF32;
+  t->param = code_of(param, "params");
+  t->grad = code_of(grad, "grads");
+  t->state = state == kU8 ? NVFP4_STATE_8BIT : NVFP4_STATE_F32;
+  t->rows.resize(tensors);
+  {
+    THPObjectPtr fast(PySequence_Fast(o[kParams], "params"));
+    if (!fast) throw python_error();
+    for (Py_ssize_t i = 0; i < tensors; ++i)
+      t->rows[i].n =
+          (uint64_t)tensor(PySequence_Fast_GET_ITEM(fast.get(), i), "params").numel();
+  }
+  auto size = [&](size_t i) { return (int64_t)t->rows[i].n; };
+  auto blocks = [&](size_t i) { return (size(i) + kStateBlock - 1) / kStateBlock; };
+  t->lists[kParams] = held(o[kParams], tensors, param, kParams, size);
+  std::vector<Held> grads = held(o[kGrads], tensors, grad, kGrads, size);
+  for (List list : {kAvgs, kAvgSqs}) t->lists[list] = held(o[list], tensors, state, list, size);
+  if (state == kU8)
+    for (List list : {kAvgScales, kAvgSqScales})
+      t->lists[list] = held(o[list], tensors, kU8, list, blocks);
+  if (o[kCopies] != Py_None)
+    t->lists[kCopies] = held(o[kCopies], tensors, ScalarType::BFloat16, kCopies, size);
+
+  const Tensor& first_param = t->lists[kParams][0].tensor;
+  TORCH_CHECK_VALUE(first_param.is_cuda(), "params: expected CUDA tensors");
+  t->device = (int)first_param.get_device();
+  for (int list = 0; list < kLists; ++list)
+    on_device(t->lists[list], t->device, kListName[list]);
+  t->amax = words(o[9], tensors, t->device, "amax_out");
+  if (o[9] != Py_None) t->words.emplace_back(tensor(o[9], "amax_out"));
+  if (o[10] != Py_None) {
+    t->words.emplace_back(tensor(o[10], "rng_state"));
+    t->rng = (const size_t*)t->words.back().data;
+  }
+
+  THPObjectPtr decays(o[7] == Py_None ? nullptr : PySequence_Fast(o[7], "weight_decays"));
+  THPObjectPtr offsets(o[8] == Py_None ? nullptr : PySequence_Fast(o[8], "offsets"));
+  if ((o[7] != Py_None && !decays) || (o[8] != Py_None && !offsets)) throw python_error();
+  uint64_t next = 0;
+  for (size_t i = 0; i < t->rows.size(); ++i) {
+    nvfp4_adamw_tensor& r = t->rows[i];
+    auto at = [&](List list) -> void* {
+      return t->lists[list].empty() ? nullptr : const_cast<void*>(t->lists[list][i].data);
+    };
+    r.param = at(kParams);
+    r.exp_avg = at(kAvgs);
+    r.exp_avg_sq = at(kAvgSqs);
+    r.exp_avg_scale = (uint8_t*)at(kAvgScales);
+    r.exp_avg_sq_scale = (uint8_t*)at(kAvgSqScales);
+    r.copy = at(kCopies);
+    r.weight_decay = decays ? real(PySequence_Fast_GET_ITEM(decays.get(), i)) : 0.0;
+    r.offset = offsets ? (uint64_t)integer(PySequence_Fast_GET_ITEM(offsets.get(), i)) : next;
+    next += (uint64_t)(blocks(i) * kStateBlock);
+  }
+  std::vector<const void*> own;
+  for (const Held& h : t->lists[kParams])
+    if (h.n) own.push_back(h.data);
+  std::sort(own.begin(), own.end());
+  TORCH_CHECK_VALUE(std::adjacent_find(own.begin(), own.end()) == own.end(),
+                    "params: the same tensor twice");
+  put_grads(*t, std::move(grads));
+  PyObject* capsule = PyCapsule_New(t.get(), kTableName, [](PyObject* c) {
+    delete static_cast<AdamWTable*>(PyCapsule_GetPointer(c, kTableName));
+  });
+  if (!capsule) throw python_error();
+  t.release();
+  return capsule;
+  END_HANDLE_TH_ERRORS
+}
+
+// table, lr, beta1, beta2, eps, step, grad_scale, scalars, new gradients or None -> ()
 PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  count(n_args, 15);
-  const int device = (int)integer(o[0]);
-  const auto* table = (const nvfp4_adamw_tensor*)integer(o[1]);
-  const int tensors = (int)integer(o[2]), param = (int)integer(o[3]), grad = (int)integer(o[4]),
-            state = (int)integer(o[5]);
-  float* amax = (float*)integer(o[6]);
-  const auto* rng = (const size_t*)integer(o[7]);
-  const double lr = real(o[8]), beta1 = real(o[9]), beta2 = real(o[10]), eps = real(o[11]);
-  const int64_t step = integer(o[12]);
-  const float *scale = words(o[13], 1, device, "grad_scale"),
-              *scalars = words(o[14], 3, device, "scalars");
-  return result(launch(device, [&](nvfp4_stream_t stream) {
-    return nvfp4_adamw_step(table, tensors, param, grad, state, lr, beta1, beta2, eps, step, scale,
-                            scalars, amax, rng, stream);
+  count(n_args, 9);
+  AdamWTable& t = table_of(o[0]);
+  const double lr = real(o[1]), beta1 = real(o[2]), beta2 = real(o[3]), eps = real(o[4]);
+  const int64_t step = integer(o[5]);
+  const float *scale = words(o[6], 1, t.device, "grad_scale"),
+              *scalars = words(o[7], 3, t.device, "scalars");
+  for (const Held& w : t.words)
+    TORCH_CHECK_VALUE(w.same(), "amax_out, rng_state: the tensor has other memory now");
+  for (int list = 0; list < kLists; ++list) {
+    if (list == kGrads && o[8] != Py_None) continue;
+    for (size_t i = 0; i < t.lists[list].size(); ++i)
+      TORCH_CHECK_VALUE(t.lists[list][i].same(), kListName[list], "[", i,
+                        "]: the tensor has other memory, size or type than when it was listed");
+  }
+  if (o[8] != Py_None) {
+    put_grads(t, held(o[8], t.rows.size(), type_of(t.grad), kGrads,
+                      [&](size_t i) { return (int64_t)t.rows[i].n; }));
+  } else {
+    for (size_t i = 0; i < t.rows.size(); ++i)
+      TORCH_CHECK_VALUE(!t.follows[i] || t.lists[kParams][i].tensor.unsafeGetTensorImpl()
+                                             ->grad().is_same(t.lists[kGrads][i].tensor),
+                        "grads[", i, "]: params[", i,
+                        "].grad is another tensor now; pass the new gradients (grads=)");
+  }
+  return result(launch(t.device, [&](nvfp4_stream_t stream) {
+    return nvfp4_adamw_step(t.rows.data(), (int)t.rows.size(), t.param, t.grad, t.state, lr,
+                            beta1, beta2, eps, step, scale, scalars, t.amax, t.rng, stream);
   }));
   END_HANDLE_TH_ERRORS
 }
@@ -368,7 +552,8 @@ PyObject* adamw_unpack_state(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
 #define NVFP4_METHOD(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {NVFP4_METHOD(matmul),    NVFP4_METHOD(matmul_dact),
                           NVFP4_METHOD(layernorm), NVFP4_METHOD(layernorm_backward),
-                          NVFP4_METHOD(adamw_step), NVFP4_METHOD(adamw_unpack_state),
+                          NVFP4_METHOD(adamw_table), NVFP4_METHOD(adamw_step),
+                          NVFP4_METHOD(adamw_unpack_state),
                           {nullptr, nullptr, 0, nullptr}};
 #undef NVFP4_METHOD
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding",

@@ -12,26 +12,16 @@ The checks and calls of the step's own operators are compiled
 device."""
 from __future__ import annotations
 
-import ctypes
-from itertools import accumulate
 from typing import Optional, Sequence
 
 import torch
 
 from . import ops
-from ._native import AdamWTensor, check, load_binding
+from ._native import check, load_binding
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _F32 = torch.float32
 STATE_BLOCK = 128   # elements that share one scale byte of an 8-bit state
-
-
-def _device(x) -> int:
-    """Index of a CUDA tensor's device."""
-    d = x.get_device() if isinstance(x, torch.Tensor) else -1
-    if d < 0:
-        raise ValueError("expected a CUDA tensor")
-    return d
 
 
 def _result(name: str, r):
@@ -39,15 +29,6 @@ def _result(name: str, r):
     if r.__class__ is int:
         check(name, r)
     return r
-
-
-def _words(t: Optional[torch.Tensor], n: int, device: int, name: str) -> int:
-    """Address of n float32 on the device, 0 for None."""
-    if t is None:
-        return 0
-    if t.numel() != n or t.dtype != _F32 or not t.is_contiguous() or t.get_device() != device:
-        raise ValueError(f"{name}: expected {n} float32 on cuda:{device}")
-    return t.data_ptr()
 
 
 def matmul_nvfp4(a: torch.Tensor, a_scales: torch.Tensor, a_amax: torch.Tensor, b: torch.Tensor,
@@ -107,7 +88,13 @@ class AdamW:
     position of its first element in the numbering that the random bits go by
     (`offsets`, multiples of 128; default: one tensor behind the other).
     `copies` (bfloat16) receive the rounded new parameters, `amax_out` (one
-    float32 per tensor) their amax.  All memory is the caller's."""
+    float32 per tensor) their amax.  All memory is the caller's.
+
+    The tensors are held, and every step looks whether each still has the memory
+    it had (after `p.data = ...`, set_ or resize_ it has not: ValueError).
+    Gradients that are new tensors are passed to step, which then uses them until
+    it gets others; a gradient that was its parameter's .grad when it was listed
+    must still be that (ValueError otherwise)."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                  exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
@@ -144,57 +131,24 @@ class AdamW:
                                       or rng_state.device != self.device):
             raise ValueError("rng_state: expected contiguous int64 {seed, offset} on the "
                              "parameters' device")
-        self._device = _device(params[0])
-        amax_ptr = _words(amax_out, count, self._device, "amax_out")
-        state = torch.uint8 if self.eight else torch.float32
-
-        # The tensors are held as long as their addresses are.
-        self._keep = [t for t in (amax_out, rng_state) if t is not None]
-        sizes = [p.numel() for p in params]
-        blocks = [-(-n // STATE_BLOCK) for n in sizes]
-
-        def take(seq, sizes, dtype, name):
-            """The addresses of contiguous tensors of these sizes."""
-            if seq is None:
-                return [0] * count
-            for i, (t, n) in enumerate(zip(seq, sizes)):
-                if (t.get_device() != self._device or t.dtype != dtype or t.numel() != n
-                        or not t.is_contiguous()):
-                    raise ValueError(f"{name}[{i}]: expected {n} contiguous {dtype} on "
-                                     f"{self.device}")
-            self._keep.extend(seq)
-            return [t.data_ptr() for t in seq]
-
-        if offsets is None:
-            offsets = [0, *accumulate(b * STATE_BLOCK for b in blocks)][:count]
-        fields = (take(params, sizes, self.param_dtype, "params"),
-                  take(grads, sizes, self.grad_dtype, "grads"),
-                  take(exp_avgs, sizes, state, "exp_avgs"),
-                  take(exp_avg_sqs, sizes, state, "exp_avg_sqs"),
-                  take(exp_avg_scales if self.eight else None, blocks, torch.uint8,
-                       "exp_avg_scales"),
-                  take(exp_avg_sq_scales if self.eight else None, blocks, torch.uint8,
-                       "exp_avg_sq_scales"),
-                  take(copies, sizes, torch.bfloat16, "copies"), sizes, map(int, offsets),
-                  map(float, weight_decays) if weight_decays is not None else [0.0] * count)
-        own = [p for p, n in zip(fields[0], sizes) if n]
-        if len(set(own)) != len(own):
-            raise ValueError("params: the same tensor twice")
-        self._table = (AdamWTensor * count)(*zip(*fields))
+        self._table = load_binding().adamw_table(
+            params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales if self.eight else None,
+            exp_avg_sq_scales if self.eight else None, copies,
+            None if weight_decays is None else [float(d) for d in weight_decays],
+            None if offsets is None else [int(x) for x in offsets], amax_out, rng_state)
         self.count = count
-        self._fixed = (self._device, ctypes.addressof(self._table), count,
-                       _DTYPES[self.param_dtype], _DTYPES[self.grad_dtype], int(self.eight),
-                       amax_ptr, 0 if rng_state is None else rng_state.data_ptr())
 
     def step(self, step: int, *, lr: float, beta1: float = 0.9, beta2: float = 0.95,
              eps: float = 1e-8, grad_scale: Optional[torch.Tensor] = None,
-             scalars: Optional[torch.Tensor] = None) -> None:
-        """One step (`step` counts from 1) on the current stream.  grad_scale
+             scalars: Optional[torch.Tensor] = None,
+             grads: Optional[Sequence[torch.Tensor]] = None) -> None:
+        """One step (`step` counts from 1) on the current stream.  `grads` take the
+        place of the gradients listed so far (same sizes and type).  grad_scale
         (one float32 on the device) multiplies the gradients; scalars (three
         float32 on the device: lr, 1 - beta1^step, 1 - beta2^step) take the
         place of lr and step in a captured step."""
         _result("nvfp4_adamw_step", load_binding().adamw_step(
-            *self._fixed, lr, beta1, beta2, eps, step, grad_scale, scalars))
+            self._table, lr, beta1, beta2, eps, step, grad_scale, scalars, grads))
 
 
 def adamw_unpack_state(codes: torch.Tensor, scales: torch.Tensor, moment: str,

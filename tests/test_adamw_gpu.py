@@ -334,3 +334,82 @@ def test_refuses_a_tensor_twice(nvlib):
     nvlib.AdamW(p, g, m, v)
     with pytest.raises(ValueError):
         nvlib.AdamW([p[0], p[0]], g, m, v)
+
+
+def listed(nvlib, sizes=(300, 70), seed=21, **kw):
+    """An optimizer with 32-bit moments, copies and amax, and its lists."""
+    cpu = make(list(sizes), torch.float32, torch.float32, seed)
+    lists = [[t.cuda() for t in x] for x in cpu]
+    lists.append([torch.empty(n, dtype=torch.bfloat16, device="cuda") for n in sizes])
+    amax = torch.empty(len(sizes), device="cuda")
+    return nvlib.AdamW(*lists[:4], copies=lists[4], amax_out=amax, **kw), lists, amax
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_a_tensor_with_other_memory_is_refused(nvlib, which):
+    """p.data = ..., set_ and resize_ leave the tensor and take its memory away."""
+    opt, lists, amax = listed(nvlib)
+    t = (lists + [[amax]])[which][-1]
+    opt.step(1, **H)
+    keep = [x.clone() for seq in lists for x in seq]
+    for change in (lambda: t.data.clone(), lambda: t.data[:t.numel() - 1],
+                   lambda: torch.zeros(2 * t.numel(), dtype=t.dtype, device="cuda")[::2]):
+        old = t.data
+        t.data = change()
+        with pytest.raises(ValueError):
+            opt.step(2, **H)
+        t.data = old
+    n = t.numel()
+    t.resize_(5 * n + 4096)
+    with pytest.raises(ValueError):
+        opt.step(2, **H)
+    torch.cuda.synchronize()
+    if which < 5:
+        now = [x.flatten()[:y.numel()] for x, y in zip((x for seq in lists for x in seq), keep)]
+        assert all(torch.equal(x, y) for x, y in zip(now, keep))
+
+
+def test_two_steps_with_new_gradients(nvlib):
+    """Gradients that are new tensors every step give the bits of an optimizer
+    that was made for them; refused ones leave it as it was."""
+    sizes = [300, 70, 0, 4097]
+    opt, lists, amax = listed(nvlib, sizes)
+    same = [[t.clone() for t in seq] for seq in lists]
+    for step in (1, 2, 3):
+        gs = [t.cuda() for t in make(sizes, torch.float32, torch.float32, 60 + step)[1]]
+        opt.step(step, grads=gs, **H)
+        nvlib.AdamW(same[0], gs, same[2], same[3], copies=same[4]).step(step, **H)
+        for bad in (gs[:3], [*gs[:3], gs[3].half()], [*gs[:3], gs[3][:-1]], [*gs[:3], gs[3].cpu()],
+                    [*gs[:3], torch.zeros(2 * 4097, device="cuda")[::2]], [*gs[:3], None]):
+            with pytest.raises(ValueError):
+                opt.step(step, grads=bad, **H)
+        for k in (0, 2, 3, 4):
+            assert all(torch.equal(x, y) for x, y in zip(lists[k], same[k])), (step, k)
+    # without new ones the last are read again
+    opt.step(4, **H)
+    nvlib.AdamW(same[0], gs, same[2], same[3], copies=same[4]).step(4, **H)
+    assert all(torch.equal(x, y) for x, y in zip(lists[0], same[0]))
+
+
+def test_the_usual_loop_does_not_read_old_gradients(nvlib):
+    """backward() after zero_grad(set_to_none=True) makes new .grad tensors."""
+    ps = [torch.randn(n, device="cuda").requires_grad_() for n in (40, 7)]
+    for p in ps:
+        (p * p).sum().backward()
+    zeros = [[torch.zeros(p.numel(), device="cuda") for p in ps] for _ in range(2)]
+    opt = nvlib.AdamW(ps, [p.grad for p in ps], *zeros)
+    opt.step(1, **H)
+    for p in ps:
+        p.grad = None
+    with pytest.raises(ValueError, match="grad"):
+        opt.step(2, **H)
+    for p in ps:
+        (3 * p).sum().backward()
+    with pytest.raises(ValueError, match="grad"):
+        opt.step(2, **H)
+    before = [m.double().cpu() for m in zeros[0]]
+    opt.step(2, grads=[p.grad for p in ps], **H)
+    for m, m0 in zip(zeros[0], before):
+        want = 0.9 * m0 + 0.1 * 3.0
+        close(m, want, 4 * 2.0 ** -24 * (0.9 * m0.abs() + 0.3), "m")
+    opt.step(3, **H)
