@@ -347,11 +347,22 @@ struct Held {
   }
 };
 
+// Memory that a step writes.
+struct Range {
+  uintptr_t begin, end;
+  const char* name;
+};
+Range range_of(const Held& h, const char* name) {
+  const uintptr_t p = (uintptr_t)h.data;
+  return {p, p + (uintptr_t)h.n * c10::elementSize(h.type), name};
+}
+
 struct AdamWTable {
   int device = 0, param = 0, grad = 0, state = 0;
   std::vector<nvfp4_adamw_tensor> rows;
   std::vector<Held> lists[kLists];
   std::vector<Held> words;             // amax_out, rng_state
+  std::vector<Range> written;          // sorted; none overlaps the next
   std::vector<char> follows;           // grads[i] is params[i].grad
   float* amax = nullptr;
   const size_t* rng = nullptr;
@@ -390,6 +401,23 @@ void on_device(const std::vector<Held>& list, int device, const char* name) {
     TORCH_CHECK_VALUE(list[i].tensor.is_cuda() && list[i].tensor.get_device() == device, name, "[",
                       i, "]: not on the parameters' device");
 }
+// Sorts what a step writes: two blocks would write an overlap at once.
+void sort_written(std::vector<Range>& w) {
+  std::sort(w.begin(), w.end(),
+            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < w.size(); ++i)
+    TORCH_CHECK_VALUE(w[i - 1].end <= w[i].begin, w[i - 1].name, " and ", w[i].name,
+                      ": tensors that the step writes overlap (the same tensor twice?)");
+}
+// Refuses memory to be read that the step writes.
+void apart(const std::vector<Range>& written, const Range& r) {
+  const auto next = std::lower_bound(
+      written.begin(), written.end(), r.end,
+      [](const Range& a, uintptr_t end) { return a.begin < end; });
+  TORCH_CHECK_VALUE(r.begin == r.end || next == written.begin() || (next - 1)->end <= r.begin,
+                    r.name, " and ", (next - 1)->name,
+                    ": a tensor that the step reads overlaps one that it writes");
+}
 // Which gradients are their parameters' own .grad.
 void see_whose(AdamWTable& t) {
   t.follows.resize(t.rows.size());
@@ -399,6 +427,7 @@ void see_whose(AdamWTable& t) {
   }
 }
 void put_grads(AdamWTable& t, std::vector<Held>&& grads) {
+  for (const Held& g : grads) apart(t.written, range_of(g, kListName[kGrads]));
   on_device(grads, t.device, kListName[kGrads]);
   t.lists[kGrads] = std::move(grads);
   for (size_t i = 0; i < t.rows.size(); ++i) t.rows[i].grad = t.lists[kGrads][i].data;
@@ -445,17 +474,25 @@ PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   if (o[kCopies] != Py_None)
     t->lists[kCopies] = held(o[kCopies], tensors, ScalarType::BFloat16, kCopies, size);
 
+  if (o[9] != Py_None) t->words.emplace_back(tensor(o[9], "amax_out"));
+  for (int list = 0; list < kLists; ++list)
+    for (const Held& h : t->lists[list])
+      if (h.n) t->written.push_back(range_of(h, kListName[list]));
+  for (const Held& h : t->words) t->written.push_back(range_of(h, "amax_out"));
+  sort_written(t->written);
+  if (o[10] != Py_None) {
+    t->words.emplace_back(tensor(o[10], "rng_state"));
+    apart(t->written, range_of(t->words.back(), "rng_state"));
+    t->rng = (const size_t*)t->words.back().data;
+  }
+  for (const Held& g : grads) apart(t->written, range_of(g, kListName[kGrads]));
+
   const Tensor& first_param = t->lists[kParams][0].tensor;
   TORCH_CHECK_VALUE(first_param.is_cuda(), "params: expected CUDA tensors");
   t->device = (int)first_param.get_device();
   for (int list = 0; list < kLists; ++list)
     on_device(t->lists[list], t->device, kListName[list]);
   t->amax = words(o[9], tensors, t->device, "amax_out");
-  if (o[9] != Py_None) t->words.emplace_back(tensor(o[9], "amax_out"));
-  if (o[10] != Py_None) {
-    t->words.emplace_back(tensor(o[10], "rng_state"));
-    t->rng = (const size_t*)t->words.back().data;
-  }
 
   THPObjectPtr decays(o[7] == Py_None ? nullptr : PySequence_Fast(o[7], "weight_decays"));
   THPObjectPtr offsets(o[8] == Py_None ? nullptr : PySequence_Fast(o[8], "offsets"));
@@ -476,12 +513,6 @@ PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     r.offset = offsets ? (uint64_t)integer(PySequence_Fast_GET_ITEM(offsets.get(), i)) : next;
     next += (uint64_t)(blocks(i) * kStateBlock);
   }
-  std::vector<const void*> own;
-  for (const Held& h : t->lists[kParams])
-    if (h.n) own.push_back(h.data);
-  std::sort(own.begin(), own.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(own.begin(), own.end()) == own.end(),
-                    "params: the same tensor twice");
   put_grads(*t, std::move(grads));
   PyObject* capsule = PyCapsule_New(t.get(), kTableName, [](PyObject* c) {
     delete static_cast<AdamWTable*>(PyCapsule_GetPointer(c, kTableName));
@@ -501,6 +532,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   const int64_t step = integer(o[5]);
   const float *scale = words(o[6], 1, t.device, "grad_scale"),
               *scalars = words(o[7], 3, t.device, "scalars");
+  if (scale) apart(t.written, {(uintptr_t)scale, (uintptr_t)(scale + 1), "grad_scale"});
+  if (scalars) apart(t.written, {(uintptr_t)scalars, (uintptr_t)(scalars + 3), "scalars"});
   for (const Held& w : t.words)
     TORCH_CHECK_VALUE(w.same(), "amax_out, rng_state: the tensor has other memory now");
   for (int list = 0; list < kLists; ++list) {

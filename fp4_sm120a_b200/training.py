@@ -90,7 +90,8 @@ class AdamW:
     `copies` (bfloat16) receive the rounded new parameters, `amax_out` (one
     float32 per tensor) their amax.  All memory is the caller's.
 
-    The tensors are held, and every step looks whether each still has the memory
+    What a step writes must not overlap, nor what it reads lie in it.  The tensors
+    are held, and every step looks whether each still has the memory
     it had (after `p.data = ...`, set_ or resize_ it has not: ValueError).
     Gradients that are new tensors are passed to step, which then uses them until
     it gets others; a gradient that was its parameter's .grad when it was listed

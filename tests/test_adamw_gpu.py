@@ -413,3 +413,13 @@ def test_the_usual_loop_does_not_read_old_gradients(nvlib):
         want = 0.9 * m0 + 0.1 * 3.0
         close(m, want, 4 * 2.0 ** -24 * (0.9 * m0.abs() + 0.3), "m")
     opt.step(3, **H)
+
+
+def test_refuses_scalars_and_gradients_in_what_it_writes(nvlib):
+    """amax_out is cleared, and parameters change, before they would be read."""
+    opt, lists, amax = listed(nvlib)
+    for kw in (dict(grad_scale=amax[1:]), dict(scalars=lists[0][0][5:8]), dict(grads=lists[2]),
+               dict(grads=[lists[1][0], lists[0][0][:70]])):
+        with pytest.raises(ValueError, match="overlap"):
+            opt.step(1, **H, **kw)
+    opt.step(1, **H)

@@ -195,3 +195,63 @@ def test_adamw_refuses_a_strided_rng_state(nvlib, rng):
     s = torch.zeros(1, dtype=torch.uint8)
     with pytest.raises(ValueError, match="rng_state"):
         nvlib.AdamW([w], [w], [u], [u], exp_avg_scales=[s], exp_avg_sq_scales=[s], rng_state=rng)
+
+
+def adamw_lists():
+    z = lambda n=200, t=torch.float32: [torch.zeros(n, dtype=t) for _ in range(2)]  # noqa: E731
+    return dict(params=z(), grads=z(), exp_avgs=z(t=torch.uint8), exp_avg_sqs=z(t=torch.uint8),
+                exp_avg_scales=z(2, torch.uint8), exp_avg_sq_scales=z(2, torch.uint8),
+                copies=z(t=torch.bfloat16), amax_out=torch.zeros(2),
+                rng_state=torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("name", ["params", "exp_avgs", "exp_avg_sqs", "exp_avg_scales",
+                                  "exp_avg_sq_scales", "copies"])
+@pytest.mark.parametrize("how", ["twice", "views", "bytes"])
+def test_adamw_refuses_lists_that_overlap(nvlib, name, how):
+    """Two blocks would write the same memory at once."""
+    a = adamw_lists()
+    n, t = a[name][0].numel(), a[name][0].dtype
+    flat = torch.zeros(2 * n, dtype=t)
+    if how == "twice":
+        a[name] = [flat[:n]] * 2
+    elif how == "views":
+        a[name] = [flat[:n], flat[n - 1:2 * n - 1]]
+    else:                                     # one list's memory in another list
+        other = "exp_avgs" if name != "exp_avgs" else "copies"
+        raw = torch.zeros(max(n, 200) * 4, dtype=torch.uint8)
+        a[name] = [raw[:n * t.itemsize].view(t), flat[:n]]
+        u = a[other][0]
+        a[other] = [raw[:200 * u.dtype.itemsize].view(u.dtype), a[other][1]]
+    lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
+    with pytest.raises(ValueError, match="overlap|twice"):
+        nvlib.AdamW(*lists, **a)
+
+
+@pytest.mark.parametrize("name", ["grads", "rng_state", "amax_out"])
+def test_adamw_refuses_what_it_reads_in_what_it_writes(nvlib, name):
+    a = adamw_lists()
+    if name == "grads":
+        a["grads"] = a["params"]
+    elif name == "rng_state":
+        raw = torch.zeros(200, dtype=torch.uint8)
+        a["exp_avgs"], a["rng_state"] = [raw, a["exp_avgs"][1]], raw[8:24].view(torch.int64)
+    else:
+        a["amax_out"] = a["params"][1][4:6]
+    lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
+    with pytest.raises(ValueError, match="overlap"):
+        nvlib.AdamW(*lists, **a)
+
+
+def test_adamw_lists_side_by_side_are_no_overlap(nvlib):
+    """What is left to refuse is the device."""
+    a = adamw_lists()
+    flat = torch.zeros(400)
+    a["params"] = [flat[:200], flat[200:]]
+    a["exp_avgs"][0] = a["exp_avgs"][0][:0]
+    a["params"][0] = a["params"][0][:0]
+    for k in ("grads", "exp_avg_sqs", "exp_avg_scales", "exp_avg_sq_scales", "copies"):
+        a[k][0] = a[k][0][:0]
+    lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
+    with pytest.raises(ValueError, match="CUDA"):
+        nvlib.AdamW(*lists, **a)
