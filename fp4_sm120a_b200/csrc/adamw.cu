@@ -501,6 +501,11 @@ NVFP4_API int nvfp4_adamw_step(const nvfp4_adamw_tensor* tensors, int count, int
   if ((uintptr_t)grad_scale % 4 || (uintptr_t)scalars % 4 || (uintptr_t)amax_out % 4 ||
       (uintptr_t)rng_state % 8)
     return NVFP4_ERR_MISALIGNED;
+  // amax_out is cleared before the scalars are read.
+  auto in_amax = [&](const float* p, int words) {
+    return amax_out && p && p < amax_out + count && p + words > amax_out;
+  };
+  if (in_amax(grad_scale, 1) || in_amax(scalars, 3)) return NVFP4_ERR_INVALID_ARGUMENT;
   const uintptr_t psize = param_dtype == NVFP4_DTYPE_F32 ? 4 : 2;
   const uintptr_t gsize = grad_dtype == NVFP4_DTYPE_F32 ? 4 : 2;
   const uintptr_t ssize = eight ? 1 : 4;

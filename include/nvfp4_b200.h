@@ -389,7 +389,8 @@ typedef struct nvfp4_adamw_tensor {
  * 1 / (1 - beta2) steps: with beta2 <= 0.98 the standard deviation of
  * exp_avg_sq stays below 10 %; for longer memories take fp32.
  * amax_out (NULL or `count` floats): max |p| of each tensor rounded to bf16,
- * NaN-propagating: what the cast of the new weights needs.
+ * NaN-propagating: what the cast of the new weights needs.  It is cleared first,
+ * so grad_scale and scalars must not lie in it.
  * count == 0 and tensors with n == 0 are skipped.  The tensors of one call
  * must not overlap. */
 NVFP4_API int nvfp4_adamw_step(const nvfp4_adamw_tensor* tensors, int count, int param_dtype,

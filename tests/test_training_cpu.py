@@ -255,3 +255,18 @@ def test_adamw_lists_side_by_side_are_no_overlap(nvlib):
     lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
     with pytest.raises(ValueError, match="CUDA"):
         nvlib.AdamW(*lists, **a)
+
+
+def test_adamw_step_refuses_scalars_in_its_amax(nvlib):
+    """amax_out is cleared before grad_scale and scalars are read."""
+    from fp4_sm120a_b200._native import AdamWTensor
+    lib = nvlib.load()
+    arr = (AdamWTensor * 3)(*[AdamWTensor(param=P, grad=P, exp_avg=P, exp_avg_sq=P, n=0)] * 3)
+
+    def step(scale=None, scalars=None):
+        return lib.nvfp4_adamw_step(arr, 3, 0, 0, 0, 0.1, 0.9, 0.95, 1e-8, 1, scale, scalars, P,
+                                    None, None)
+    for word in (P, P + 8):
+        assert step(scale=word) == ARG
+    for words in (P - 8, P, P + 8):
+        assert step(scalars=words) == ARG
