@@ -132,11 +132,15 @@ class AdamW:
                                       or rng_state.device != self.device):
             raise ValueError("rng_state: expected contiguous int64 {seed, offset} on the "
                              "parameters' device")
+        if offsets is not None:
+            offsets = [int(x) for x in offsets]
+            if any(x < 0 or x >= 2 ** 62 or (self.eight and x % STATE_BLOCK) for x in offsets):
+                raise ValueError(f"offsets: expected multiples of {STATE_BLOCK} from 0 on")
         self._table = load_binding().adamw_table(
             params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales if self.eight else None,
             exp_avg_sq_scales if self.eight else None, copies,
             None if weight_decays is None else [float(d) for d in weight_decays],
-            None if offsets is None else [int(x) for x in offsets], amax_out, rng_state)
+            offsets, amax_out, rng_state)
         self.count = count
 
     def step(self, step: int, *, lr: float, beta1: float = 0.9, beta2: float = 0.95,

@@ -270,3 +270,12 @@ def test_adamw_step_refuses_scalars_in_its_amax(nvlib):
         assert step(scale=word) == ARG
     for words in (P - 8, P, P + 8):
         assert step(scalars=words) == ARG
+
+
+@pytest.mark.parametrize("offsets", [[0, -128], [0, 200], [-2**63, 0], [0, 2**63]])
+def test_adamw_refuses_offsets_that_are_no_places(nvlib, offsets):
+    """Random bits are numbered from 0 on, in blocks of 128."""
+    a = adamw_lists()
+    lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
+    with pytest.raises(ValueError, match="offsets"):
+        nvlib.AdamW(*lists, offsets=offsets, **a)
