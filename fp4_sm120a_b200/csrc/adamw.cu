@@ -44,6 +44,7 @@ constexpr int kVec = 4;                              // elements a thread takes 
 constexpr int kUnroll = 4;
 constexpr uint32_t kChunk = kThreads * kVec * kUnroll;  // elements per thread block
 constexpr int kStateBlock = 128;                     // = 32 lanes x kVec: one warp's share
+constexpr uint32_t kTopScale = 247;                  // of a block of finite values
 static_assert(kStateBlock == 32 * kVec, "a warp holds whole state blocks");
 
 struct Tensor {
@@ -271,13 +272,18 @@ __device__ __forceinline__ uint32_t adamw_chunk(const Args<CAP>& a, const Tensor
       }
       uint32_t om = top_bytes(bm[0], bm[1], bm[2], bm[3]);
       uint32_t ov = top_bytes(bv[0], bv[1], bv[2], bv[3]);
-      if (sm == 255u) {
-        // No code has a value here; the signs stay.
-        om = 0u;
+      // Under the largest scale the code of 256 stands for 2^128, which is not
+      // finite: the code below takes its place.
+      if (sm >= kTopScale) {
+        om = (om & 0x80808080u) | __vminu4(om & 0x7F7F7F7Fu, 0x77777777u);
+        if (sm == 255u) {
+          // No code has a value here; the signs stay.
+          om = 0u;
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) om |= mu[k] < 0.0f ? 0x80u << (8 * k) : 0u;
+          for (int k = 0; k < kVec; ++k) om |= mu[k] < 0.0f ? 0x80u << (8 * k) : 0u;
+        }
       }
-      if (sv == 255u) ov = 0u;
+      if (sv >= kTopScale) ov = sv == 255u ? 0u : __vminu4(ov, 0xEFEFEFEFu);
       store4_bytes(reinterpret_cast<uint8_t*>(t.m), i, n, full, om);
       store4_bytes(reinterpret_cast<uint8_t*>(t.v), i, n, full, ov);
       if ((threadIdx.x & 31) == 0 && (FULL || i < n)) {

@@ -423,3 +423,46 @@ def test_refuses_scalars_and_gradients_in_what_it_writes(nvlib):
         with pytest.raises(ValueError, match="overlap"):
             opt.step(1, **H, **kw)
     opt.step(1, **H)
+
+
+@pytest.mark.parametrize("moment", ["exp_avg", "exp_avg_sq"])
+def test_8_bit_moments_at_the_top_of_fp32_stay_finite(nvlib, moment):
+    """Values whose next code would stand for 2^128: 256 codes of the largest scale
+    that a block gets take the code below it."""
+    n = 512
+    value = 3.39e38 if moment == "exp_avg" else math.sqrt(3.39e38)
+    g = torch.full((n,), value, device="cuda")
+    g[::3] *= -1
+    p = torch.zeros(n, device="cuda")
+    (m, ms), (v, vs) = zeros8([n]), zeros8([n])
+    opt = nvlib.AdamW([p], [g], m, v, exp_avg_scales=ms, exp_avg_sq_scales=vs,
+                      rng_state=torch.tensor([5, 0], device="cuda"))
+    opt.step(1, lr=1e-3, beta1=0.0, beta2=0.0)
+    codes, scales, largest = (m, ms, 240.0) if moment == "exp_avg" else (v, vs, 248.0)
+    got = nvlib.adamw_unpack_state(codes[0], scales[0], moment, torch.float32)
+    sign = g.sign() if moment == "exp_avg" else torch.ones_like(g)
+    assert bool((scales[0] == 247).all())
+    assert torch.equal(got, sign * torch.tensor(largest * 2.0 ** 120, device="cuda"))
+    # and the next step reads them: half of what was held, nothing new
+    g.zero_()
+    opt.step(2, lr=1e-3, beta1=0.5, beta2=0.5)
+    again = nvlib.adamw_unpack_state(codes[0], scales[0], moment, torch.float32)
+    assert torch.equal(again, got / 2)
+
+
+@pytest.mark.parametrize("moment", ["exp_avg", "exp_avg_sq"])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_unpack_large_scales(nvlib, moment, shift):
+    """All codes under scales up to the largest finite one; a value above fp32's
+    range is infinite."""
+    tops = torch.tensor([126, 128, 200, 238, 239, 240, 246, 247, 248, 254], dtype=torch.uint8)
+    scales = tops.repeat_interleave(2)
+    raw = (torch.arange(scales.numel() * 128 + shift) % 256).to(torch.uint8)
+    if moment == "exp_avg":
+        raw[(raw & 127) == 127] = 0
+    codes = raw.cuda()[shift:]
+    want = orc.unpack8(codes.cpu(), scales, moment).float()
+    got = nvlib.adamw_unpack_state(codes, scales.cuda(), moment, torch.float32).cpu()
+    assert torch.equal(got, want)
+    b16 = nvlib.adamw_unpack_state(codes, scales.cuda(), moment).cpu()
+    assert torch.equal(b16, want.to(torch.bfloat16))
