@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <limits>
 #include <memory>
 #include <utility>
 #include <vector>
@@ -282,6 +283,11 @@ PyObject* layernorm(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   float* amax = words(o[4], 1, device, "amax_out");
   const Tensor y = empty({a.rows, a.cols}, a.type, device);
   const Tensor mean = empty({a.rows}, kF32, device), rstd = empty({a.rows}, kF32, device);
+  if (a.cols == 0) {
+    // Statistics of nothing, which the library leaves as they are.
+    const c10::cuda::CUDAGuard guard(device);
+    for (const Tensor& t : {mean, rstd}) t.fill_(std::numeric_limits<float>::quiet_NaN());
+  }
   const int status = launch(device, [&](nvfp4_stream_t stream) {
     return nvfp4_layernorm_fwd(a.rows, a.cols, a.x, a.ldx, a.gamma, beta, a.code, a.weight, eps,
                                y.data_ptr(), a.cols, (float*)mean.data_ptr(),

@@ -318,3 +318,16 @@ def test_mean_of_rows_with_an_offset(nvlib, cols, offset):
     g, h = gamma.double().abs(), spread * wr[:, None]
     close(y, wy, g * ((wr * em)[:, None] + 64 * 2.0 ** -22 * h) + 2.0 ** -22 * beta.double().abs()
           + 2.0 ** -23 * wy.abs(), "y")
+
+
+def test_rows_without_columns(nvlib):
+    """Nothing has no mean: NaN, not what the memory held."""
+    rows = 1000
+    for _ in range(3):
+        torch.full((rows,), 5.0, device="cuda")      # freed at once: the next ones' memory
+    x, w = torch.empty(rows, 0, device="cuda"), torch.empty(0, device="cuda")
+    y, mean, rstd = nvlib.layernorm(x, w)
+    assert y.shape == (rows, 0)
+    assert bool(torch.isnan(mean).all()) and bool(torch.isnan(rstd).all())
+    dx, dg, db = nvlib.layernorm_backward(x, x, mean, rstd, w)
+    assert dx.shape == (rows, 0) and dg.numel() == db.numel() == 0
