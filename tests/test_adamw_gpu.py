@@ -466,3 +466,43 @@ def test_unpack_large_scales(nvlib, moment, shift):
     assert torch.equal(got, want)
     b16 = nvlib.adamw_unpack_state(codes, scales.cuda(), moment).cpu()
     assert torch.equal(b16, want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("sizes", [[1], [4, 300, 127, 4096 + 37], [513] * 40])
+@pytest.mark.parametrize("param,grad", [("bf16", "bf16"), ("bf16", "f16"), ("bf16", "f32"),
+                                        ("f32", "f16")])
+def test_8_bit_moments_of_all_types(nvlib, sizes, param, grad):
+    """The same as in fp32: two steps, codes and scales bit for bit."""
+    ps = make(sizes, TYPES[param], TYPES[grad], 31)[0]
+    dp, dg = [p.cuda() for p in ps], [torch.empty(n, dtype=TYPES[grad], device="cuda")
+                                      for n in sizes]
+    (dm, ms), (dv, vs) = zeros8(sizes), zeros8(sizes)
+    copies = ([torch.empty(n, dtype=torch.bfloat16, device="cuda") for n in sizes]
+              if param == "f32" else None)
+    amax, rng = torch.empty(len(sizes), device="cuda"), torch.tensor([99, 7], device="cuda")
+    wds = [0.1 * (i % 2) for i in range(len(sizes))]
+    opt = nvlib.AdamW(dp, dg, dm, dv, exp_avg_scales=ms, exp_avg_sq_scales=vs, copies=copies,
+                      amax_out=amax, rng_state=rng, weight_decays=wds)
+    for step in (1, 2):
+        gs = make(sizes, TYPES[param], TYPES[grad], 200 + step)[1]
+        for d, g in zip(dg, gs):
+            d.copy_(g)
+        before = [(p.cpu(), orc.unpack8(m.cpu(), s.cpu(), "exp_avg"),
+                   orc.unpack8(v.cpu(), t.cpu(), "exp_avg_sq"))
+                  for p, m, s, v, t in zip(dp, dm, ms, dv, vs)]
+        opt.step(step, **H)
+        torch.cuda.synchronize()
+        at = 0
+        for i, n in enumerate(sizes):
+            p0, m0, v0 = before[i]
+            g = f32(gs[i])
+            m = f32(m0) * torch.tensor(0.9) + g * torch.tensor(1 - 0.9)
+            v = f32(v0) * torch.tensor(0.95) + (g * g) * torch.tensor(1 - 0.95)
+            lo, hi = moment_words(n, at, 99, 7 + step)
+            for x, words, kind, codes, scales in ((m, lo, "exp_avg", dm, ms),
+                                                  (v, hi, "exp_avg_sq", dv, vs)):
+                code, scale = expect8(x, kind, words)
+                assert torch.equal(scales[i].cpu(), scale) and torch.equal(codes[i].cpu(), code)
+            want, _, wv = orc.adamw(p0, g, m0, v0, step=step, wd=wds[i], **H)
+            check_param(dp[i], p0, g, m0, wv, step, want, copies, amax, i)
+            at += -(-n // 128) * 128

@@ -334,3 +334,10 @@ def test_repeats_and_sm_cap(nvlib, m, n, k):
     torch.cuda.synchronize()
     assert torch.equal(gd, new) and torch.equal(gb, nb2)
     assert nvlib.device_error() == 0
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 512), (40, 300, 2048), (333, 514, 256),
+                                   (2500, 2177, 96), (1030, 1800, 64), (130, 200, 4096)])
+def test_backward_epilogue_in_f16(nvlib, m, n, k, act):
+    test_backward_epilogue(nvlib, m, n, k, "f16", act)

@@ -331,3 +331,39 @@ def test_rows_without_columns(nvlib):
     assert bool(torch.isnan(mean).all()) and bool(torch.isnan(rstd).all())
     dx, dg, db = nvlib.layernorm_backward(x, x, mean, rstd, w)
     assert dx.shape == (rows, 0) and dg.numel() == db.numel() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,pad", [(8300, 1011, 0), (4100, 2050, 1), (1100, 8190, 3)])
+def test_unaligned_rows_with_16_bit_weights(nvlib, rows, cols, pad, dtype):
+    """Enough elements for the backward pass by vectors with partial ends."""
+    x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], TYPES[dtype], rows - cols)
+
+    def place(t):
+        flat = torch.zeros(rows * (cols + pad) + 8, dtype=t.dtype, device="cuda")
+        v = flat[1:1 + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        v.copy_(t)
+        return v
+    xd, dyd, rd = place(x), place(dy), place(res)
+    mean, rstd = check_forward(nvlib, x, gamma, beta, xd)
+    # dx is a tensor of its own: the phases agree where its rows are as long as x's
+    check_backward(nvlib, x, gamma, dy, res, mean, rstd, (xd, dyd, rd))
+    check_backward(nvlib, x, gamma, dy, None, mean, rstd, (xd, dyd, None))
+    # and over dy, whose rows start where x's do
+    dx, dg, db = nvlib.layernorm_backward(dyd, xd, mean, rstd, gamma.cuda(), residual=rd)
+    ws = torch.empty(nvlib.layernorm_bwd_workspace_bytes(rows, cols), dtype=torch.uint8,
+                     device="cuda")
+    dg2, db2, ld = torch.empty_like(dg), torch.empty_like(db), cols + pad
+    nvlib.layernorm_bwd(rows, cols, dyd, ld, xd, ld, mean, rstd, gamma.cuda(), rd, ld, x.dtype,
+                        gamma.dtype, dyd, ld, dg2, db2, ws, ws.numel())
+    wdx, wdg, wdb = orc.layernorm_backward(dy, x, mean.cpu(), rstd.cpu(), gamma, res)
+    m, r = mean.double().cpu()[:, None], rstd.double().cpu()[:, None]
+    h, L = (x.double() - m) * r, max(32, cols // 256) + 16
+    u = (dy.double() * gamma.double()).abs()
+    part = r * (u + u.mean(1, keepdim=True) + h.abs() * (u * h.abs()).mean(1, keepdim=True))
+    close(dyd, wdx, L * 2.0 ** -22 * part + 2.0 ** -23 * res.double().abs()
+          + orc.half_step(x.dtype) * wdx.abs() + orc.least_step(x.dtype), "dx over dy")
+    for got, want, t in ((dg2, wdg, (dy.double() * h).abs()), (db2, wdb, dy.double().abs())):
+        close(got, want, ((rows + 64) * 2.0 ** -24 + 2.0 ** -22) * t.sum(0)
+              + orc.half_step(gamma.dtype) * want.abs() + orc.least_step(gamma.dtype), "weights")
+    assert nvlib.device_error() == 0
