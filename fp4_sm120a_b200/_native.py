@@ -6,13 +6,13 @@ if the library is missing or fails to load, every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from ctypes import (c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p,
                     POINTER)
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnvfp4_b200.so"
-BINDING_PATH = LIB_PATH.with_name("_torch_binding.so")
 
 
 class AdamWTensor(ctypes.Structure):
@@ -139,11 +139,16 @@ def load_binding():
     global _binding
     if _binding is None:
         load()
-        if not BINDING_PATH.exists():
-            raise ImportError(f"{BINDING_PATH.name} is not built; run "
-                              "`python -m fp4_sm120a_b200.build`")
-        from . import _torch_binding
-        _binding = _torch_binding
+        from .build import binding_path
+        path = binding_path()
+        if path is None or not path.exists():
+            raise ImportError(f"{path.name if path else 'the tensor-level binding'} is not "
+                              "built; run `python -m fp4_sm120a_b200.build`")
+        name = f"{__package__}._torch_binding"
+        spec = importlib.util.spec_from_file_location(name, path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
     return _binding
 
 

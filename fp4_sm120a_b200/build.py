@@ -1,9 +1,11 @@
 """Build the in-tree CUDA library libnvfp4_b200.so for sm_100a with nvcc, and the
-tensor-level binding _torch_binding.so against torch's headers with the host
+tensor-level binding _torch_binding.*.so against torch's headers with the host
 compiler.
 
 Both are built next to this file so that they travel with the source
-tree; nothing is installed into site-packages.
+tree; nothing is installed into site-packages.  The library needs nvcc alone
+(`python fp4_sm120a_b200/build.py` imports no package): where the binding cannot be
+built, for want of torch, its headers or g++, the library is there all the same.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
@@ -20,7 +23,6 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libnvfp4_b200.so"
 OBJDIR = PKG / "_build"
-BINDING = PKG / "_torch_binding.so"
 BINDING_SOURCE = CSRC / "torch_binding.cpp"
 
 # The system's compiler, whatever CXX says: the binding must share torch's
@@ -52,8 +54,19 @@ def _binding_deps() -> list[Path]:
     return [BINDING_SOURCE, INCLUDE / "nvfp4_b200.h"]
 
 
+def binding_path() -> Optional[Path]:
+    """The binding's file, named by the Python and the torch it is built against and
+    for (under others it is another file); None without torch."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    return PKG / f"_torch_binding.{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}.so"
+
+
 def needs_build() -> bool:
-    return _stale(LIB, _deps()) or _stale(BINDING, _binding_deps())
+    binding = binding_path()
+    return _stale(LIB, _deps()) or (binding is not None and _stale(binding, _binding_deps()))
 
 
 def _run(cmd: list[str], what: str, verbose: bool = False) -> None:
@@ -64,11 +77,11 @@ def _run(cmd: list[str], what: str, verbose: bool = False) -> None:
         raise RuntimeError(f"{what} failed")
 
 
-def _build_binding(verbose: bool) -> None:
+def _build_binding(binding: Path, verbose: bool) -> None:
     """Needs LIB: the binding links against it (found beside it at run time)."""
     import torch
     root = Path(torch.__file__).resolve().parent
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     _run([CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
@@ -77,7 +90,7 @@ def _build_binding(verbose: bool) -> None:
           "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
           "-ltorch", "-lc10_cuda", "-lc10", f"-L{PKG}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"],
          "building the torch binding", verbose)
-    os.replace(tmp, BINDING)
+    os.replace(tmp, binding)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -101,8 +114,16 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         _run([NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", *objs, "-o",
               str(tmp)], "link")
         os.replace(tmp, LIB)
-    if force or _stale(BINDING, _binding_deps()):
-        _build_binding(verbose)
+    binding = binding_path()
+    if binding is None:
+        sys.stderr.write("no torch: the tensor-level binding is not built\n")
+    elif force or _stale(binding, _binding_deps()):
+        # An old file would be imported as it is; the tensor-level calls raise without one.
+        binding.unlink(missing_ok=True)
+        try:
+            _build_binding(binding, verbose)
+        except (RuntimeError, OSError) as e:
+            sys.stderr.write(f"the tensor-level binding is not built: {e}\n")
     return LIB
 
 
