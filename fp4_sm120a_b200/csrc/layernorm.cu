@@ -163,10 +163,9 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
 
 // A row's bytes in whole 16-byte units, which is what bulk copies move.  The first
 // and last unit of an unaligned row hold its neighbours' bytes too: they are read
-// (an aligned unit lies within one allocation) and left unused, whatever is being
-// written to them meanwhile.  Loading the row's share of them apart, a row ahead,
-// made the first warp late for every barrier (fp32 backward 10000 x 4097: 151 us
-// against 102).
+// and left unused, whatever is being written to them meanwhile.  Loading the row's
+// share of them apart, a row ahead, made the first warp late for every barrier (fp32
+// backward 10000 x 4097: 151 us against 102).
 template <int MODE>
 __device__ __forceinline__ uint32_t span_bytes(const void* row, uint32_t row_bytes) {
   if constexpr (MODE == kWhole) return row_bytes;
@@ -177,6 +176,38 @@ __device__ __forceinline__ void span_load(uint32_t slot, const void* row, uint32
                                           uint32_t bar) {
   bulk_load(slot, reinterpret_cast<const void*>((uintptr_t)row & ~(uintptr_t)15),
             span_bytes<MODE>(row, row_bytes), bar);
+}
+// Only the unit before the first row's start and the one behind the last row's end
+// reach outside the caller's rows.  Those two rows are edges: their copies leave such
+// units out (`lo`, `bytes`: of the row's whole units), and put_edges adds the elements
+// in them.
+struct Span {
+  uint32_t lo, bytes;
+};
+__device__ __forceinline__ Span edge_span(const void* row, uint32_t row_bytes, bool first,
+                                          bool last) {
+  const uint32_t lead = (uint32_t)(uintptr_t)row & 15u, end = lead + row_bytes;
+  const uint32_t lo = first && lead ? 16u : 0u, hi = (last ? end : end + 15u) & ~15u;
+  return {lo, hi > lo ? hi - lo : 0u};
+}
+__device__ __forceinline__ void edge_load(uint32_t slot, const void* row, const Span& s,
+                                          uint32_t bar) {
+  if (s.bytes)
+    bulk_load(slot + s.lo,
+              reinterpret_cast<const unsigned char*>((uintptr_t)row & ~(uintptr_t)15) + s.lo,
+              s.bytes, bar);
+}
+// The elements that an edge's copy leaves out, by the lanes of a warp, into the slot
+// whose other bytes the copy fills.
+template <typename T>
+__device__ __forceinline__ void put_edges(unsigned char* slot, const T* row, int cols, bool first,
+                                          bool last) {
+  constexpr int kUnit = 16 / (int)sizeof(T);
+  const int lead = (int)((uintptr_t)row & 15u) / (int)sizeof(T), lane = (int)threadIdx.x & 31;
+  const int head = first && lead ? min(kUnit - lead, cols) : 0;
+  const int tail = last ? min((lead + cols) % kUnit, cols) : 0;
+  const int l = lane & 15, c = lane < 16 ? l : cols - tail + l;
+  if (l < (lane < 16 ? head : tail)) reinterpret_cast<T*>(slot)[lead + c] = row[c];
 }
 // A thread's items (vectors or elements) within the row: the first `count`.
 template <typename T, int MODE, int ITEMS>
@@ -315,7 +346,8 @@ struct Shared {
   uint64_t bar[kMaxStages];
   float2 red[2][32];
   uint32_t abort_flag;
-  uint32_t pad[3];
+  int last;               // which of this block's rows is the last of all (-1: none)
+  uint32_t pad[2];
 };
 
 // Position of a row in the ring: its stage and the parity its barrier completes
@@ -375,16 +407,30 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   ring.stages = a.stages;
   const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
   auto row_at = [&](int64_t k) { return (int64_t)blockIdx.x + k * gridDim.x; };
-  auto issue = [&](int64_t k, uint32_t stage) {
+  // Which of this block's rows is the last of all (-1: none): in a register where
+  // there is one to spare.
+  const int own_last =
+      blockIdx.x + (int64_t)(mine - 1) * gridDim.x == a.rows - 1 ? (int)(mine - 1) : -1;
+  auto last_row = [&] { return MODE == kOdd ? own_last : sh.last; };
+  auto is_edge = [&](int k) { return (blockIdx.x | k) == 0 || k == last_row(); };
+  auto issue = [&](int k, uint32_t stage) {
     const T* row = x + row_at(k) * a.ldx;
-    mbar_arrive_expect_tx(ring.bar + 8 * stage, span_bytes<MODE>(row, row_bytes));
-    span_load<MODE>(ring.base + stage * ring.stage_bytes, row, row_bytes, ring.bar + 8 * stage);
+    const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
+    if (MODE != kWhole && is_edge(k)) {
+      const Span span = edge_span(row, row_bytes, (blockIdx.x | k) == 0, k == last_row());
+      mbar_arrive_expect_tx(bar, span.bytes);
+      edge_load(dst, row, span, bar);
+      return;
+    }
+    mbar_arrive_expect_tx(bar, span_bytes<MODE>(row, row_bytes));
+    span_load<MODE>(dst, row, row_bytes, bar);
   };
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
+    sh.last = own_last;
     fence_barrier_init();
-    for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
+    for (int k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   const W* wb = reinterpret_cast<const W*>(a.beta);
@@ -420,6 +466,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   RingAt at;
   for (; k < mine; ++k, at.next(ring)) {
     const int64_t row = row_at(k);
+    if (MODE != kWhole && is_edge(k)) {
+      const bool first = row == 0, last = k == last_row();
+      if (warp == 0)
+        put_edges(smem + at.stage * ring.stage_bytes, x + row * a.ldx, a.cols, first, last);
+      __syncthreads();
+    }
     float f[E];
     if (ring_wait(ring, at, &sh.abort_flag)) {
       fetch<T, MODE, ITEMS>(my, smem + at.stage * ring.stage_bytes, x + row * a.ldx, f);
@@ -523,18 +575,20 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
 // afterwards: the error of a sum of a long row does not grow with its length.
 template <typename F>
 __device__ __forceinline__ float2 wide_sums(int cols, const F& f) {
-  constexpr int kRun = 32;
+  constexpr int kRun = 32, kStep = kRun * kWideThreads;
   float a = 0.0f, b = 0.0f;
   int c = threadIdx.x;
-  while (c < cols) {
+  for (; c < cols - (kStep - kWideThreads); c += kStep) {
     float ra = 0.0f, rb = 0.0f;
-    const int end = min(c + kRun * kWideThreads, cols);
-#pragma unroll 8
-    for (; c < end; c += kWideThreads) f(c, ra, rb);
+#pragma unroll 16
+    for (int j = 0; j < kRun; ++j) f(c + j * kWideThreads, ra, rb);
     a += ra;
     b += rb;
   }
-  return make_float2(warp_sum(a), warp_sum(b));
+  float ra = 0.0f, rb = 0.0f;
+#pragma unroll 4
+  for (; c < cols; c += kWideThreads) f(c, ra, rb);
+  return make_float2(warp_sum(a + ra), warp_sum(b + rb));
 }
 // Rows wider than the registers hold: three passes over a row, the second and
 // third mostly from cache.
@@ -629,11 +683,28 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   ring.bar = smem_addr(sh.bar);
   ring.stages = a.stages;
   const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  // Which of this block's rows is the last of all (-1: none): in a register where
+  // there is one to spare.
+  const int own_last =
+      blockIdx.x + (int64_t)(mine - 1) * gridDim.x == a.rows - 1 ? (int)(mine - 1) : -1;
+  auto last_row = [&] { return MODE == kOdd ? own_last : sh.last; };
+  auto is_edge = [&](int64_t k) { return (blockIdx.x | k) == 0 || k == last_row(); };
   auto issue = [&](int64_t k, uint32_t stage) {
     const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
     const int64_t row = blockIdx.x + k * gridDim.x;
     const T *rx = x + row * a.ldx, *rdy = dy + row * a.lddy;
     const T* rr = RES ? res + row * a.ldr : nullptr;
+    if (MODE != kWhole && is_edge(k)) {
+      const bool first = row == 0, last = k == last_row();
+      const Span sx = edge_span(rx, row_bytes, first, last),
+                 sdy = edge_span(rdy, row_bytes, first, last),
+                 sr = RES ? edge_span(rr, row_bytes, first, last) : Span{0u, 0u};
+      mbar_arrive_expect_tx(bar, sx.bytes + sdy.bytes + sr.bytes);
+      edge_load(dst, rx, sx, bar);
+      edge_load(dst + ring.slot_bytes, rdy, sdy, bar);
+      if constexpr (RES) edge_load(dst + 2 * ring.slot_bytes, rr, sr, bar);
+      return;
+    }
     mbar_arrive_expect_tx(bar, span_bytes<MODE>(rx, row_bytes) + span_bytes<MODE>(rdy, row_bytes) +
                                    (RES ? span_bytes<MODE>(rr, row_bytes) : 0u));
     span_load<MODE>(dst, rx, row_bytes, bar);
@@ -643,6 +714,7 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
+    sh.last = own_last;
     fence_barrier_init();
     for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
   }
@@ -665,6 +737,17 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
     if (k + 1 < mine) {
       next_mean = a.mean[row + gridDim.x];
       next_rstd = a.rstd[row + gridDim.x];
+    }
+    if (MODE != kWhole && is_edge(k)) {
+      const bool first = row == 0, last = k == last_row();
+      unsigned char* slot = smem + at.stage * ring.stage_bytes;
+      if (warp == 0) {
+        put_edges(slot, x + row * a.ldx, a.cols, first, last);
+        put_edges(slot + ring.slot_bytes, dy + row * a.lddy, a.cols, first, last);
+        if constexpr (RES)
+          put_edges(slot + 2 * ring.slot_bytes, res + row * a.ldr, a.cols, first, last);
+      }
+      __syncthreads();
     }
     float h[E], u[E], fr[RES ? E : 2];
     const bool ok = ring_wait(ring, at, &sh.abort_flag);

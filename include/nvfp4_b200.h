@@ -323,9 +323,9 @@ NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, co
  * x and y of dtype, gamma and beta (NULL: 0) of weight_dtype, which is dtype
  * or fp32.  mean and rstd (rows floats each) may be NULL.  amax_out as in
  * nvfp4_gemm, of y.  y may be x.  cols <= 2^24 (0: mean and rstd are left as they
- * are).  Around an
- * unaligned row the whole aligned 16-byte units are read; nothing outside the row
- * is used or written. */
+ * are).  Around unaligned rows the whole aligned 16-byte units are read, between
+ * the first row's start and the last row's end; nothing outside the rows is used
+ * or written. */
 NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int64_t ldx,
                                   const void* gamma, const void* beta, int dtype,
                                   int weight_dtype, float eps, void* y, int64_t ldy, float* mean,

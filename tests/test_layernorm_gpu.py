@@ -367,3 +367,25 @@ def test_unaligned_rows_with_16_bit_weights(nvlib, rows, cols, pad, dtype):
         close(got, want, ((rows + 64) * 2.0 ** -24 + 2.0 ** -22) * t.sum(0)
               + orc.half_step(gamma.dtype) * want.abs() + orc.least_step(gamma.dtype), "weights")
     assert nvlib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 2), (2, 3), (1, 7), (3, 8), (1, 9), (2, 15),
+                                       (1, 17), (2, 130), (1, 705), (3, 1023), (301, 709)])
+def test_ends_of_the_first_and_last_row(nvlib, rows, cols, dtype):
+    """Rows that start and end anywhere in 16 bytes, also both in the same: what lies
+    before the first and behind the last is not read (NaN there shows nowhere)."""
+    unit = 16 // TYPES[dtype].itemsize
+    for at in range(unit):
+        x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], torch.float32, 7 * cols + at)
+
+        def place(t, at):
+            flat = torch.full((rows * cols + 3 * unit,), math.nan, dtype=t.dtype, device="cuda")
+            v = flat[unit + at:unit + at + rows * cols].view(rows, cols)
+            v.copy_(t)
+            return v
+        px, pdy, pres = place(x, at), place(dy, (at * 3) % unit), place(res, (at * 5 + 1) % unit)
+        mean, rstd = check_forward(nvlib, x, gamma, beta, px)
+        check_backward(nvlib, x, gamma, dy, res, mean, rstd, (px, pdy, pres))
+        check_backward(nvlib, x, gamma, dy, None, mean, rstd, (px, place(dy, at), None))
+    assert nvlib.device_error() == 0
