@@ -716,6 +716,12 @@ int run(const Call& c) {
   if (!empty) {
     if (!c.a || !c.sfa || !c.b || !c.sfb || !c.amax_a || !c.amax_b || !c.d || (c.dact && !c.res))
       return NVFP4_ERR_INVALID_ARGUMENT;
+    auto partly = [&](const void* x, int64_t ldx, const void* y, int64_t ldy) {
+      return partly_over(x, ldx, y, ldy, c.m, c.n, (int64_t)es);
+    };
+    if (partly(c.d, c.ldd, c.res, c.ldr) || partly(c.aux, c.ldaux, c.res, c.ldr) ||
+        partly(c.d, c.ldd, c.aux, c.ldaux) || (c.aux && c.aux == c.d))
+      return NVFP4_ERR_INVALID_ARGUMENT;
     // amax_out is cleared before the operands' amax are read.
     if (c.amax_out && (c.amax_out == c.amax_a || c.amax_out == c.amax_b))
       return NVFP4_ERR_INVALID_ARGUMENT;

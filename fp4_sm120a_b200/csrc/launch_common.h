@@ -23,6 +23,24 @@ int device_sm_count(int* sms);
 int gemm_device_error(uint32_t* code, int clear);
 int layernorm_device_error(uint32_t* code, int clear);
 
+// Whether an output of m rows of n elements (strides lda, ldb) shares memory with
+// another matrix of the same sizes without being the same one: rows would be read
+// after others had been written over them.  Side by side in the same rows is no
+// overlap.
+inline bool partly_over(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m,
+                        int64_t n, int64_t elem) {
+  if (!a || !b || m < 1 || n < 1) return false;
+  if (a == b && (lda == ldb || m == 1)) return false;
+  using Wide = __int128;
+  const Wide a0 = (Wide)(uintptr_t)a, b0 = (Wide)(uintptr_t)b;
+  const Wide a1 = a0 + ((Wide)(m - 1) * lda + n) * elem, b1 = b0 + ((Wide)(m - 1) * ldb + n) * elem;
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (lda != ldb || (b0 - a0) % elem != 0) return true;
+  // Columns of b in a's rows.
+  const Wide c = (((b0 - a0) / elem) % lda + lda) % lda;
+  return c < n || c + n > lda;
+}
+
 // Allows KERNEL `bytes` of dynamic shared memory, once a device (asking again
 // for every launch costs about as much as the launch).
 template <auto KERNEL>

@@ -1136,6 +1136,7 @@ NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int
       (uintptr_t)mean % 4 || (uintptr_t)rstd % 4 || (uintptr_t)amax_out % 4)
     return NVFP4_ERR_MISALIGNED;
   if (empty && !amax_out) return NVFP4_OK;
+  if (partly_over(y, ldy, x, ldx, rows, cols, (int64_t)es)) return NVFP4_ERR_INVALID_ARGUMENT;
   int sms = 0;
   if (int e = device_sm_count(&sms)) return e;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1177,6 +1178,10 @@ NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, in
       (uintptr_t)gamma % ws || (uintptr_t)dgamma % ws || (uintptr_t)dbeta % ws ||
       (uintptr_t)mean % 4 || (uintptr_t)rstd % 4 || (uintptr_t)workspace % 4)
     return NVFP4_ERR_MISALIGNED;
+  if (partly_over(dx, lddx, dy, lddy, rows, cols, (int64_t)es) ||
+      partly_over(dx, lddx, residual, ldr, rows, cols, (int64_t)es) ||
+      partly_over(dx, lddx, x, ldx, rows, cols, (int64_t)es))
+    return NVFP4_ERR_INVALID_ARGUMENT;
   int sms = 0;
   if (int e = device_sm_count(&sms)) return e;
   cudaStream_t st = (cudaStream_t)stream;

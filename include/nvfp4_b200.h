@@ -285,8 +285,9 @@ enum { NVFP4_ACT_NONE = 0, NVFP4_ACT_RELU = 1, NVFP4_ACT_GELU = 2, NVFP4_ACT_SIL
  *   out_dtype   NVFP4_DTYPE_*: type of D, residual and aux
  *   ldd, ldr, ldaux   row strides in elements, >= n
  *   bias        n values of bias_dtype, or NULL
- *   residual    m x n, or NULL; may be D itself (accumulation in place)
- *   aux         receives z (what the backward pass needs), or NULL
+ *   residual    m x n, or NULL; may be D itself (accumulation in place), or lie
+ *               beside it in the same rows, but not partly over it
+ *   aux         receives z (what the backward pass needs), or NULL; not over D
  *   amax_out    receives max |D| as stored, NaN-propagating (what the cast of
  *               D needs), or NULL; not amax_a or amax_b
  *   workspace   scratch of nvfp4_gemm_workspace_bytes(m, n, k) bytes, 256-byte
@@ -322,10 +323,10 @@ NVFP4_API int nvfp4_gemm_dact(int64_t m, int64_t n, int64_t k, const void* A, co
  * elements): y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps).
  * x and y of dtype, gamma and beta (NULL: 0) of weight_dtype, which is dtype
  * or fp32.  mean and rstd (rows floats each) may be NULL.  amax_out as in
- * nvfp4_gemm, of y.  y may be x.  cols <= 2^24 (0: mean and rstd are left as they
- * are).  Around unaligned rows the whole aligned 16-byte units are read, between
- * the first row's start and the last row's end; nothing outside the rows is used
- * or written. */
+ * nvfp4_gemm, of y.  y may be x (or lie beside it in the same rows; not partly
+ * over it).  cols <= 2^24 (0: mean and rstd are left as they are).  Around
+ * unaligned rows the whole aligned 16-byte units are read, between the first row's
+ * start and the last row's end; nothing outside the rows is used or written. */
 NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int64_t ldx,
                                   const void* gamma, const void* beta, int dtype,
                                   int weight_dtype, float eps, void* y, int64_t ldy, float* mean,
@@ -335,7 +336,7 @@ NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int
  *   dx = rstd (u - mean(u) - h mean(u h)) + residual,  u = dy gamma, h = (x - mean) rstd
  *   dgamma = sum_rows dy h,  dbeta = sum_rows dy      (of weight_dtype, added in fp32)
  * residual (NULL: none) is the gradient that reaches x past the norm.  dx may
- * be dy or residual.  dgamma, dbeta may be NULL.  `workspace`: scratch of
+ * be dy or residual (not partly over an input).  dgamma, dbeta may be NULL.  `workspace`: scratch of
  * nvfp4_layernorm_bwd_workspace_bytes(rows, cols) bytes without initial or
  * kept state.  rows == 0 clears dgamma and dbeta.  Results repeat bit for bit. */
 NVFP4_API size_t nvfp4_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);

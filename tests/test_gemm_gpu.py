@@ -341,3 +341,21 @@ def test_repeats_and_sm_cap(nvlib, m, n, k):
                                    (2500, 2177, 96), (1030, 1800, 64), (130, 200, 4096)])
 def test_backward_epilogue_in_f16(nvlib, m, n, k, act):
     test_backward_epilogue(nvlib, m, n, k, "f16", act)
+
+
+@pytest.mark.parametrize("m", [5, 200, 2200])
+def test_matrices_side_by_side(nvlib, m):
+    """D, residual and aux in the same rows of one buffer are no overlap; a shifted
+    residual is one, and refused."""
+    n, k = 2192 if m == 2200 else 160, 160
+    a, b, z, tol = problem(m, n, k, 13)
+    buf = torch.randn(m, 3 * n, device="cuda")
+    d, res, other = buf[:, :n], buf[:, n:2 * n], buf[:, 2 * n:].clone()
+    before = res.double().cpu()
+    nvlib.matmul_nvfp4(*cuda(a), *cuda(b), residual=res, out=d)
+    want = z + before
+    close(d, want, tol + 2.0 ** -22 * (want.abs() + z.abs()), "d")
+    assert torch.equal(res.double().cpu(), before) and torch.equal(buf[:, 2 * n:], other)
+    for shifted in (buf[:, 1:n + 1], buf[:, n - 1:2 * n - 1]):
+        with pytest.raises(nvlib.NVFP4Error):
+            nvlib.matmul_nvfp4(*cuda(a), *cuda(b), residual=shifted, out=d)

@@ -279,3 +279,27 @@ def test_adamw_refuses_offsets_that_are_no_places(nvlib, offsets):
     lists = [a.pop(k) for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")]
     with pytest.raises(ValueError, match="offsets"):
         nvlib.AdamW(*lists, offsets=offsets, **a)
+
+
+@pytest.mark.parametrize("at,ldr", [(2, 64), (-2, 64), (128, 64), (62, 64), (66, 64), (0, 32),
+                                    (3 * 128 + 62, 32), (-2, 2**62)])
+def test_outputs_partly_over_their_inputs_are_refused(nvlib, at, ldr):
+    """4 x 32 values, rows 64 apart: an input may be the output itself, or lie beside
+    it in the same rows, but not shifted under it (rows read after others were written)."""
+    lib, R, far = nvlib.load(), 1 << 20, 1 << 30
+    over = R + at
+
+    def bwd(dy=far, lddy=32, res=None, ldr=32):
+        return lib.nvfp4_layernorm_bwd(4, 32, dy, lddy, 2 * far, 32, P, P, P, res, ldr, 1, 0, R, 64,
+                                       P, P, P, 1 << 20, None)
+    assert gemm(lib, m=4, n=32, D=R, ldd=64, res=over, ldr=ldr) == ARG
+    assert gemm(lib, m=4, n=32, D=R, ldd=64, aux=over, ldaux=ldr) == ARG
+    assert lib.nvfp4_gemm_dact(4, 32, 64, P, P, P, P, P, P, over, ldr, 2, R, 64, 1, None, None,
+                               None, 0, 0, None) == ARG
+    assert lib.nvfp4_layernorm_fwd(4, 32, over, ldr, P, P, 1, 0, 1e-5, R, 64, None, None, None,
+                                   None) == ARG
+    assert bwd(dy=over, lddy=ldr) == ARG and bwd(res=over, ldr=ldr) == ARG
+
+
+def test_two_outputs_in_one_place_are_refused(nvlib):
+    assert gemm(nvlib.load(), aux=P) == ARG
