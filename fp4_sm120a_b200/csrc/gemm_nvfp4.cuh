@@ -81,15 +81,18 @@ static inline int read_error_word(uint32_t* code, int clear) {
   return NVFP4_OK;
 }
 
+template <bool RELAXED = false>
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                      uint32_t err) {
-  return mbar_wait_bounded(bar, parity, abort_flag, kWaitLimitNs, err, &g_gemm_error_word);
+  return mbar_wait_bounded<RELAXED>(bar, parity, abort_flag, kWaitLimitNs, err,
+                                    &g_gemm_error_word);
 }
 
 // The same by a whole warp, which stays together.
+template <bool RELAXED = false>
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity,
                                           volatile uint32_t* abort_flag, uint32_t err) {
-  return __all_sync(0xFFFFFFFFu, wait(bar, parity, abort_flag, err));
+  return __all_sync(0xFFFFFFFFu, wait<RELAXED>(bar, parity, abort_flag, err));
 }
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
