@@ -558,8 +558,11 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
                         "grads[", i, "]: params[", i,
                         "].grad is another tensor now; pass the new gradients (grads=)");
   }
+  // Another thread may give the table other gradients while the interpreter is free.
+  const std::vector<nvfp4_adamw_tensor> rows = t.rows;
+  const std::vector<Held> grads = t.lists[kGrads];
   return result(launch(t.device, [&](nvfp4_stream_t stream) {
-    return nvfp4_adamw_step(t.rows.data(), (int)t.rows.size(), t.param, t.grad, t.state, lr,
+    return nvfp4_adamw_step(rows.data(), (int)rows.size(), t.param, t.grad, t.state, lr,
                             beta1, beta2, eps, step, scale, scalars, t.amax, t.rng, stream);
   }));
   END_HANDLE_TH_ERRORS

@@ -506,3 +506,32 @@ def test_8_bit_moments_of_all_types(nvlib, sizes, param, grad):
             want, _, wv = orc.adamw(p0, g, m0, v0, step=step, wd=wds[i], **H)
             check_param(dp[i], p0, g, m0, wv, step, want, copies, amax, i)
             at += -(-n // 128) * 128
+
+
+def test_two_threads_with_one_optimizer(nvlib):
+    """Steps of two threads on one stream, each with its own new gradients: every step
+    reads one thread's gradients whole (all ones or all twos; the first moment is
+    then the same in every element), and none that were freed."""
+    import threading
+    sizes = [64] * 200
+    ps = [torch.zeros(n, device="cuda") for n in sizes]
+    ms, vs = ([torch.zeros(n, device="cuda") for n in sizes] for _ in range(2))
+    opt = nvlib.AdamW(ps, [torch.zeros(n, device="cuda") for n in sizes], ms, vs)
+    errors = []
+
+    def work(value):
+        try:
+            for step in range(1, 40):
+                opt.step(step, lr=0.0, beta1=0.0, beta2=0.0,
+                         grads=[torch.full((n,), value, device="cuda") for n in sizes])
+        except Exception as e:                # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(v,)) for v in (1.0, 2.0)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    m = torch.cat(ms)
+    assert float(m[0]) in (1.0, 2.0) and bool((m == m[0]).all())
