@@ -344,12 +344,16 @@ struct Held {
   Tensor tensor;
   const void* data;
   int64_t n;
-  ScalarType type;
+  caffe2::TypeMeta dtype;
   explicit Held(const Tensor& t)
-      : tensor(t), data(t.data_ptr()), n(t.numel()), type(t.scalar_type()) {}
+      : tensor(t), data(t.data_ptr()), n(t.numel()), dtype(t.dtype()) {}
+  // (By the fields: the accessors' own checks are most of the time of a step of many
+  // short tensors.)
   bool same() const {
-    return tensor.const_data_ptr() == data && tensor.numel() == n &&
-           tensor.scalar_type() == type && tensor.is_contiguous();
+    const c10::TensorImpl& t = *tensor.unsafeGetTensorImpl();
+    const char* p = static_cast<const char*>(t.unsafe_storage().data());
+    return t.numel() == n && t.dtype() == dtype && t.is_contiguous() &&
+           (n == 0 || p + t.storage_offset() * (int64_t)dtype.itemsize() == data);
   }
 };
 
@@ -360,13 +364,21 @@ struct Range {
 };
 Range range_of(const Held& h, const char* name) {
   const uintptr_t p = (uintptr_t)h.data;
-  return {p, p + (uintptr_t)h.n * c10::elementSize(h.type), name};
+  return {p, p + (uintptr_t)h.n * h.dtype.itemsize(), name};
 }
+
+// The gradients, and the library's descriptors of all tensors with them.  Replaced as a
+// whole: another thread may pass new ones while a step's call runs.
+struct Rows {
+  std::vector<nvfp4_adamw_tensor> rows;
+  std::vector<Held> grads;
+};
 
 struct AdamWTable {
   int device = 0, param = 0, grad = 0, state = 0;
-  std::vector<nvfp4_adamw_tensor> rows;
-  std::vector<Held> lists[kLists];
+  size_t count = 0;
+  std::shared_ptr<const Rows> now;
+  std::vector<Held> lists[kLists];     // (kGrads: in `now`)
   std::vector<Held> words;             // amax_out, rng_state
   std::vector<Range> written;          // sorted; none overlaps the next
   std::vector<char> follows;           // grads[i] is params[i].grad
@@ -424,20 +436,17 @@ void apart(const std::vector<Range>& written, const Range& r) {
                     r.name, " and ", (next - 1)->name,
                     ": a tensor that the step reads overlaps one that it writes");
 }
-// Which gradients are their parameters' own .grad.
-void see_whose(AdamWTable& t) {
-  t.follows.resize(t.rows.size());
-  for (size_t i = 0; i < t.rows.size(); ++i) {
-    const Tensor& g = t.lists[kParams][i].tensor.unsafeGetTensorImpl()->grad();
-    t.follows[i] = g.defined() && g.is_same(t.lists[kGrads][i].tensor);
-  }
-}
-void put_grads(AdamWTable& t, std::vector<Held>&& grads) {
+// Takes the gradients (looked at by held), and sees which are their parameters' own
+// .grad.
+void put_grads(AdamWTable& t, std::vector<nvfp4_adamw_tensor> rows, std::vector<Held>&& grads) {
   for (const Held& g : grads) apart(t.written, range_of(g, kListName[kGrads]));
   on_device(grads, t.device, kListName[kGrads]);
-  t.lists[kGrads] = std::move(grads);
-  for (size_t i = 0; i < t.rows.size(); ++i) t.rows[i].grad = t.lists[kGrads][i].data;
-  see_whose(t);
+  for (size_t i = 0; i < t.count; ++i) {
+    rows[i].grad = grads[i].data;
+    const Tensor& own = t.lists[kParams][i].tensor.unsafeGetTensorImpl()->grad();
+    t.follows[i] = own.defined() && own.is_same(grads[i].tensor);
+  }
+  t.now = std::make_shared<const Rows>(Rows{std::move(rows), std::move(grads)});
 }
 
 // params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, copies,
@@ -461,15 +470,16 @@ PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   t->param = code_of(param, "params");
   t->grad = code_of(grad, "grads");
   t->state = state == kU8 ? NVFP4_STATE_8BIT : NVFP4_STATE_F32;
-  t->rows.resize(tensors);
+  t->count = (size_t)tensors;
+  t->follows.resize(t->count);
+  std::vector<nvfp4_adamw_tensor> rows(t->count);
   {
     THPObjectPtr fast(PySequence_Fast(o[kParams], "params"));
     if (!fast) throw python_error();
     for (Py_ssize_t i = 0; i < tensors; ++i)
-      t->rows[i].n =
-          (uint64_t)tensor(PySequence_Fast_GET_ITEM(fast.get(), i), "params").numel();
+      rows[i].n = (uint64_t)tensor(PySequence_Fast_GET_ITEM(fast.get(), i), "params").numel();
   }
-  auto size = [&](size_t i) { return (int64_t)t->rows[i].n; };
+  auto size = [&](size_t i) { return (int64_t)rows[i].n; };
   auto blocks = [&](size_t i) { return (size(i) + kStateBlock - 1) / kStateBlock; };
   t->lists[kParams] = held(o[kParams], tensors, param, kParams, size);
   std::vector<Held> grads = held(o[kGrads], tensors, grad, kGrads, size);
@@ -504,8 +514,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   THPObjectPtr offsets(o[8] == Py_None ? nullptr : PySequence_Fast(o[8], "offsets"));
   if ((o[7] != Py_None && !decays) || (o[8] != Py_None && !offsets)) throw python_error();
   uint64_t next = 0;
-  for (size_t i = 0; i < t->rows.size(); ++i) {
-    nvfp4_adamw_tensor& r = t->rows[i];
+  for (size_t i = 0; i < t->count; ++i) {
+    nvfp4_adamw_tensor& r = rows[i];
     auto at = [&](List list) -> void* {
       return t->lists[list].empty() ? nullptr : const_cast<void*>(t->lists[list][i].data);
     };
@@ -519,7 +529,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     r.offset = offsets ? (uint64_t)integer(PySequence_Fast_GET_ITEM(offsets.get(), i)) : next;
     next += (uint64_t)(blocks(i) * kStateBlock);
   }
-  put_grads(*t, std::move(grads));
+  put_grads(*t, std::move(rows), std::move(grads));
   PyObject* capsule = PyCapsule_New(t.get(), kTableName, [](PyObject* c) {
     delete static_cast<AdamWTable*>(PyCapsule_GetPointer(c, kTableName));
   });
@@ -542,28 +552,28 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
   if (scalars) apart(t.written, {(uintptr_t)scalars, (uintptr_t)(scalars + 3), "scalars"});
   for (const Held& w : t.words)
     TORCH_CHECK_VALUE(w.same(), "amax_out, rng_state: the tensor has other memory now");
-  for (int list = 0; list < kLists; ++list) {
-    if (list == kGrads && o[8] != Py_None) continue;
-    for (size_t i = 0; i < t.lists[list].size(); ++i)
-      TORCH_CHECK_VALUE(t.lists[list][i].same(), kListName[list], "[", i,
+  auto look = [](const std::vector<Held>& list, const char* name) {
+    for (size_t i = 0; i < list.size(); ++i)
+      TORCH_CHECK_VALUE(list[i].same(), name, "[", i,
                         "]: the tensor has other memory, size or type than when it was listed");
-  }
+  };
+  for (int list = 0; list < kLists; ++list) look(t.lists[list], kListName[list]);
   if (o[8] != Py_None) {
-    put_grads(t, held(o[8], t.rows.size(), type_of(t.grad), kGrads,
-                      [&](size_t i) { return (int64_t)t.rows[i].n; }));
+    const std::vector<nvfp4_adamw_tensor>& rows = t.now->rows;
+    put_grads(t, rows, held(o[8], t.count, type_of(t.grad), kGrads,
+                            [&](size_t i) { return (int64_t)rows[i].n; }));
   } else {
-    for (size_t i = 0; i < t.rows.size(); ++i)
+    look(t.now->grads, kListName[kGrads]);
+    for (size_t i = 0; i < t.count; ++i)
       TORCH_CHECK_VALUE(!t.follows[i] || t.lists[kParams][i].tensor.unsafeGetTensorImpl()
-                                             ->grad().is_same(t.lists[kGrads][i].tensor),
+                                             ->grad().is_same(t.now->grads[i].tensor),
                         "grads[", i, "]: params[", i,
                         "].grad is another tensor now; pass the new gradients (grads=)");
   }
-  // Another thread may give the table other gradients while the interpreter is free.
-  const std::vector<nvfp4_adamw_tensor> rows = t.rows;
-  const std::vector<Held> grads = t.lists[kGrads];
+  const std::shared_ptr<const Rows> now = t.now;
   return result(launch(t.device, [&](nvfp4_stream_t stream) {
-    return nvfp4_adamw_step(rows.data(), (int)rows.size(), t.param, t.grad, t.state, lr,
-                            beta1, beta2, eps, step, scale, scalars, t.amax, t.rng, stream);
+    return nvfp4_adamw_step(now->rows.data(), (int)t.count, t.param, t.grad, t.state, lr, beta1,
+                            beta2, eps, step, scale, scalars, t.amax, t.rng, stream);
   }));
   END_HANDLE_TH_ERRORS
 }
