@@ -39,6 +39,7 @@
 // TB/s), backward 189.
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -55,6 +56,8 @@ __device__ uint32_t g_layernorm_error_word;
 
 constexpr int kMaxStages = 8;
 constexpr size_t kRingBytes = 200 * 1024;      // of an SM, over its blocks
+constexpr size_t kSmBytes = 228 * 1024;        // of an SM
+constexpr size_t kBlockBytes = 2048;           // of a block beside its ring: 1 KB reserved, statics
 constexpr size_t kRingMost = 226 * 1024;       // dynamic shared memory a block may ask for
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr int kWideThreads = 256;
@@ -180,7 +183,30 @@ __device__ __forceinline__ void span_load(uint32_t slot, const void* row, uint32
 // Only the unit before the first row's start and the one behind the last row's end
 // reach outside the caller's rows.  Those two rows are edges: their copies leave such
 // units out (`lo`, `bytes`: of the row's whole units), and put_edges adds the elements
-// in them.
+// in them.  They are among the rows that a block asks for before its loop, which knows
+// nothing of them: the block of the last row takes its rows from there back (and the
+// host sees to it that it is not the first row's block too).  (Looked for row by row
+// instead: fp32 backward 10000 x 4097 124 us against 108.)
+template <int MODE>
+struct Order {
+  int start, step;
+  bool first, last;       // whether the block's first row is the first, the last of all
+  __device__ __forceinline__ Order(int64_t rows, int64_t mine)
+      : start((int)blockIdx.x), step((int)gridDim.x), first(blockIdx.x == 0), last(false) {
+    if constexpr (MODE != kWhole) {
+      last = start + (mine - 1) * step == rows - 1;
+      if (last) {
+        start = (int)(rows - 1);
+        step = -step;
+      }
+    }
+  }
+  template <typename I>
+  __device__ __forceinline__ int64_t row(I j) const {
+    if constexpr (MODE == kWhole) return blockIdx.x + (int64_t)j * gridDim.x;
+    return start + (int64_t)j * step;
+  }
+};
 struct Span {
   uint32_t lo, bytes;
 };
@@ -346,8 +372,7 @@ struct Shared {
   uint64_t bar[kMaxStages];
   float2 red[2][32];
   uint32_t abort_flag;
-  int last;               // which of this block's rows is the last of all (-1: none)
-  uint32_t pad[2];
+  uint32_t pad[3];
 };
 
 // Position of a row in the ring: its stage and the parity its barrier completes
@@ -406,32 +431,28 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   ring.bar = smem_addr(sh.bar);
   ring.stages = a.stages;
   const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
-  auto row_at = [&](int64_t k) { return (int64_t)blockIdx.x + k * gridDim.x; };
-  // Which of this block's rows is the last of all (-1: none): in a register where
-  // there is one to spare.
-  const int own_last =
-      blockIdx.x + (int64_t)(mine - 1) * gridDim.x == a.rows - 1 ? (int)(mine - 1) : -1;
-  auto last_row = [&] { return MODE == kOdd ? own_last : sh.last; };
-  auto is_edge = [&](int k) { return (blockIdx.x | k) == 0 || k == last_row(); };
-  auto issue = [&](int k, uint32_t stage) {
-    const T* row = x + row_at(k) * a.ldx;
-    const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
-    if (MODE != kWhole && is_edge(k)) {
-      const Span span = edge_span(row, row_bytes, (blockIdx.x | k) == 0, k == last_row());
-      mbar_arrive_expect_tx(bar, span.bytes);
-      edge_load(dst, row, span, bar);
-      return;
-    }
+  const Order<MODE> order(a.rows, mine);
+  auto issue = [&](int j, uint32_t stage) {
+    const T* row = x + order.row(j) * a.ldx;
+    const uint32_t bar = ring.bar + 8 * stage;
     mbar_arrive_expect_tx(bar, span_bytes<MODE>(row, row_bytes));
-    span_load<MODE>(dst, row, row_bytes, bar);
+    span_load<MODE>(ring.base + stage * ring.stage_bytes, row, row_bytes, bar);
   };
+  const bool edge = MODE != kWhole && (order.first || order.last);
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
-    sh.last = own_last;
     fence_barrier_init();
-    for (int k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
+    if (edge) {
+      const T* row = x + order.row(0) * a.ldx;
+      const Span span = edge_span(row, row_bytes, order.first, order.last);
+      mbar_arrive_expect_tx(ring.bar, span.bytes);
+      edge_load(ring.base, row, span, ring.bar);
+    }
+    for (int j = edge; j < ring.stages && j < mine; ++j) issue(j, (uint32_t)j);
   }
+  if (edge && warp == (nthr >> 5) - 1)
+    put_edges(smem, x + order.row(0) * a.ldx, a.cols, order.first, order.last);
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   const W* wb = reinterpret_cast<const W*>(a.beta);
   // Weights stay in registers while there is room for them.
@@ -465,13 +486,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   int k = 0;
   RingAt at;
   for (; k < mine; ++k, at.next(ring)) {
-    const int64_t row = row_at(k);
-    if (MODE != kWhole && is_edge(k)) {
-      const bool first = row == 0, last = k == last_row();
-      if (warp == 0)
-        put_edges(smem + at.stage * ring.stage_bytes, x + row * a.ldx, a.cols, first, last);
-      __syncthreads();
-    }
+    const int64_t row = order.row(k);
     float f[E];
     if (ring_wait(ring, at, &sh.abort_flag)) {
       fetch<T, MODE, ITEMS>(my, smem + at.stage * ring.stage_bytes, x + row * a.ldx, f);
@@ -659,7 +674,7 @@ struct BwdArgs {
 };
 
 template <typename T, typename W, int MODE, int ITEMS, int THREADS, bool RES>
-__global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) k_bwd_rows(const BwdArgs a) {
   // k_bwd_reduce may be scheduled; it waits for this kernel to complete.  (Only
   // when it follows: a caller's own programmatic dependent must not start this
   // early.)
@@ -682,41 +697,47 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   ring.base = smem_addr(smem);
   ring.bar = smem_addr(sh.bar);
   ring.stages = a.stages;
-  const int64_t mine = (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;
-  // Which of this block's rows is the last of all (-1: none): in a register where
-  // there is one to spare.
-  const int own_last =
-      blockIdx.x + (int64_t)(mine - 1) * gridDim.x == a.rows - 1 ? (int)(mine - 1) : -1;
-  auto last_row = [&] { return MODE == kOdd ? own_last : sh.last; };
-  auto is_edge = [&](int64_t k) { return (blockIdx.x | k) == 0 || k == last_row(); };
-  auto issue = [&](int64_t k, uint32_t stage) {
+  // 64 bits for whole rows, 32 for the others: what the compiler made the faster loop of
+  // (bf16 16384 x 5120 120 us against 124, 16000 x 1001 42.6 against 43.3).
+  using Index = std::conditional_t<MODE == kWhole, int64_t, int>;
+  const Index mine = (Index)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const Order<MODE> order(a.rows, mine);
+  auto issue = [&](Index j, uint32_t stage) {
     const uint32_t bar = ring.bar + 8 * stage, dst = ring.base + stage * ring.stage_bytes;
-    const int64_t row = blockIdx.x + k * gridDim.x;
+    const int64_t row = order.row(j);
     const T *rx = x + row * a.ldx, *rdy = dy + row * a.lddy;
     const T* rr = RES ? res + row * a.ldr : nullptr;
-    if (MODE != kWhole && is_edge(k)) {
-      const bool first = row == 0, last = k == last_row();
-      const Span sx = edge_span(rx, row_bytes, first, last),
-                 sdy = edge_span(rdy, row_bytes, first, last),
-                 sr = RES ? edge_span(rr, row_bytes, first, last) : Span{0u, 0u};
-      mbar_arrive_expect_tx(bar, sx.bytes + sdy.bytes + sr.bytes);
-      edge_load(dst, rx, sx, bar);
-      edge_load(dst + ring.slot_bytes, rdy, sdy, bar);
-      if constexpr (RES) edge_load(dst + 2 * ring.slot_bytes, rr, sr, bar);
-      return;
-    }
     mbar_arrive_expect_tx(bar, span_bytes<MODE>(rx, row_bytes) + span_bytes<MODE>(rdy, row_bytes) +
                                    (RES ? span_bytes<MODE>(rr, row_bytes) : 0u));
     span_load<MODE>(dst, rx, row_bytes, bar);
     span_load<MODE>(dst + ring.slot_bytes, rdy, row_bytes, bar);
     if constexpr (RES) span_load<MODE>(dst + 2 * ring.slot_bytes, rr, row_bytes, bar);
   };
+  const bool edge = MODE != kWhole && (order.first || order.last);
   if (tid == 0) {
     for (int s = 0; s < ring.stages; ++s) mbar_init(ring.bar + 8 * s, 1);
     sh.abort_flag = 0u;
-    sh.last = own_last;
     fence_barrier_init();
-    for (int64_t k = 0; k < ring.stages && k < mine; ++k) issue(k, (uint32_t)k);
+    if (edge) {
+      const int64_t row = order.row(0);
+      const T *rx = x + row * a.ldx, *rdy = dy + row * a.lddy;
+      const T* rr = RES ? res + row * a.ldr : nullptr;
+      const Span sx = edge_span(rx, row_bytes, order.first, order.last),
+                 sdy = edge_span(rdy, row_bytes, order.first, order.last),
+                 sr = RES ? edge_span(rr, row_bytes, order.first, order.last) : Span{0u, 0u};
+      mbar_arrive_expect_tx(ring.bar, sx.bytes + sdy.bytes + sr.bytes);
+      edge_load(ring.base, rx, sx, ring.bar);
+      edge_load(ring.base + ring.slot_bytes, rdy, sdy, ring.bar);
+      if constexpr (RES) edge_load(ring.base + 2 * ring.slot_bytes, rr, sr, ring.bar);
+    }
+    for (Index j = edge; j < ring.stages && j < mine; ++j) issue(j, (uint32_t)j);
+  }
+  if (edge && warp == (nthr >> 5) - 1) {
+    const int64_t row = order.row(0);
+    put_edges(smem, x + row * a.ldx, a.cols, order.first, order.last);
+    put_edges(smem + ring.slot_bytes, dy + row * a.lddy, a.cols, order.first, order.last);
+    if constexpr (RES)
+      put_edges(smem + 2 * ring.slot_bytes, res + row * a.ldr, a.cols, order.first, order.last);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   constexpr bool kKeep = E <= 16;      // gamma stays in registers
@@ -726,28 +747,18 @@ __global__ void __launch_bounds__(THREADS) k_bwd_rows(const BwdArgs a) {
   if constexpr (kKeep) fetch_weights<T, W, MODE, ITEMS>(my, wg, a.cols, gamma);
   __syncthreads();
   const float inv_n = 1.0f / (float)a.cols;
-  int64_t k = 0;
+  Index k = 0;
   RingAt at;
   // A row's statistics are fetched a row ahead.
-  float next_mean = mine > 0 ? a.mean[blockIdx.x] : 0.0f;
-  float next_rstd = mine > 0 ? a.rstd[blockIdx.x] : 0.0f;
+  float next_mean = a.mean[order.row(0)];
+  float next_rstd = a.rstd[order.row(0)];
   for (; k < mine; ++k, at.next(ring)) {
-    const int64_t row = blockIdx.x + k * gridDim.x;
+    const int64_t row = order.row(k);
     const float mean = next_mean, rstd = next_rstd;
     if (k + 1 < mine) {
-      next_mean = a.mean[row + gridDim.x];
-      next_rstd = a.rstd[row + gridDim.x];
-    }
-    if (MODE != kWhole && is_edge(k)) {
-      const bool first = row == 0, last = k == last_row();
-      unsigned char* slot = smem + at.stage * ring.stage_bytes;
-      if (warp == 0) {
-        put_edges(slot, x + row * a.ldx, a.cols, first, last);
-        put_edges(slot + ring.slot_bytes, dy + row * a.lddy, a.cols, first, last);
-        if constexpr (RES)
-          put_edges(slot + 2 * ring.slot_bytes, res + row * a.ldr, a.cols, first, last);
-      }
-      __syncthreads();
+      const int64_t next = order.row(k + 1);
+      next_mean = a.mean[next];
+      next_rstd = a.rstd[next];
     }
     float h[E], u[E], fr[RES ? E : 2];
     const bool ok = ring_wait(ring, at, &sh.abort_flag);
@@ -929,23 +940,39 @@ int blocks_of(int threads, int* blocks) {
 
 // Ring and grid of a launch: the SM's shared memory over the blocks that fit it
 // otherwise, two stages a block at least (fewer blocks then) while they fit.  A
-// block's rows, `grid` apart, start at the same phase of 16 bytes.
+// block's rows, `grid` apart, start at the same phase of 16 bytes.  Of unaligned rows
+// the first and the last are not one block's, unless it is the only row.  (There is
+// such a grid for all sizes that fit the memory: rows - 1 would have to be a multiple of
+// all grids down to 0, and the launch is refused then.)
+constexpr int kTooWide = -1;          // rows for the kernels of the widest
 struct Launch {
   int stages;
   size_t smem;
   unsigned grid;
 };
 Launch launch_shape(int blocks, size_t stage_bytes, int sms, int64_t rows, int64_t most,
-                    int phases) {
+                    int phases, bool unaligned) {
   Launch l;
   const size_t least = 2 * stage_bytes <= kRingMost ? 2 : 1;
-  while (blocks > 1 && kRingBytes / blocks < least * stage_bytes) --blocks;
-  const size_t fit = kRingBytes / blocks / stage_bytes;
+  // (Small rings: what the block holds beside them counts, or not all the blocks that
+  // the grid is made for run at once.)
+  auto room = [](int n) {
+    const size_t all = kSmBytes / n - kBlockBytes;
+    return all < kRingBytes / n ? all : kRingBytes / n;
+  };
+  while (blocks > 1 && room(blocks) < least * stage_bytes) --blocks;
+  const size_t fit = room(blocks) / stage_bytes;
   l.stages = (int)(fit < least ? least : fit > (size_t)kMaxStages ? kMaxStages : fit);
   l.smem = l.stages * stage_bytes;
   int64_t g = (int64_t)blocks * sms;
   if (g > most) g = most;
-  l.grid = (unsigned)(g < rows ? g - g % phases : rows);
+  if (g >= rows) {
+    g = rows;
+  } else {
+    g -= g % phases;
+    while (unaligned && g > 0 && (rows - 1) % g == 0) g -= phases;
+  }
+  l.grid = (unsigned)g;
   return l;
 }
 // Partial rows of the weights' gradients: enough blocks to fill the SMs, more
@@ -982,10 +1009,26 @@ int launch_fwd_rows(FwdArgs a, int threads, int sms, cudaStream_t st) {
   if (int e = blocks_of<kernel>(threads, &blocks)) return e;
   a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), MODE == kWhole);
   const Launch l = launch_shape(blocks, a.slot_bytes, sms, a.rows, INT32_MAX,
-                                phases_of(a.ldx * (int64_t)sizeof(T)));
+                                phases_of(a.ldx * (int64_t)sizeof(T)), MODE != kWhole);
   a.stages = l.stages;
   kernel<<<l.grid, threads, l.smem, st>>>(a);
   return cuda_status(cudaGetLastError());
+}
+
+template <typename T, typename W>
+int launch_fwd_unaligned(const FwdArgs& a, int sms, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.cols >= kPhasedCols && in_phase(a.x, a.ldx, a.y, a.ldy, sizeof(T))) {
+    const int64_t n = (a.cols + 2 * V - 2) / V;        // with the largest shift
+    if (int t = row_threads(n, 16 / V); t <= 512)
+      return launch_fwd_rows<T, W, kPhased, 16 / V, 512, 2>(a, t, sms, st);
+  }
+  // Element-wise addressing takes more registers: 80 at two blocks of 384.
+  if (a.cols <= 32 * 4) return launch_fwd_rows<T, W, kOdd, 4, 32, 16>(a, 32, sms, st);
+  const int t = row_threads(a.cols, 16);
+  if (t <= 384) return launch_fwd_rows<T, W, kOdd, 16, 384, 2>(a, t, sms, st);
+  if (t <= 512) return launch_fwd_rows<T, W, kOdd, 16, 512, 1>(a, t, sms, st);
+  return kTooWide;
 }
 
 template <typename T, typename W>
@@ -1002,17 +1045,8 @@ int launch_fwd(const FwdArgs& a, int sms, cudaStream_t st) {
       return launch_fwd_rows<T, W, kWhole, 16 / V, 512, 2>(a, t, sms, st);
     if (int t = row_threads(n, 32 / V); t <= 512)
       return launch_fwd_rows<T, W, kWhole, 32 / V, 512, 1>(a, t, sms, st);
-  } else {
-    if (a.cols >= kPhasedCols && in_phase(a.x, a.ldx, a.y, a.ldy, sizeof(T))) {
-      const int64_t n = (a.cols + 2 * V - 2) / V;        // with the largest shift
-      if (int t = row_threads(n, 16 / V); t <= 512)
-        return launch_fwd_rows<T, W, kPhased, 16 / V, 512, 2>(a, t, sms, st);
-    }
-    // Element-wise addressing takes more registers: 80 at two blocks of 384.
-    if (a.cols <= 32 * 4) return launch_fwd_rows<T, W, kOdd, 4, 32, 16>(a, 32, sms, st);
-    const int t = row_threads(a.cols, 16);
-    if (t <= 384) return launch_fwd_rows<T, W, kOdd, 16, 384, 2>(a, t, sms, st);
-    if (t <= 512) return launch_fwd_rows<T, W, kOdd, 16, 512, 1>(a, t, sms, st);
+  } else if (int e = launch_fwd_unaligned<T, W>(a, sms, st); e != kTooWide) {
+    return e;
   }
   const int64_t most = (int64_t)sms * 8;
   k_fwd_wide<T, W><<<(unsigned)(a.rows < most ? a.rows : most), kWideThreads, 0, st>>>(a);
@@ -1027,11 +1061,31 @@ int launch_bwd_rows(BwdArgs& a, int threads, int sms, cudaStream_t st) {
   a.slot_bytes = slot_of((size_t)a.cols * sizeof(T), MODE == kWhole);
   const Launch l = launch_shape(blocks, (RES ? 3 : 2) * (size_t)a.slot_bytes, sms, a.rows,
                                 most_partials(a.rows, a.cols),
-                                phases_of(a.ldx * (int64_t)sizeof(T)));
+                                phases_of(a.ldx * (int64_t)sizeof(T)), MODE != kWhole);
   a.stages = l.stages;
   a.partials = (int)l.grid;
   kernel<<<l.grid, threads, l.smem, st>>>(a);
   return cuda_status(cudaGetLastError());
+}
+
+template <typename T, typename W, bool RES>
+int launch_bwd_unaligned(BwdArgs& a, int sms, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.cols >= kPhasedCols && a.rows * a.cols >= kPhasedSize &&
+      in_phase(a.x, a.ldx, a.dy, a.lddy, sizeof(T)) &&
+      in_phase(a.x, a.ldx, a.dx, a.lddx, sizeof(T)) &&
+      (!RES || in_phase(a.x, a.ldx, a.res, a.ldr, sizeof(T)))) {
+    const int64_t n = (a.cols + 2 * V - 2) / V;
+    if (int t = row_threads(n, 8 / V); t <= 704)
+      return launch_bwd_rows<T, W, kPhased, 8 / V, 704, RES>(a, t, sms, st);
+    if (int t = row_threads(n, 16 / V); t <= 512)
+      return launch_bwd_rows<T, W, kPhased, 16 / V, 512, RES>(a, t, sms, st);
+  }
+  if (int t = row_threads(a.cols, 8); t <= 704)
+    return launch_bwd_rows<T, W, kOdd, 8, 704, RES>(a, t, sms, st);
+  if (int t = row_threads(a.cols, 16); t <= 512)
+    return launch_bwd_rows<T, W, kOdd, 16, 512, RES>(a, t, sms, st);
+  return kTooWide;
 }
 
 template <typename T, typename W, bool RES>
@@ -1052,21 +1106,8 @@ int launch_bwd(BwdArgs& a, int sms, cudaStream_t st) {
       return launch_bwd_rows<T, W, kWhole, 16 / V, 512, RES>(a, t, sms, st);
     if (int t = row_threads(n, 32 / V); t <= 512)
       return launch_bwd_rows<T, W, kWhole, 32 / V, 512, RES>(a, t, sms, st);
-  } else {
-    if (a.cols >= kPhasedCols && a.rows * a.cols >= kPhasedSize &&
-        in_phase(a.x, a.ldx, a.dy, a.lddy, sizeof(T)) &&
-        in_phase(a.x, a.ldx, a.dx, a.lddx, sizeof(T)) &&
-        (!RES || in_phase(a.x, a.ldx, a.res, a.ldr, sizeof(T)))) {
-      const int64_t n = (a.cols + 2 * V - 2) / V;
-      if (int t = row_threads(n, 8 / V); t <= 704)
-        return launch_bwd_rows<T, W, kPhased, 8 / V, 704, RES>(a, t, sms, st);
-      if (int t = row_threads(n, 16 / V); t <= 512)
-        return launch_bwd_rows<T, W, kPhased, 16 / V, 512, RES>(a, t, sms, st);
-    }
-    if (int t = row_threads(a.cols, 8); t <= 704)
-      return launch_bwd_rows<T, W, kOdd, 8, 704, RES>(a, t, sms, st);
-    if (int t = row_threads(a.cols, 16); t <= 512)
-      return launch_bwd_rows<T, W, kOdd, 16, 512, RES>(a, t, sms, st);
+  } else if (int e = launch_bwd_unaligned<T, W, RES>(a, sms, st); e != kTooWide) {
+    return e;
   }
   // The weights' partial sums first: dx may overwrite dy.
   a.partials = (int)most_partials(a.rows, a.cols);
