@@ -24,7 +24,7 @@
 // Each byte of the parameters, gradients and states moves once.  With fp32 moments
 // the step is bound by memory: 147 M parameters in 605 us (6.8 TB/s).  With 8-bit
 // moments it is bound by issue slots (72 % taken; some 75 instructions a parameter, of
-// which Philox and the rounding are most): 294 M parameters in 927 us (5.1 TB/s).
+// which Philox and the rounding are most): 294 M parameters in 880 us (5.3 TB/s).
 #include <cmath>
 #include <cstdint>
 #include <cuda_bf16.h>

@@ -28,7 +28,7 @@
 // Measured: 8192 x 14336 x 5120 230-237 us without an epilogue (5.1-5.2 PFLOP/s; k =
 // 20480: 5.7-6.1), 260-286 us with GELU, aux and amax; odd rows, 4099 x 14335 x 5120,
 // 150 us.  Those are bursts: in a stream of such calls the board reaches its power
-// limit, the clock falls below 1.5 GHz, and the same take 273 and 314-319 us.  A
+// limit, the clock falls below 1.5 GHz, and the same take 273 and 314-336 us.  A
 // 256 x 256 x 256 slice of a pair takes 0.415 us; its products and scale copies
 // alone 0.32, its loads alone 0.26.
 #include "gemm_nvfp4.cuh"

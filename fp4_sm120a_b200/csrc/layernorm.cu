@@ -17,8 +17,8 @@
 // registers and writes one partial row a block, which k_bwd_reduce sums in a
 // fixed order (no atomics: results repeat bit for bit).  Unaligned rows take the
 // same arithmetic with vectors that are partly the row's (kPhased) or element by
-// element (kOdd); rows wider than the registers hold are read again instead
-// (k_fwd_wide, k_bwd_wide).
+// element (kOdd); rows wider than the registers hold (16384 columns, unaligned 8192)
+// are read again instead (k_fwd_wide; k_bwd_wide_w and k_bwd_wide_dx).
 //
 // The statistics come from two passes over registers: each warp's mean, then
 // its sum of squares about that mean, and of what the first pass's rounding left
@@ -29,14 +29,17 @@
 // mean of a constant row is its value exactly: x - mean is zero there, which an
 // rstd of 1 / sqrt(eps) would otherwise blow up.
 //
-// Measured, bf16 with fp32 weights: forward with the amax 16384 x 8192 105 us (5.1
-// TB/s), 16384 x 5120 74 us; backward with a residual 16384 x 5120 122 us (5.5
-// TB/s), 16384 x 8192 171 us (6.3 TB/s), fp32 16384 x 4096 159 us (6.8 TB/s).  The
-// forward pass is bound by the latency of a row's two reductions at the 32 warps an
-// SM that the registers allow (issue slots 61 % taken), the backward pass by memory.
-// Unaligned rows: bf16 forward 8192 x 5121 66 us, backward 95; fp32 10000 x 5001 81 us
-// (5.0 TB/s) and 122 us (6.5 TB/s), backward 1003 x 4099 17 us.  Rows wider than the registers: bf16 forward 4096 x 16384 94 us (2.8
-// TB/s), backward 189.
+// Measured on the device, inputs from memory, fp32 weights: forward with the amax bf16
+// 16384 x 8192 103 us (5.2 TB/s), 16384 x 5120 74 us; backward with a residual 16384 x
+// 5120 121 us (5.5 TB/s), 16384 x 8192 171 us (6.3 TB/s), fp32 16384 x 4096 160 us (6.7
+// TB/s).  The forward pass is bound by issue slots (72 % taken) and the latency of a
+// row's two reductions at the 32 warps an SM that the registers allow, the backward pass
+// by memory.
+// Unaligned rows: bf16 8192 x 5121 forward 62 us, backward with a residual 91; fp32
+// 10000 x 5001 78 us (5.1 TB/s) and 128 us (6.2 TB/s); fp32 1003 x 4099 backward 20.5 us
+// (18.6 with the inputs in L2).  Weights that do not stay in registers: bf16 4096 x
+// 16384 forward 91 us (2.9 TB/s), backward 198.  Rows wider than the registers: bf16
+// 2048 x 18432 75-82 us and 240.
 #include <atomic>
 #include <cstdint>
 #include <type_traits>
@@ -992,11 +995,11 @@ bool in_phase(const void* x, int64_t ldx, const void* p, int64_t ld, int64_t es)
 }
 // Unaligned rows of at least so many columns, and in the backward pass of at
 // least so many elements, go by vectors with partial ends (kPhased); the others
-// element by element, which starts sooner.  Forward, bf16: 16000 x 1001 31 us against
-// 41, 4000 x 4099 29 against 43, 16000 x 777 30 against 37, but fp32 16000 x 501 25
-// against 23 and 16000 x 201 23 against 19.  Backward, bf16: 4000 x 4099 49 us against
-// 53, 16000 x 1001 44 against 46, but 1200 x 4099 22 against 21 and 4000 x 777 18
-// against 16.
+// element by element, which starts sooner.  Forward, bf16: 16000 x 1001 32 us against
+// 41, 4000 x 4099 31 against 47, 16000 x 777 32 against 38, but fp32 16000 x 501 29
+// against 26 and 16000 x 201 25 against 23.  Backward with a residual, bf16: 4000 x
+// 4099 50 us against 55, 16000 x 1001 45 against 49, but 1200 x 4099 24.7 against 24.2
+// and 4000 x 777 20 against 19.
 constexpr int64_t kPhasedCols = 700, kPhasedSize = 1 << 23;
 uint32_t slot_of(size_t row_bytes, bool aligned) {
   return (uint32_t)(aligned ? row_bytes : (row_bytes + 15) / 16 * 16 + 16);

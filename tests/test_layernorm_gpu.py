@@ -389,3 +389,21 @@ def test_ends_of_the_first_and_last_row(nvlib, rows, cols, dtype):
         check_backward(nvlib, x, gamma, dy, res, mean, rstd, (px, pdy, pres))
         check_backward(nvlib, x, gamma, dy, None, mean, rstd, (px, place(dy, at), None))
     assert nvlib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(149, 5003), (297, 4099), (297, 709), (1185, 131), (4737, 33)])
+def test_ends_where_a_grid_would_give_them_to_one_block(nvlib, rows, cols, dtype):
+    """One row more than a multiple of the blocks that fill 148 SMs."""
+    x, gamma, beta, dy, res = make(rows, cols, TYPES[dtype], torch.float32, rows)
+
+    def place(t, at):
+        flat = torch.full((rows * cols + 48,), math.nan, dtype=t.dtype, device="cuda")
+        v = flat[16 + at:16 + at + rows * cols].view(rows, cols)
+        v.copy_(t)
+        return v
+    for places in ((1, 1, 1), (3, 1, 2)):
+        px, pdy, pres = (place(t, at) for t, at in zip((x, dy, res), places))
+        mean, rstd = check_forward(nvlib, x, gamma, beta, px)
+        check_backward(nvlib, x, gamma, dy, res, mean, rstd, (px, pdy, pres))
+    assert nvlib.device_error() == 0
