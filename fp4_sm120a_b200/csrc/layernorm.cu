@@ -237,6 +237,7 @@ __device__ __forceinline__ void put_edges(unsigned char* slot, const T* row, int
   const int tail = last ? min((lead + cols) % kUnit, cols) : 0;
   const int l = lane & 15, c = lane < 16 ? l : cols - tail + l;
   if (l < (lane < 16 ? head : tail)) reinterpret_cast<T*>(slot)[lead + c] = row[c];
+  fence_proxy_async_smem();       // a later copy writes these bytes
 }
 // A thread's items (vectors or elements) within the row: the first `count`.
 template <typename T, int MODE, int ITEMS>

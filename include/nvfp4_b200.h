@@ -295,8 +295,9 @@ enum { NVFP4_ACT_NONE = 0, NVFP4_ACT_RELU = 1, NVFP4_ACT_GELU = 2, NVFP4_ACT_SIL
  *               keeps none, but no two calls may use it at the same time
  *   sm_count    0: all SMs; else a cap on the persistent grid (a call short
  *               enough to split k over a cluster takes its own grid)
- * Accumulates in fp32; each output is rounded once.  The same call gives the
- * same bits.  k % 32 == 0 and k > 0; A and B 16-byte aligned; m, n any size (0: a
+ * Accumulates in fp32; each output is rounded once.  (The two operands' scales are
+ * multiplied in fp32: where amax_a amax_b is below 2^-103, D loses digits.)  The same
+ * call gives the same bits.  k % 32 == 0 and k > 0; A and B 16-byte aligned; m, n any size (0: a
  * no-op but for *amax_out = 0); m, n, k <= 2^30. */
 NVFP4_API size_t nvfp4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 NVFP4_API int nvfp4_gemm(int64_t m, int64_t n, int64_t k, const void* A, const void* SFA,
@@ -338,7 +339,8 @@ NVFP4_API int nvfp4_layernorm_fwd(int64_t rows, int64_t cols, const void* x, int
  * residual (NULL: none) is the gradient that reaches x past the norm.  dx may
  * be dy or residual (not partly over an input).  dgamma, dbeta may be NULL.  `workspace`: scratch of
  * nvfp4_layernorm_bwd_workspace_bytes(rows, cols) bytes without initial or
- * kept state.  rows == 0 clears dgamma and dbeta.  Results repeat bit for bit. */
+ * kept state.  rows == 0 clears dgamma and dbeta.  Unaligned rows are read as in the
+ * forward call.  Results repeat bit for bit. */
 NVFP4_API size_t nvfp4_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
 NVFP4_API int nvfp4_layernorm_bwd(int64_t rows, int64_t cols, const void* dy, int64_t lddy,
                                   const void* x, int64_t ldx, const float* mean,
