@@ -35,8 +35,8 @@
 // TB/s).  The forward pass is bound by issue slots (72 % taken) and the latency of a
 // row's two reductions at the 32 warps an SM that the registers allow, the backward pass
 // by memory.
-// Unaligned rows: bf16 8192 x 5121 forward 62 us, backward with a residual 91; fp32
-// 10000 x 5001 78 us (5.1 TB/s) and 128 us (6.2 TB/s); fp32 1003 x 4099 backward 20.5 us
+// Unaligned rows: bf16 8192 x 5121 forward 60 us, backward with a residual 93; fp32
+// 10000 x 5001 76 us (5.3 TB/s) and 123 us (6.5 TB/s); fp32 1003 x 4099 backward 20.8 us
 // (18.6 with the inputs in L2).  Weights that do not stay in registers: bf16 4096 x
 // 16384 forward 91 us (2.9 TB/s), backward 198.  Rows wider than the registers: bf16
 // 2048 x 18432 75-82 us and 240.
@@ -186,28 +186,29 @@ __device__ __forceinline__ void span_load(uint32_t slot, const void* row, uint32
 // Only the unit before the first row's start and the one behind the last row's end
 // reach outside the caller's rows.  Those two rows are edges: their copies leave such
 // units out (`lo`, `bytes`: of the row's whole units), and put_edges adds the elements
-// in them.  They are among the rows that a block asks for before its loop, which knows
-// nothing of them: the block of the last row takes its rows from there back (and the
+// in them.  They are the rows that a block asks for first, before its loop, which knows
+// nothing of them: the block of the last row takes that one before its others (and the
 // host sees to it that it is not the first row's block too).  (Looked for row by row
-// instead: fp32 backward 10000 x 4097 124 us against 108.)
+// instead: fp32 backward 10000 x 4097 124 us against 103.  That block's rows all
+// backwards: 108; it then reads far from the others all the time.)
 template <int MODE>
 struct Order {
-  int start, step;
-  bool first, last;       // whether the block's first row is the first, the last of all
+  int start, base;        // the block's first row, and the others less j * gridDim.x
+  bool first, last;       // whether that row is the first, the last of all
   __device__ __forceinline__ Order(int64_t rows, int64_t mine)
-      : start((int)blockIdx.x), step((int)gridDim.x), first(blockIdx.x == 0), last(false) {
+      : start((int)blockIdx.x), base((int)blockIdx.x), first(blockIdx.x == 0), last(false) {
     if constexpr (MODE != kWhole) {
-      last = start + (mine - 1) * step == rows - 1;
+      last = start + (mine - 1) * gridDim.x == rows - 1;
       if (last) {
         start = (int)(rows - 1);
-        step = -step;
+        base -= (int)gridDim.x;
       }
     }
   }
   template <typename I>
   __device__ __forceinline__ int64_t row(I j) const {
     if constexpr (MODE == kWhole) return blockIdx.x + (int64_t)j * gridDim.x;
-    return start + (int64_t)j * step;
+    return j == 0 ? start : base + (int64_t)j * gridDim.x;
   }
 };
 struct Span {
