@@ -185,8 +185,8 @@ __device__ __forceinline__ void span_load(uint32_t slot, const void* row, uint32
 }
 // Only the unit before the first row's start and the one behind the last row's end
 // reach outside the caller's rows.  Those two rows are edges: their copies leave such
-// units out (`lo`, `bytes`: of the row's whole units), and put_edges adds the elements
-// in them.  They are the rows that a block asks for first, before its loop, which knows
+// units out (`lo`, `bytes`: of the row's whole units), and EdgeElement adds the
+// elements in them.  They are the rows that a block asks for first, before its loop, which knows
 // nothing of them: the block of the last row takes that one before its others (and the
 // host sees to it that it is not the first row's block too).  (Looked for row by row
 // instead: fp32 backward 10000 x 4097 124 us against 103.  That block's rows all
@@ -227,19 +227,28 @@ __device__ __forceinline__ void edge_load(uint32_t slot, const void* row, const 
               reinterpret_cast<const unsigned char*>((uintptr_t)row & ~(uintptr_t)15) + s.lo,
               s.bytes, bar);
 }
-// The elements that an edge's copy leaves out, by the lanes of a warp, into the slot
-// whose other bytes the copy fills.
+// The elements that an edge's copy leaves out, one a lane of a warp: asked for before
+// the weights, put into the slot (whose other bytes the copy fills) after them, so that
+// one latency serves all.
 template <typename T>
-__device__ __forceinline__ void put_edges(unsigned char* slot, const T* row, int cols, bool first,
-                                          bool last) {
-  constexpr int kUnit = 16 / (int)sizeof(T);
-  const int lead = (int)((uintptr_t)row & 15u) / (int)sizeof(T), lane = (int)threadIdx.x & 31;
-  const int head = first && lead ? min(kUnit - lead, cols) : 0;
-  const int tail = last ? min((lead + cols) % kUnit, cols) : 0;
-  const int l = lane & 15, c = lane < 16 ? l : cols - tail + l;
-  if (l < (lane < 16 ? head : tail)) reinterpret_cast<T*>(slot)[lead + c] = row[c];
-  fence_proxy_async_smem();       // a later copy writes these bytes
-}
+struct EdgeElement {
+  T value;
+  int at = -1;              // place in the slot, -1: none
+  __device__ __forceinline__ void load(const T* row, int cols, bool first, bool last) {
+    constexpr int kUnit = 16 / (int)sizeof(T);
+    const int lead = (int)((uintptr_t)row & 15u) / (int)sizeof(T), lane = (int)threadIdx.x & 31;
+    const int head = first && lead ? min(kUnit - lead, cols) : 0;
+    const int tail = last ? min((lead + cols) % kUnit, cols) : 0;
+    const int l = lane & 15, c = lane < 16 ? l : cols - tail + l;
+    if (l < (lane < 16 ? head : tail)) {
+      value = row[c];
+      at = lead + c;
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* slot) const {
+    if (at >= 0) reinterpret_cast<T*>(slot)[at] = value;
+  }
+};
 // A thread's items (vectors or elements) within the row: the first `count`.
 template <typename T, int MODE, int ITEMS>
 struct Mine {
@@ -456,8 +465,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
     }
     for (int j = edge; j < ring.stages && j < mine; ++j) issue(j, (uint32_t)j);
   }
-  if (edge && warp == (nthr >> 5) - 1)
-    put_edges(smem, x + order.row(0) * a.ldx, a.cols, order.first, order.last);
+  const bool edge_warp = edge && warp == (nthr >> 5) - 1;
+  EdgeElement<T> ex;
+  if (edge_warp) ex.load(x + order.row(0) * a.ldx, a.cols, order.first, order.last);
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   const W* wb = reinterpret_cast<const W*>(a.beta);
   // Weights stay in registers while there is room for them.
@@ -467,6 +477,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) k_fwd_rows(const FwdArgs a) {
   if constexpr (kKeep) {
     fetch_weights<T, W, MODE, ITEMS>(my, wg, a.cols, gamma);
     fetch_weights<T, W, MODE, ITEMS>(my, wb, a.cols, beta);
+  }
+  if (edge_warp) {
+    ex.store(smem);
+    if (mine > ring.stages) fence_proxy_async_smem();   // a later copy writes these bytes
   }
   static_assert(THREADS <= 512, "a half warp joins all warps");
   const int share = lane & 15;        // the warp whose sums this lane joins
@@ -737,12 +751,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_bwd_rows(const BwdArgs a) {
     }
     for (Index j = edge; j < ring.stages && j < mine; ++j) issue(j, (uint32_t)j);
   }
-  if (edge && warp == (nthr >> 5) - 1) {
+  const bool edge_warp = edge && warp == (nthr >> 5) - 1;
+  EdgeElement<T> ex, edy, er;
+  if (edge_warp) {
     const int64_t row = order.row(0);
-    put_edges(smem, x + row * a.ldx, a.cols, order.first, order.last);
-    put_edges(smem + ring.slot_bytes, dy + row * a.lddy, a.cols, order.first, order.last);
-    if constexpr (RES)
-      put_edges(smem + 2 * ring.slot_bytes, res + row * a.ldr, a.cols, order.first, order.last);
+    ex.load(x + row * a.ldx, a.cols, order.first, order.last);
+    edy.load(dy + row * a.lddy, a.cols, order.first, order.last);
+    if constexpr (RES) er.load(res + row * a.ldr, a.cols, order.first, order.last);
   }
   const W* wg = reinterpret_cast<const W*>(a.gamma);
   constexpr bool kKeep = E <= 16;      // gamma stays in registers
@@ -750,6 +765,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_bwd_rows(const BwdArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) dg[e] = db[e] = 0.0f;
   if constexpr (kKeep) fetch_weights<T, W, MODE, ITEMS>(my, wg, a.cols, gamma);
+  if (edge_warp) {
+    ex.store(smem);
+    edy.store(smem + ring.slot_bytes);
+    if constexpr (RES) er.store(smem + 2 * ring.slot_bytes);
+    if (mine > ring.stages) fence_proxy_async_smem();   // later copies write these bytes
+  }
   __syncthreads();
   const float inv_n = 1.0f / (float)a.cols;
   Index k = 0;
